@@ -1,0 +1,505 @@
+// holoscene_amd/csrc/embed_rows.hip -- learned codes looked up by index (gfx950):
+//     out_i = scale * table[idx_i],          d table_v = scale * sum over {i : idx_i = v} of g_i.
+// An index outside [0, V) reads a row of zeros and takes no gradient (as a point outside the hash grid's cube does), so no launch reads or writes
+// outside the table whatever the indices hold; `padding` (or -1) is looked up like any other row and takes no gradient.
+//
+// The gradient sums each row's run in the order of the positions, so it is the same from run to run: (index, position) pairs are sorted by
+// index with a stable counting sort, and the table's gradient is then written row by row, once, zeros included -- no fill, no atomics on it.
+//   sort    N <= 16 384: one workgroup, the pairs in registers, one pass per <= 8 bits of the index through LDS (one launch);
+//           longer: passes of <= 11 bits, two launches each (block histograms; ranks, every workgroup adding up the histograms itself).
+//   chunks  sorted positions in chunks of 64: a chunk that lies inside one run is summed to fp32 partials (a run of one index may be the whole batch).
+//   rows    bounds of a row's run by bisection in the sorted indices; head and tail of the run from g, its whole chunks from the partials.
+//           Short runs: a wave per row.  Long ones: all four waves of the workgroup on one row, joined through LDS in a fixed order.
+// fp32 sums: 64 terms per chunk, then the partials; the last operation rounds to the table's type.
+#include "holoscene_hip.h"
+#include "launch_util.h"
+#include "row_types.h"
+
+namespace {
+
+using namespace hs_row;
+
+// ------------------------------------------------------------------------------------------------ lookup
+// one thread per VEC elements of the output; `per_row` = D / VEC
+template <typename T, typename O, typename I, int VEC>
+__global__ __launch_bounds__(256) void k_embed_fwd(const I *__restrict__ idx, const T *__restrict__ table, int64_t ld, O *__restrict__ out, int64_t total,
+                                                   uint32_t per_row, int64_t V, float scale) {
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (id >= total) return;
+    int64_t row;
+    uint32_t c;
+    if (total <= 0xffffffffll) {        // (uniform: a 32-bit division is a tenth of the 64-bit one)
+        row = (uint32_t)id / per_row;
+        c = (uint32_t)id - (uint32_t)row * per_row;
+    } else {
+        row = id / per_row;
+        c = (uint32_t)(id - row * per_row);
+    }
+    const int64_t v = (int64_t)idx[row];
+    Pack<O, VEC> o;
+    if (v >= 0 && v < V) {
+        const Pack<T, VEC> t = *reinterpret_cast<const Pack<T, VEC> *>(table + v * ld + (int64_t)c * VEC);
+#pragma unroll
+        for (int e = 0; e < VEC; e++) o.v[e] = from_f32<O>(to_f32(t.v[e]) * scale);
+    } else {
+#pragma unroll
+        for (int e = 0; e < VEC; e++) o.v[e] = from_f32<O>(0.f);
+    }
+    *reinterpret_cast<Pack<O, VEC> *>(out + id * VEC) = o;
+}
+
+// ------------------------------------------------------------------------------------------------ sort
+// Keys: the index where it takes a gradient, V otherwise (sorted behind every row).
+template <typename I> __device__ __forceinline__ uint32_t sort_key(const I *__restrict__ idx, int64_t i, int64_t V, int64_t padding) {
+    const int64_t v = (int64_t)idx[i];
+    return v >= 0 && v < V && v != padding ? (uint32_t)v : (uint32_t)V;
+}
+
+constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
+constexpr int kTile = 4096;                         // pairs per tile of the multi-block sort: 4 per thread
+constexpr int kOneMax = 16384, kOneDigit = 8;       // the one-workgroup sort
+constexpr int kMultiDigit = 11;
+constexpr int kMaxBlocks = 64;                      // workgroups of the multi-block sort (each adds up all their histograms)
+
+// Lanes of this wave whose digit equals mine, among those with `on`.
+__device__ __forceinline__ uint64_t same_digit(uint32_t digit, int bits, bool on) {
+    uint64_t m = __ballot(on);
+    for (int b = 0; b < bits; b++) {
+        const uint64_t set = __ballot((digit >> b) & 1u);
+        m &= ((digit >> b) & 1u) ? set : ~set;
+    }
+    return m;
+}
+
+// Ranks of a tile's pairs among those of equal digit in front of them.  Wave w holds pairs [w * 64 * R, (w + 1) * 64 * R) of the tile, round r lane l
+// the pair 64 r + l of them.  cnt [waves][bins] must be zero; afterwards it holds, per wave and digit, the pairs of that digit in earlier waves
+// of the tile, and tile_total[digit] (may alias nothing) the tile's count.
+template <int R> __device__ __forceinline__ void tile_ranks(const uint32_t (&digit)[R], const bool (&on)[R], uint32_t (&rank)[R], int bits, int bins, uint16_t *cnt,
+                                                            uint32_t *tile_total) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    uint16_t *mine = cnt + wave * bins;
+    const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const uint64_t peers = same_digit(digit[r], bits, on[r]);
+        uint32_t base = 0;
+        if (on[r]) {
+            base = mine[digit[r]];
+            rank[r] = base + __popcll(peers & below);
+        }
+        __builtin_amdgcn_wave_barrier();            // (a wave's LDS operations complete in order: every read above precedes the write below)
+        if (on[r] && (peers & below) == 0) mine[digit[r]] = (uint16_t)(base + __popcll(peers));
+        __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+    for (int d = tid; d < bins; d += kSortThreads) {
+        uint32_t sum = 0;
+#pragma unroll
+        for (int w = 0; w < kSortWaves; w++) {
+            const uint32_t c = cnt[w * bins + d];
+            cnt[w * bins + d] = (uint16_t)sum;
+            sum += c;
+        }
+        tile_total[d] = sum;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; r++)
+        if (on[r]) rank[r] += mine[digit[r]];
+}
+
+// exclusive scan of v[0, n) in place by the whole workgroup; n <= 2 * kSortThreads
+__device__ __forceinline__ void scan_exclusive(uint32_t *v, int n, uint32_t *wave_sums) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint32_t a = 2 * tid < n ? v[2 * tid] : 0, b = 2 * tid + 1 < n ? v[2 * tid + 1] : 0;
+    uint32_t s = a + b;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const uint32_t t = __shfl_up(s, off);
+        if (lane >= off) s += t;
+    }
+    if (lane == 63) wave_sums[wave] = s;
+    __syncthreads();
+    uint32_t before = 0;
+    for (int w = 0; w < wave; w++) before += wave_sums[w];
+    const uint32_t ex = before + s - (a + b);
+    if (2 * tid < n) v[2 * tid] = ex;
+    if (2 * tid + 1 < n) v[2 * tid + 1] = ex + a;
+    __syncthreads();
+}
+
+// All of it in one workgroup: R = pairs per thread (N <= 1024 R), `passes` passes of <= 8 bits, the pairs through LDS between passes.
+template <typename I, int R>
+__global__ __launch_bounds__(kSortThreads) void k_sort_one(const I *__restrict__ idx, int n, int64_t V, int64_t padding, int bits, int passes, uint32_t *__restrict__ keys,
+                                                           uint32_t *__restrict__ pos) {
+    extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
+    uint32_t *total = lds, *wave_sums = lds + 256;
+    uint16_t *cnt = reinterpret_cast<uint16_t *>(lds + 256 + kSortWaves);
+    uint32_t *lk = lds + 256 + kSortWaves + kSortWaves * 256 / 2, *lp = lk + 1024 * R;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    uint32_t key[R], at[R], digit[R], rank[R];
+    bool on[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const int i = (wave * R + r) * 64 + lane;
+        on[r] = i < n;
+        key[r] = on[r] ? sort_key(idx, i, V, padding) : 0;
+        at[r] = (uint32_t)i;
+    }
+    int shift = 0;
+    for (int p = 0; p < passes; p++) {
+        const int nb = (bits - shift + passes - p - 1) / (passes - p), bins = 1 << nb;
+        for (int i = tid; i < kSortWaves * bins / 2; i += kSortThreads) reinterpret_cast<uint32_t *>(cnt)[i] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < R; r++) digit[r] = (key[r] >> shift) & (uint32_t)(bins - 1);
+        tile_ranks<R>(digit, on, rank, nb, bins, cnt, total);
+        __syncthreads();
+        scan_exclusive(total, bins, wave_sums);
+        const bool last = p + 1 == passes;
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            if (!on[r]) continue;
+            const uint32_t to = total[digit[r]] + rank[r];
+            (last ? keys : lk)[to] = key[r];
+            (last ? pos : lp)[to] = at[r];
+        }
+        __syncthreads();
+        if (!last) {
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                const int i = (wave * R + r) * 64 + lane;
+                if (on[r]) { key[r] = lk[i]; at[r] = lp[i]; }
+            }
+        }
+        shift += nb;
+    }
+}
+
+// Multi-block, first launch of a pass: hist[block][digit] over the block's `per` pairs.  keys_in == NULL: the first pass, from the indices.
+template <typename I>
+__global__ __launch_bounds__(kSortThreads) void k_sort_hist(const I *__restrict__ idx, const uint32_t *__restrict__ keys_in, int64_t n, int64_t per, int64_t V, int64_t padding,
+                                                            int shift, int nb, uint32_t *__restrict__ hist) {
+    __shared__ uint32_t h[1 << kMultiDigit];
+    const int tid = threadIdx.x, bins = 1 << nb;
+    for (int d = tid; d < bins; d += kSortThreads) h[d] = 0;
+    __syncthreads();
+    const int64_t begin = blockIdx.x * per, end = begin + per < n ? begin + per : n;
+    for (int64_t i = begin + tid; i < end; i += kSortThreads) {
+        const uint32_t k = keys_in ? keys_in[i] : sort_key(idx, i, V, padding);
+        atomicAdd(&h[(k >> shift) & (uint32_t)(bins - 1)], 1u);        // (counts only: their order does not matter)
+    }
+    __syncthreads();
+    for (int d = tid; d < bins; d += kSortThreads) hist[(size_t)blockIdx.x * bins + d] = h[d];
+}
+
+// second launch: ranks.  A workgroup's first place for a digit = all pairs of smaller digits + the pairs of this digit in earlier workgroups.
+template <typename I>
+__global__ __launch_bounds__(kSortThreads) void k_sort_scatter(const I *__restrict__ idx, const uint32_t *__restrict__ keys_in, const uint32_t *__restrict__ pos_in, int64_t n,
+                                                               int64_t per, int64_t V, int64_t padding, int shift, int nb, const uint32_t *__restrict__ hist,
+                                                               uint32_t *__restrict__ keys, uint32_t *__restrict__ pos) {
+    constexpr int R = kTile / kSortThreads;
+    extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
+    const int bins = 1 << nb, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    uint32_t *place = lds, *tile_total = lds + bins, *wave_sums = lds + 2 * bins;
+    uint16_t *cnt = reinterpret_cast<uint16_t *>(wave_sums + kSortWaves);
+    uint32_t before[2] = {0, 0};
+#pragma unroll
+    for (int q = 0; q < 2; q++) {
+        const int d = 2 * tid + q;          // (the layout scan_exclusive works on: the pair 2 tid, 2 tid + 1 stays with the thread)
+        if (d >= bins) continue;
+        uint32_t all = 0;
+        for (int b = 0; b < (int)gridDim.x; b++) {
+            const uint32_t c = hist[(size_t)b * bins + d];
+            if (b < (int)blockIdx.x) before[q] += c;
+            all += c;
+        }
+        place[d] = all;
+    }
+    __syncthreads();
+    scan_exclusive(place, bins, wave_sums);
+#pragma unroll
+    for (int q = 0; q < 2; q++)
+        if (2 * tid + q < bins) place[2 * tid + q] += before[q];
+    const int64_t begin = blockIdx.x * per, end = begin + per < n ? begin + per : n;
+    for (int64_t t0 = begin; t0 < end; t0 += kTile) {
+        for (int i = tid; i < kSortWaves * bins; i += kSortThreads) cnt[i] = 0;
+        uint32_t key[R], at[R], digit[R], rank[R];
+        bool on[R];
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const int64_t i = t0 + (wave * R + r) * 64 + lane;
+            on[r] = i < end;
+            key[r] = on[r] ? (keys_in ? keys_in[i] : sort_key(idx, i, V, padding)) : 0;
+            at[r] = on[r] && pos_in ? pos_in[i] : (uint32_t)i;
+            digit[r] = (key[r] >> shift) & (uint32_t)(bins - 1);
+        }
+        __syncthreads();
+        tile_ranks<R>(digit, on, rank, nb, bins, cnt, tile_total);
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            if (!on[r]) continue;
+            const uint32_t to = place[digit[r]] + rank[r];
+            keys[to] = key[r];
+            pos[to] = at[r];
+        }
+        __syncthreads();
+        for (int d = tid; d < bins; d += kSortThreads) place[d] += tile_total[d];
+        __syncthreads();
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ sums
+constexpr int kChunk = 64;
+
+// VEC elements of a row at any alignment of the row, zeros behind column `cols`
+template <typename T, int VEC> __device__ __forceinline__ void add_row(const T *__restrict__ p, int cols, float (&acc)[VEC]) {
+    if (cols >= VEC) {
+        const Loose<T, VEC> t = *reinterpret_cast<const Loose<T, VEC> *>(p);
+#pragma unroll
+        for (int e = 0; e < VEC; e++) acc[e] += to_f32(t.v[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < VEC; e++)
+            if (e < cols) acc[e] += to_f32(p[e]);
+    }
+}
+
+// Column layout of the two kernels below: a workgroup covers `lanes` * VEC columns (blockIdx.y the column block), lanes = a power of two <= 64; the
+// 256 / lanes groups of lanes are slots that take entries in turn.
+
+// partial[c][D] of the chunks that lie inside one run
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void k_embed_chunks(const uint32_t *__restrict__ keys, const uint32_t *__restrict__ pos, const T *__restrict__ grad, int64_t ldg,
+                                                      int64_t n, uint32_t V, int D, int lanes, float *__restrict__ partial) {
+    __shared__ float join[256 * VEC];
+    const int64_t c0 = (int64_t)blockIdx.x * kChunk;
+    const uint32_t first = keys[c0];
+    if (c0 + kChunk > n || first == V || first != keys[c0 + kChunk - 1]) return;        // (uniform in the workgroup)
+    const int tid = threadIdx.x, col = ((int)blockIdx.y * lanes + (tid & (lanes - 1))) * VEC, slot = tid / lanes, slots = 256 / lanes;
+    float acc[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; e++) acc[e] = 0.f;
+    if (col < D) {
+#pragma unroll 4
+        for (int j = slot; j < kChunk; j += slots) add_row<T, VEC>(grad + (int64_t)pos[c0 + j] * ldg + col, D - col, acc);
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; e++) join[e * 256 + tid] = acc[e];
+    __syncthreads();
+    if (slot != 0 || col >= D) return;
+    for (int s = 1; s < slots; s++)
+#pragma unroll
+        for (int e = 0; e < VEC; e++) acc[e] += join[e * 256 + s * lanes + tid];
+    float *out = partial + (int64_t)blockIdx.x * D + col;
+#pragma unroll
+    for (int e = 0; e < VEC; e++)
+        if (col + e < D) out[e] = acc[e];
+}
+
+// first place in keys[0, n) that is >= v
+__device__ __forceinline__ int64_t lower_bound(const uint32_t *__restrict__ keys, int64_t n, uint32_t v) {
+    int64_t lo = 0, hi = n;
+    while (lo < hi) {
+        const int64_t mid = (lo + hi) >> 1;
+        if (keys[mid] < v) lo = mid + 1; else hi = mid;
+    }
+    return lo;
+}
+
+constexpr int kRowsPerGroup = 16, kShort = 8;       // rows per workgroup; runs up to kShort entries are summed by one slot
+
+template <typename T, typename O, int VEC>
+__global__ __launch_bounds__(256) void k_embed_rows(const uint32_t *__restrict__ keys, const uint32_t *__restrict__ pos, const T *__restrict__ grad, int64_t ldg, int64_t n,
+                                                    int64_t V, int D, int lanes, const float *__restrict__ partial, float scale, O *__restrict__ gtable) {
+    __shared__ int64_t bound[kRowsPerGroup + 1];
+    __shared__ float join[256 * VEC];
+    const int tid = threadIdx.x, lane = tid & (lanes - 1), slot = tid / lanes, slots = 256 / lanes, col = ((int)blockIdx.y * lanes + lane) * VEC;
+    const int64_t v0 = (int64_t)blockIdx.x * kRowsPerGroup;
+    const int rows = V - v0 < kRowsPerGroup ? (int)(V - v0) : kRowsPerGroup;
+    if (tid <= rows) bound[tid] = lower_bound(keys, n, (uint32_t)(v0 + tid));
+    __syncthreads();
+    auto write = [&](int r, const float (&acc)[VEC]) {
+        O *out = gtable + (v0 + r) * D + col;
+        Loose<O, VEC> o;
+#pragma unroll
+        for (int e = 0; e < VEC; e++) o.v[e] = from_f32<O>(acc[e] * scale);
+        if (col + VEC <= D) *reinterpret_cast<Loose<O, VEC> *>(out) = o;
+        else
+#pragma unroll
+            for (int e = 0; e < VEC; e++)
+                if (col + e < D) out[e] = o.v[e];
+    };
+    for (int r = slot; r < rows; r += slots) {              // short runs: a slot each
+        const int64_t s = bound[r], e_ = bound[r + 1];
+        if (e_ - s > kShort || col >= D) continue;
+        float acc[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; e++) acc[e] = 0.f;
+        for (int64_t j = s; j < e_; j++) add_row<T, VEC>(grad + (int64_t)pos[j] * ldg + col, D - col, acc);
+        write(r, acc);
+    }
+    for (int r = 0; r < rows; r++) {                        // long runs: all slots, joined in the order of the slots
+        const int64_t s = bound[r], e_ = bound[r + 1];
+        if (e_ - s <= kShort) continue;                     // (uniform)
+        const int64_t c_first = (s + kChunk - 1) / kChunk, c_last = e_ / kChunk;      // whole chunks [c_first, c_last)
+        const int64_t head = c_first < c_last ? c_first * kChunk : e_, tail = c_first < c_last ? c_last * kChunk : e_;
+        float acc[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; e++) acc[e] = 0.f;
+        if (col < D) {
+#pragma unroll 4
+            for (int64_t j = s + slot; j < head; j += slots) add_row<T, VEC>(grad + (int64_t)pos[j] * ldg + col, D - col, acc);
+#pragma unroll 4
+            for (int64_t j = tail + slot; j < e_; j += slots) add_row<T, VEC>(grad + (int64_t)pos[j] * ldg + col, D - col, acc);
+#pragma unroll 4
+            for (int64_t c = c_first + slot; c < c_last; c += slots) add_row<float, VEC>(partial + c * D + col, D - col, acc);
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; e++) join[e * 256 + tid] = acc[e];
+        __syncthreads();
+        if (slot == 0 && col < D) {
+            for (int q = 1; q < slots; q++)
+#pragma unroll
+                for (int e = 0; e < VEC; e++) acc[e] += join[e * 256 + q * lanes + lane];
+            write(r, acc);
+        }
+        __syncthreads();
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+struct BwdPlan {
+    int bits, passes, nb_max;
+    int64_t blocks, per;            // multi-block sort
+    int64_t off_keys[2], off_pos[2], off_hist, off_partial, bytes;
+};
+
+int64_t up256(int64_t b) { return (b + 255) / 256 * 256; }
+
+BwdPlan plan_bwd(int64_t n, int64_t V, int64_t D) {
+    BwdPlan p = {};
+    while (p.bits < 32 && ((uint64_t)V >> p.bits) != 0) p.bits++;        // keys 0 .. V
+    const bool one = n <= kOneMax;
+    const int digit = one ? kOneDigit : kMultiDigit;
+    p.passes = (p.bits + digit - 1) / digit;
+    p.nb_max = (p.bits + p.passes - 1) / p.passes;
+    const int64_t tiles = (n + kTile - 1) / kTile;
+    p.per = ((tiles + kMaxBlocks - 1) / kMaxBlocks) * kTile;
+    p.blocks = one ? 1 : (n + p.per - 1) / p.per;
+    int64_t at = 0;
+    auto take = [&](int64_t b) { const int64_t r = at; at += up256(b); return r; };
+    const int copies = one || p.passes == 1 ? 1 : 2;
+    for (int k = 0; k < 2; k++) {
+        p.off_keys[k] = k < copies ? take(4 * n) : p.off_keys[0];
+        p.off_pos[k] = k < copies ? take(4 * n) : p.off_pos[0];
+    }
+    p.off_hist = one ? 0 : take(p.blocks * 4ll << p.nb_max);
+    p.off_partial = take((n / kChunk) * D * 4);
+    p.bytes = at;
+    return p;
+}
+
+template <typename I, int R>
+void launch_one(const I *idx, int n, int64_t V, int64_t padding, const BwdPlan &p, uint32_t *keys, uint32_t *pos, hipStream_t s) {
+    const int lds = 4 * (256 + kSortWaves + kSortWaves * 256 / 2 + 2 * 1024 * R);
+    static hsLdsAttrOnce attr;
+    attr.set((const void *)k_sort_one<I, R>, lds);
+    k_sort_one<I, R><<<1, kSortThreads, lds, s>>>(idx, n, V, padding, p.bits, p.passes, keys, pos);
+}
+
+template <typename I>
+void launch_sort(const I *idx, int64_t n, int64_t V, int64_t padding, const BwdPlan &p, char *ws, uint32_t *&keys, uint32_t *&pos, hipStream_t s) {
+    if (n <= kOneMax) {
+        keys = (uint32_t *)(ws + p.off_keys[0]);
+        pos = (uint32_t *)(ws + p.off_pos[0]);
+        if (n <= 1024) launch_one<I, 1>(idx, (int)n, V, padding, p, keys, pos, s);
+        else if (n <= 4096) launch_one<I, 4>(idx, (int)n, V, padding, p, keys, pos, s);
+        else launch_one<I, 16>(idx, (int)n, V, padding, p, keys, pos, s);
+        return;
+    }
+    static hsLdsAttrOnce attr;
+    attr.set((const void *)k_sort_scatter<I>, 4 * (2 * 2048 + kSortWaves) + 2 * kSortWaves * 2048);
+    uint32_t *hist = (uint32_t *)(ws + p.off_hist), *k_in = nullptr, *p_in = nullptr;
+    int shift = 0;
+    for (int pass = 0; pass < p.passes; pass++) {
+        const int nb = (p.bits - shift + p.passes - pass - 1) / (p.passes - pass), bins = 1 << nb;
+        keys = (uint32_t *)(ws + p.off_keys[pass & 1]);
+        pos = (uint32_t *)(ws + p.off_pos[pass & 1]);
+        k_sort_hist<I><<<(unsigned)p.blocks, kSortThreads, 0, s>>>(idx, k_in, n, p.per, V, padding, shift, nb, hist);
+        k_sort_scatter<I><<<(unsigned)p.blocks, kSortThreads, 4 * (2 * bins + kSortWaves) + 2 * kSortWaves * bins, s>>>(idx, k_in, p_in, n, p.per, V, padding, shift, nb,
+                                                                                                                     hist, keys, pos);
+        k_in = keys;
+        p_in = pos;
+        shift += nb;
+    }
+}
+
+bool sizes_ok(int64_t n, int64_t V, int64_t D) { return n >= 0 && n <= 0x7fffffff && V >= 0 && V < 0x7fffffff && D >= 0 && D <= (1 << 20); }
+
+int pow2_at_least(int v) { int p = 1; while (p < v) p <<= 1; return p; }
+
+}  // namespace
+
+extern "C" {
+
+int hs_embed_fwd(const void *indices, int32_t index_bytes, const void *table, int64_t ld, void *out, int64_t n, int64_t V, int64_t D, float scale, int32_t table_dtype,
+                 int32_t out_dtype, void *stream) {
+    if (!sizes_ok(n, V, D) || (index_bytes != 4 && index_bytes != 8) || !known_dtype(table_dtype) || !known_dtype(out_dtype) || ld < D) return HS_ERR_ARG;
+    if (n == 0 || D == 0) return HS_OK;
+    if (!indices || !out || (V > 0 && !table)) return HS_ERR_NULL;
+    const int tb = elem_bytes(table_dtype), ob = elem_bytes(out_dtype);
+    // the widest group that the row starts of both sides allow
+    int vec = 8;
+    while (vec > 1 && (D % vec || ld % vec || (uintptr_t)table % (vec * tb < 16 ? vec * tb : 16) || (uintptr_t)out % (vec * ob < 16 ? vec * ob : 16))) vec >>= 1;
+    if (vec == 2) vec = 1;
+    const int64_t total = n * (D / vec), blocks = (total + 255) / 256;
+    if (blocks > 0x7fffffff) return HS_ERR_ARG;
+    hipStream_t s = (hipStream_t)stream;
+#define HS_EMBED_FWD(I, VEC)                                                                                                                                      \
+    HS_BY_DTYPE(table_dtype, {                                                                                                                                    \
+        using TT = T;                                                                                                                                             \
+        HS_BY_DTYPE(out_dtype, (k_embed_fwd<TT, T, I, VEC><<<(unsigned)blocks, 256, 0, s>>>((const I *)indices, (const TT *)table, ld, (T *)out, total,           \
+                                                                                           (uint32_t)(D / VEC), V, scale)));                                     \
+    })
+    if (index_bytes == 8) {
+        if (vec == 8) HS_EMBED_FWD(int64_t, 8); else if (vec == 4) HS_EMBED_FWD(int64_t, 4); else HS_EMBED_FWD(int64_t, 1);
+    } else {
+        if (vec == 8) HS_EMBED_FWD(int32_t, 8); else if (vec == 4) HS_EMBED_FWD(int32_t, 4); else HS_EMBED_FWD(int32_t, 1);
+    }
+    return hipGetLastError() == hipSuccess ? HS_OK : HS_ERR_LAUNCH;
+}
+
+int64_t hs_embed_bwd_ws_bytes(int64_t n, int64_t V, int64_t D) { return sizes_ok(n, V, D) ? plan_bwd(n, V, D).bytes : HS_ERR_ARG; }
+
+int hs_embed_bwd(const void *indices, int32_t index_bytes, const void *grad, int64_t ldg, void *grad_table, int64_t n, int64_t V, int64_t D, float scale, int64_t padding,
+                 int32_t grad_dtype, int32_t table_dtype, void *ws, int64_t ws_bytes, void *stream) {
+    if (!sizes_ok(n, V, D) || (index_bytes != 4 && index_bytes != 8) || !known_dtype(grad_dtype) || !known_dtype(table_dtype) || ldg < D) return HS_ERR_ARG;
+    if (V == 0 || D == 0) return HS_OK;
+    if (!grad_table || (n > 0 && (!indices || !grad || !ws))) return HS_ERR_NULL;
+    const BwdPlan p = plan_bwd(n, V, D);
+    if (ws_bytes < p.bytes) return HS_ERR_ARG;
+    hipStream_t s = (hipStream_t)stream;
+    uint32_t *keys = nullptr, *pos = nullptr;
+    float *partial = (float *)((char *)ws + p.off_partial);
+    if (n > 0) {
+        if (index_bytes == 8) launch_sort((const int64_t *)indices, n, V, padding, p, (char *)ws, keys, pos, s);
+        else launch_sort((const int32_t *)indices, n, V, padding, p, (char *)ws, keys, pos, s);
+    }
+    const int VEC = grad_dtype == HS_F32 ? 4 : 8;
+    int lanes = pow2_at_least((int)((D + VEC - 1) / VEC));
+    lanes = lanes > 64 ? 64 : lanes;
+    const unsigned col_blocks = (unsigned)((D + (int64_t)lanes * VEC - 1) / ((int64_t)lanes * VEC));
+    const int64_t row_blocks = (V + kRowsPerGroup - 1) / kRowsPerGroup;
+    HS_BY_DTYPE(grad_dtype, {
+        using G = T;
+        constexpr int W = sizeof(T) == 4 ? 4 : 8;
+        if (n >= kChunk)
+            k_embed_chunks<G, W><<<dim3((unsigned)(n / kChunk), col_blocks), 256, 0, s>>>(keys, pos, (const G *)grad, ldg, n, (uint32_t)V, (int)D, lanes, partial);
+        HS_BY_DTYPE(table_dtype, (k_embed_rows<G, T, W><<<dim3((unsigned)row_blocks, col_blocks), 256, 0, s>>>(keys, pos, (const G *)grad, ldg, n, V, (int)D, lanes, partial,
+                                                                                                           scale, (T *)grad_table)));
+    });
+    return hipGetLastError() == hipSuccess ? HS_OK : HS_ERR_LAUNCH;
+}
+
+}  // extern "C"

@@ -1,0 +1,253 @@
+// gated_mlp.h -- the gated feed-forward block on rows_gemm.h, one instantiation per user type (gated_mlp_{bf16,f16,f32}.hip):
+//     G = x Wg^T, U = x Wu^T, H = act(G) U (one launch), y = H Wd^T;
+//     gH = gy Wd, gg = gH U act'(G), gu = gH act(G) (one launch), gx = gg Wg + gu Wu, gWg = gg^T x, gWu = gu^T x (one launch), gWd = gy^T H.
+// Roundings besides the results' own: H, gg and gu to the operand type, because the matrix cores multiply 16-bit operands (fp32: as three bf16 planes,
+// 24 bits); G and U to the user's type where the backward pass will read them again (the forward pass uses them unrounded).
+#pragma once
+#include "rows_gemm.h"
+
+namespace hs_gemm {
+
+// An operand as the products read it: 16-byte aligned rows whose contiguous extent is a multiple of 8 (zeros behind the matrix's own).
+struct Operand {
+    const void *p;
+    int64_t ld, plane;
+};
+
+// Hands out pieces of the caller's work space; without one it only counts.
+struct Arena {
+    char *base;
+    int64_t at = 0;
+    void *take(int64_t bytes) {
+        const int64_t r = at;
+        at += (bytes + 255) / 256 * 256;
+        return base ? base + r : nullptr;
+    }
+};
+
+inline int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
+
+// src [rows, cols] -> dst [planes][rows][ldp], ldp = up8(cols), zeros behind cols
+template <typename U>
+__global__ __launch_bounds__(256) void k_rows_pack(const U *__restrict__ src, int64_t ld, int64_t rows, int64_t cols, int64_t chunks, void *__restrict__ dst, int64_t plane) {
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (id >= rows * chunks) return;
+    const int64_t r = id / chunks, c = (id - r * chunks) * 8;
+    const U *s = src + r * ld + c;
+    Loose<U, 8> v;
+    if (c + 8 <= cols) v = *reinterpret_cast<const Loose<U, 8> *>(s);
+    else
+#pragma unroll
+        for (int e = 0; e < 8; e++) v.v[e] = c + e < cols ? s[e] : (U)0.f;
+    if constexpr (sizeof(U) == 4) {
+        Pack<bf16_t, 8> o[3];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            bf16_t q[3];
+            split3(v.v[e], q);
+            o[0].v[e] = q[0]; o[1].v[e] = q[1]; o[2].v[e] = q[2];
+        }
+#pragma unroll
+        for (int q = 0; q < 3; q++) *reinterpret_cast<Pack<bf16_t, 8> *>((bf16_t *)dst + q * plane + id * 8) = o[q];
+    } else {
+        Pack<U, 8> o;
+#pragma unroll
+        for (int e = 0; e < 8; e++) o.v[e] = v.v[e];
+        *reinterpret_cast<Pack<U, 8> *>((U *)dst + id * 8) = o;
+    }
+}
+
+// out = sum of the slices' partial results, in the order of the slices
+template <typename U>
+__global__ __launch_bounds__(256) void k_rows_reduce(const float *__restrict__ parts0, const float *__restrict__ parts1, int64_t n, int slices, U *__restrict__ out0, U *__restrict__ out1) {
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= n) return;
+    const float *p = (blockIdx.y ? parts1 : parts0) + i;
+    U *o = (blockIdx.y ? out1 : out0) + i;
+    const int64_t stride = (n + 3) / 4 * 4;
+    float4 v = *reinterpret_cast<const float4 *>(p);
+    for (int s = 1; s < slices; s++) {
+        const float4 t = *reinterpret_cast<const float4 *>(p + s * stride);
+        v.x += t.x; v.y += t.y; v.z += t.z; v.w += t.w;
+    }
+    const float r[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (i + e < n) o[e] = from_f32<U>(r[e]);
+}
+
+// ------------------------------------------------------------------------------------------------ products
+// Tile by the number of workgroups: 256 CUs want at least one each; the larger tile reads less per product.
+template <typename T, typename U, bool AKS, bool BKS, int EPI> int launch_product(Args &p, int problems, hipStream_t s) {
+    const int64_t cols = EPI == EPI_GATE ? 2 * p.ldh : EPI == EPI_GATE_BWD ? p.ldh : p.J;
+    auto tiles = [&](int64_t b) { return (p.I + b - 1) / b * ((cols + b - 1) / b) * problems * p.slices; };
+    if (tiles(256) >= 192) return launch_tile<T, U, 256, 256, 2, 4, AKS, BKS, EPI>(p, problems, s);
+    if (tiles(128) >= 192) return launch_tile<T, U, 128, 128, 2, 2, AKS, BKS, EPI>(p, problems, s);
+    return launch_tile<T, U, 64, 64, 2, 2, AKS, BKS, EPI>(p, problems, s);
+}
+
+// the segments of one product: one pair, or the six plane products of an fp32 one
+template <typename U> int add_segments(Seg *seg, int n, const Operand &a, const Operand &b, const Operand *b1 = nullptr) {
+    if constexpr (sizeof(U) == 4) {
+        static const int pa[6] = {0, 1, 2, 0, 1, 0}, pb[6] = {2, 1, 0, 1, 0, 0};
+        for (int t = 0; t < 6; t++)
+            seg[n++] = Seg{(const bf16_t *)a.p + pa[t] * a.plane, (const bf16_t *)b.p + pb[t] * b.plane, b1 ? (const void *)((const bf16_t *)b1->p + pb[t] * b1->plane) : nullptr};
+    } else {
+        seg[n++] = Seg{a.p, b.p, b1 ? b1->p : nullptr};
+    }
+    return n;
+}
+
+template <typename U> constexpr int planes() { return sizeof(U) == 4 ? 3 : 1; }
+
+template <typename T, typename U> struct Block {
+    const hsGatedMlp &a;
+    Arena ws;
+    hipStream_t s;
+    bool run;
+    int rc = HS_OK;
+    int64_t M, D, F, ldh, ldd;
+
+    Block(const hsGatedMlp &args, bool run_, hipStream_t stream) : a(args), ws{run_ ? (char *)args.ws : nullptr}, s(stream), run(run_), M(args.rows), D(args.dim), F(args.hidden),
+                                                                  ldh(up8(args.hidden)), ldd(up8(args.dim)) {}
+
+    void check(int r) { if (rc == HS_OK) rc = r; }
+
+    Operand operand(const void *p, int64_t ld, int64_t rows, int64_t cols, bool force = false) {
+        if (sizeof(U) == 2 && !force && (uintptr_t)p % 16 == 0 && ld % 8 == 0 && cols % 8 == 0) return Operand{p, ld, 0};
+        const int64_t ldp = up8(cols), n = rows * ldp;
+        void *dst = ws.take(n * 2 * planes<U>());
+        if (run && rc == HS_OK) {
+            const int64_t blocks = (n / 8 + 255) / 256;
+            if (blocks > 0x7fffffff) { check(HS_ERR_ARG); return Operand{}; }
+            k_rows_pack<U><<<(unsigned)blocks, 256, 0, s>>>((const U *)p, ld, rows, cols, ldp / 8, dst, n);
+            check(hipGetLastError() == hipSuccess ? HS_OK : HS_ERR_LAUNCH);
+        }
+        return Operand{dst, ldp, n};
+    }
+
+    // both projections' weights with one row distance
+    void projections(Operand &wg, Operand &wu) {
+        const bool differ = a.ld_gate != a.ld_up;
+        wg = operand(a.w_gate, a.ld_gate, F, D, differ);
+        wu = operand(a.w_up, a.ld_up, F, D, differ);
+        if (wg.ld != wu.ld) {        // (one needed a copy: so does the other)
+            if (wg.ld == a.ld_gate && wg.p == a.w_gate) wg = operand(a.w_gate, a.ld_gate, F, D, true);
+            else wu = operand(a.w_up, a.ld_up, F, D, true);
+        }
+    }
+
+    struct Saved { U *g, *u; Operand h; int64_t bytes; };
+    Saved saved_in(char *base) const {
+        Saved v = {};
+        const int64_t n = M * ldh, gu = (n * (int64_t)sizeof(U) + 255) / 256 * 256;
+        v.g = (U *)base;
+        v.u = (U *)(base + gu);
+        v.h = Operand{base + 2 * gu, ldh, n};
+        v.bytes = 2 * gu + n * 2 * planes<U>();
+        return v;
+    }
+
+    template <bool AKS, bool BKS> bool fits(const Operand &x, const Operand &y) {       // 32-bit offsets inside a tile's step
+        const int64_t most = 0x7fffffffll - 4096;
+        if (256 * x.ld * 2 > most || 256 * y.ld * 2 > most) { check(HS_ERR_ARG); return false; }
+        return rc == HS_OK;
+    }
+
+    void fwd() {
+        const Operand x = operand(a.x, a.ldx, M, D);
+        Operand wg, wu;
+        projections(wg, wu);
+        const Operand wd = operand(a.w_down, a.ld_down, D, F);
+        Saved sv = saved_in((char *)a.saved);
+        if (!a.saved) {
+            sv.g = sv.u = nullptr;
+            sv.h = Operand{ws.take(M * ldh * 2 * planes<U>()), ldh, M * ldh};
+        }
+        if (!run || !fits<false, false>(x, wg) || !fits<false, false>(wd, sv.h)) return;
+        Args p = {};
+        p.n_seg = add_segments<U>(p.seg[0], 0, x, wg, &wu);
+        p.lda = x.ld; p.ldb = wg.ld; p.I = M; p.J = (int)F; p.K = (int)D; p.slices = 1;
+        p.g = sv.g; p.u = sv.u; p.h = (void *)sv.h.p; p.ldh = ldh; p.plane = sv.h.plane; p.act = a.activation;
+        check(launch_product<T, U, false, false, EPI_GATE>(p, 1, s));
+        Args q = {};
+        q.n_seg = add_segments<U>(q.seg[0], 0, sv.h, wd);
+        q.lda = ldh; q.ldb = wd.ld; q.I = M; q.J = (int)D; q.K = (int)F; q.slices = 1;
+        q.out[0] = a.y; q.ldo = D;
+        if (rc == HS_OK) check(launch_product<T, U, false, false, EPI_STORE>(q, 1, s));
+    }
+
+    // C_z [I, J] = A_z^T B over the rows, z < problems: sliced along them when the result alone does not fill the device
+    void weight_gradient(const Operand *av, const Operand &b, void *const *out, int problems, int64_t I, int64_t J) {
+        const int64_t tiles = (I + 127) / 128 * ((J + 127) / 128) * problems, steps = (M + BK - 1) / BK * (sizeof(U) == 4 ? 6 : 1);
+        int64_t slices = 1;
+        while (slices < 64 && tiles * slices < 512 && steps / (slices * 2) >= 8) slices *= 2;
+        const int64_t n = I * J, stride = (n + 3) / 4 * 4;
+        float *parts = slices > 1 ? (float *)ws.take(stride * 4 * slices * problems) : nullptr;
+        if (!run || !fits<true, true>(av[0], b)) return;
+        Args p = {};
+        for (int z = 0; z < problems; z++) p.n_seg = add_segments<U>(p.seg[z], 0, av[z], b);
+        p.lda = av[0].ld; p.ldb = b.ld; p.I = I; p.J = (int)J; p.K = (int)M; p.slices = (int)slices; p.ldo = J; p.slice_stride = stride;
+        for (int z = 0; z < problems; z++) p.out[z] = slices > 1 ? (void *)(parts + z * slices * stride) : out[z];
+        if (slices == 1) {
+            check(launch_product<T, U, true, true, EPI_STORE>(p, problems, s));
+            return;
+        }
+        check(launch_product<T, U, true, true, EPI_PARTIAL>(p, problems, s));
+        if (rc != HS_OK) return;
+        const int64_t blocks = (n + 1023) / 1024;
+        k_rows_reduce<U><<<dim3((unsigned)blocks, problems), 256, 0, s>>>(parts, parts + (problems - 1) * slices * stride, n, (int)slices, (U *)out[0], (U *)out[problems - 1]);
+        check(hipGetLastError() == hipSuccess ? HS_OK : HS_ERR_LAUNCH);
+    }
+
+    void bwd() {
+        const Operand gy = operand(a.grad, a.ld_grad, M, D);
+        const Saved sv = saved_in((char *)a.saved);
+        if (a.gx || a.gw_gate || a.gw_up) {
+            const Operand wd = operand(a.w_down, a.ld_down, D, F);
+            const int64_t n = M * ldh;
+            const Operand gg{ws.take(n * 2 * planes<U>()), ldh, n}, gu{ws.take(n * 2 * planes<U>()), ldh, n};
+            if (run && fits<false, true>(gy, wd)) {
+                Args p = {};
+                p.n_seg = add_segments<U>(p.seg[0], 0, gy, wd);
+                p.lda = gy.ld; p.ldb = wd.ld; p.I = M; p.J = (int)F; p.K = (int)D; p.slices = 1;
+                p.g = sv.g; p.u = sv.u; p.gg = (void *)gg.p; p.gu = (void *)gu.p; p.ldh = ldh; p.plane = n; p.act = a.activation;
+                check(launch_product<T, U, false, true, EPI_GATE_BWD>(p, 1, s));
+            }
+            if (a.gx) {
+                Operand wg, wu;
+                projections(wg, wu);
+                if (run && fits<false, true>(gg, wg)) {
+                    Args p = {};
+                    p.n_seg = add_segments<U>(p.seg[0], 0, gg, wg);
+                    p.n_seg = add_segments<U>(p.seg[0], p.n_seg, gu, wu);
+                    p.lda = ldh; p.ldb = wg.ld; p.I = M; p.J = (int)D; p.K = (int)F; p.slices = 1;
+                    p.out[0] = a.gx; p.ldo = D;
+                    check(launch_product<T, U, false, true, EPI_STORE>(p, 1, s));
+                }
+            }
+            if (a.gw_gate || a.gw_up) {
+                const Operand x = operand(a.x, a.ldx, M, D);
+                const Operand av[2] = {a.gw_gate ? gg : gu, gu};
+                void *const out[2] = {a.gw_gate ? a.gw_gate : a.gw_up, a.gw_up};
+                weight_gradient(av, x, out, a.gw_gate && a.gw_up ? 2 : 1, F, D);
+            }
+        }
+        if (a.gw_down) weight_gradient(&gy, sv.h, &a.gw_down, 1, D, F);
+    }
+};
+
+template <typename T, typename U> int64_t block_call(const hsGatedMlp &a, int what, hipStream_t s) {
+    if (what == 4) return Block<T, U>(a, false, s).saved_in(nullptr).bytes;
+    Block<T, U> b(a, what < 2, s);
+    if (what % 2 == 0) b.fwd(); else b.bwd();
+    if (what >= 2) return b.ws.at;
+    return b.rc;
+}
+
+// what: 0 forward, 1 backward, 2 / 3 their work spaces' bytes, 4 the saved buffer's bytes
+int64_t gated_mlp_bf16(const hsGatedMlp &a, int what, hipStream_t s);
+int64_t gated_mlp_f16(const hsGatedMlp &a, int what, hipStream_t s);
+int64_t gated_mlp_f32(const hsGatedMlp &a, int what, hipStream_t s);
+
+}  // namespace hs_gemm

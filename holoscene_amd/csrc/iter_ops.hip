@@ -19,6 +19,7 @@
 
 #include "holoscene_hip.h"
 #include "batch_draw.h"
+#include "philox.h"
 
 namespace {
 
@@ -58,18 +59,6 @@ __device__ __forceinline__ void wn_row(const WnJobsI &jobs, int row_g, int lane)
     }
 }
 
-// Philox-4x32-10 (Salmon et al., SC'11): counter (c0..c3), key (k0, k1) -> four 32-bit words
-__device__ __forceinline__ uint4 philox4x32_10(uint4 c, uint2 k) {
-    constexpr uint32_t M0 = 0xD2511F53u, M1 = 0xCD9E8D57u, W0 = 0x9E3779B9u, W1 = 0xBB67AE85u;
-#pragma unroll
-    for (int r = 0; r < 10; r++) {
-        const uint32_t hi0 = __umulhi(M0, c.x), lo0 = M0 * c.x, hi1 = __umulhi(M1, c.z), lo1 = M1 * c.z;
-        c = make_uint4(hi1 ^ c.y ^ k.x, lo1, hi0 ^ c.w ^ k.y, lo0);
-        k.x += W0;
-        k.y += W1;
-    }
-    return c;
-}
 __device__ __forceinline__ float u01(uint32_t x) { return (float)(x >> 8) * 5.9604644775390625e-08f; }      // 24 bits: [0, 1)
 
 constexpr int kRngPerThread = 16, kRngPerBlock = 256 * kRngPerThread;

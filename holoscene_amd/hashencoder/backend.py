@@ -99,7 +99,13 @@ class hsDrawSched(ctypes.Structure):
                 ("counter_base", ctypes.c_uint64), ("n_sched", ctypes.c_int32), ("n_frames", ctypes.c_int32)]
 
 
-ABI_VERSION = 9
+class hsGatedMlp(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "w_gate", "w_up", "w_down")] + [(n, ctypes.c_int64) for n in ("ldx", "ld_gate", "ld_up", "ld_down", "rows", "dim", "hidden")]
+                + [("dtype", ctypes.c_int32), ("activation", ctypes.c_int32), ("y", ctypes.c_void_p), ("saved", ctypes.c_void_p), ("grad", ctypes.c_void_p),
+                   ("ld_grad", ctypes.c_int64)] + [(n, ctypes.c_void_p) for n in ("gx", "gw_gate", "gw_up", "gw_down", "ws")] + [("ws_bytes", ctypes.c_int64)])
+
+
+ABI_VERSION = 10
 
 # Small zero-initialised accumulators (bias-gradient sums the backward kernels add to by atomics): slices of a pool the optimiser zeroes
 # together with the flat gradient buffer -- one memset per iteration instead of one ~5 us fill launch per accumulator.  The sequence of
@@ -145,6 +151,9 @@ def _gate(gate):
 
 
 _lib = None
+_ROW_BYTES = ("hs_embed_bwd_ws_bytes", "hs_gated_mlp_saved_bytes", "hs_gated_mlp_fwd_ws_bytes", "hs_gated_mlp_bwd_ws_bytes")      # sizes, or a negative error
+ROW_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}        # HS_F32 / HS_BF16 / HS_F16: section 10 (row operators)
+ROW_ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "sigmoid": 3, "relu": 4}       # HS_ACT_*
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}  # HS_F32 / HS_BF16
 
 
@@ -159,7 +168,7 @@ def load_library():
         _lib.hs_target_arch.restype = ctypes.c_char_p
         for name in dir_symbols():
             if name != "hs_target_arch":
-                getattr(_lib, name).restype = ctypes.c_int
+                getattr(_lib, name).restype = ctypes.c_int64 if name in _ROW_BYTES else ctypes.c_int
         if _lib.hs_abi_version() != ABI_VERSION:
             raise RuntimeError(f"{LIB_PATH}: ABI version {_lib.hs_abi_version()}, this package needs {ABI_VERSION} -- rebuild "
                                "(python -m holoscene_amd.csrc.build)")
@@ -171,7 +180,9 @@ def dir_symbols():
     return ["hs_abi_version", "hs_target_arch", "hs_hash_encode_forward", "hs_hash_encode_backward", "hs_hash_encode_second_backward",
             "hs_hash_fwd", "hs_hash_bwd", "hs_hash_bwd2", "hs_hash_bwd_jac", "hs_hash_encode_forward_dt", "hs_hash_encode_backward_dt", "hs_hash_encode_second_backward_dt", "hs_hash_scatter_ws_bytes", "hs_sampler_update", "hs_sampler_draw", "hs_sampler_final", "hs_sampler_step", "hs_sampler_pick", "hs_sampler_draw_step", "hs_sampler_draw_steps", "hs_sampler_tail", "hs_sampler_update_draw", "hs_softplus_tangent_fwd", "hs_softplus_tangent_bwd", "hs_adam_tick", "hs_adam_flat", "hs_adam_flat_shard", "hs_copy_many", "hs_composite_fwd", "hs_composite_bwd", "hs_sdf_mlp_fwd", "hs_sdf_mlp2_pack_bytes", "hs_sdf_mlp2_pack", "hs_sdf_mlp2_fwd", "hs_sdf_mlp2_fwd_wide", "hs_sdf_sweep_fwd", "hs_sdf_mlp32_pack_bytes", "hs_sdf_mlp32_pack", "hs_sdf_mlp32_fwd", "hs_trunk_mlp2_input_column", "hs_trunk_mlp2_fwd", "hs_trunk_mlp2_fwd_wide", "hs_trunk_mlp_fwd", "hs_trunk_mlp_bwd", "hs_trunk_bwd_parts", "hs_trunk_split_fwd", "hs_trunk_split_bwd", "hs_softplus_tangent_bwd_h", "hs_trunk_input_fwd", "hs_trunk_input_bwd", "hs_render_input_fwd", "hs_render_input_bwd", "hs_loss_rays", "hs_loss_eikonal", "hs_loss_stage1", "hs_bg_smooth_loss", "hs_ray_setup", "hs_ray_points", "hs_render_points", "hs_appearance_mask_words", "hs_appearance_fwd", "hs_appearance_bwd", "hs_pack_bf16", "hs_sum_slices", "hs_weight_norm", "hs_gather_rows", "hs_wgrad_rows", "hs_draw_pixels", "hs_draw_gather", "hs_draw_gather_sched", "hs_hash_bwd_draw", "hs_hash_bwd_jac_sums", "hs_iter_prologue", "hs_iter_prologue_draw", "hs_iter_epilogue", "hs_pack_iteration", "hs_trunk_rr_gy", "hs_trunk_rr_gy_split", "hs_trunk_rr_pack_bytes", "hs_trunk_rr_pack", "hs_trunk_rr_fwd_value", "hs_trunk_rr_fwd_wide", "hs_trunk_rr_bwd_value_wide",
             "hs_trunk_rr_fwd_grad", "hs_trunk_rr_fwd", "hs_trunk_rr_bwd_grad", "hs_trunk_rr_bwd_value", "hs_wgrad_pairs", "hs_assemble", "hs_abs_shift", "hs_trunk_pack_all", "hs_appearance2_pack_bytes", "hs_appearance2_enc_column", "hs_appearance2_pack",
-            "hs_appearance2_fwd", "hs_appearance2_pack_t_bytes", "hs_appearance2_bwd", "hs_gemm_split_nt", "hs_gemm_split_tn"]
+            "hs_appearance2_fwd", "hs_appearance2_pack_t_bytes", "hs_appearance2_bwd", "hs_gemm_split_nt", "hs_gemm_split_tn", "hs_embed_fwd",
+            "hs_embed_bwd_ws_bytes", "hs_embed_bwd", "hs_dropout_rows", "hs_gated_mlp_saved_bytes", "hs_gated_mlp_fwd_ws_bytes", "hs_gated_mlp_bwd_ws_bytes",
+            "hs_gated_mlp_fwd", "hs_gated_mlp_bwd"]
 
 
 def _check(rc, what):
@@ -1579,6 +1590,81 @@ class _HipBackend:
         lib = load_library()
         _check(lib.hs_loss_eikonal(_dev(g1, "g1"), _dev(g2, "g2"), ctypes.c_int64(g1.shape[0]), ctypes.c_float(w_eik), ctypes.c_float(w_smooth),
                                    _dev(acc2, "acc2"), _dev(d_g1, "d_g1"), _dev(d_g2, "d_g2"), _stream()), "hs_loss_eikonal")
+
+
+    # ---- row operators (include/holoscene_hip.h section 10).  Callers (model/row_ops.py) have checked shapes, types and devices and made the
+    # tensors' device current; rows may be strided, elements of a row are consecutive.
+    @staticmethod
+    def _rows(t):
+        """(pointer, row distance) of a 2-D tensor; a matrix of one row (or none) may carry any stride."""
+        return ctypes.c_void_p(t.data_ptr()), ctypes.c_int64(t.stride(0) if t.shape[0] > 1 else t.shape[1])
+
+    @classmethod
+    def embed_fwd(cls, indices, table, out, scale):
+        lib = load_library()
+        tp, ld = cls._rows(table)
+        _check(lib.hs_embed_fwd(ctypes.c_void_p(indices.data_ptr()), indices.element_size(), tp, ld, ctypes.c_void_p(out.data_ptr()), ctypes.c_int64(indices.numel()),
+                                ctypes.c_int64(table.shape[0]), ctypes.c_int64(table.shape[1]), ctypes.c_float(scale), ROW_DTYPES[table.dtype], ROW_DTYPES[out.dtype],
+                                _stream()), "hs_embed_fwd")
+
+    @classmethod
+    def embed_bwd(cls, indices, grad, grad_table, scale, padding):
+        lib = load_library()
+        n, V, D = ctypes.c_int64(indices.numel()), ctypes.c_int64(grad_table.shape[0]), ctypes.c_int64(grad_table.shape[1])
+        nbytes = lib.hs_embed_bwd_ws_bytes(n, V, D)
+        _check(min(nbytes, 0), "hs_embed_bwd")
+        ws = torch.empty(nbytes, device=grad.device, dtype=torch.uint8)
+        gp, ldg = cls._rows(grad)
+        _check(lib.hs_embed_bwd(ctypes.c_void_p(indices.data_ptr()), indices.element_size(), gp, ldg, ctypes.c_void_p(grad_table.data_ptr()), n, V, D, ctypes.c_float(scale),
+                                ctypes.c_int64(padding), ROW_DTYPES[grad.dtype], ROW_DTYPES[grad_table.dtype], ctypes.c_void_p(ws.data_ptr()), ctypes.c_int64(nbytes), _stream()), "hs_embed_bwd")
+
+    @staticmethod
+    def dropout_rows(x, residual, y, drop, rng):
+        lib = load_library()
+        _check(lib.hs_dropout_rows(ctypes.c_void_p(x.data_ptr()), None if residual is None else ctypes.c_void_p(residual.data_ptr()), ctypes.c_void_p(y.data_ptr()),
+                                   ctypes.c_int64(x.numel()), ROW_DTYPES[x.dtype], int(drop), ctypes.c_void_p(rng.data_ptr()), _stream()), "hs_dropout_rows")
+
+    @classmethod
+    def _gated_args(cls, x, w_gate, w_up, w_down, activation):
+        a = hsGatedMlp(rows=x.shape[0], dim=x.shape[1], hidden=w_gate.shape[0], dtype=ROW_DTYPES[x.dtype], activation=ROW_ACTIVATIONS[activation])
+        for name, ld, t in (("x", "ldx", x), ("w_gate", "ld_gate", w_gate), ("w_up", "ld_up", w_up), ("w_down", "ld_down", w_down)):
+            p, d = cls._rows(t)
+            setattr(a, name, p)
+            setattr(a, ld, d.value)
+        return a
+
+    @staticmethod
+    def _gated_call(a, fn, nbytes, device):
+        _check(min(nbytes, 0), fn)
+        ws = torch.empty(nbytes, device=device, dtype=torch.uint8)
+        a.ws, a.ws_bytes = ws.data_ptr(), nbytes
+        _check(getattr(load_library(), fn)(ctypes.byref(a), _stream()), fn)
+
+    @classmethod
+    def gated_mlp_fwd(cls, x, w_gate, w_up, w_down, activation, y, save):
+        """save: also returns the buffer that gated_mlp_bwd reads."""
+        lib = load_library()
+        a = cls._gated_args(x, w_gate, w_up, w_down, activation)
+        saved = None
+        if save:
+            nbytes = lib.hs_gated_mlp_saved_bytes(ctypes.byref(a))
+            _check(min(nbytes, 0), "hs_gated_mlp_fwd")
+            saved = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
+            a.saved = saved.data_ptr()
+        a.y = y.data_ptr()
+        cls._gated_call(a, "hs_gated_mlp_fwd", lib.hs_gated_mlp_fwd_ws_bytes(ctypes.byref(a)), x.device)
+        return saved
+
+    @classmethod
+    def gated_mlp_bwd(cls, grad, x, w_gate, w_up, w_down, activation, saved, gx, gw_gate, gw_up, gw_down):
+        """gx, gw_*: written, None = not wanted."""
+        lib = load_library()
+        a = cls._gated_args(x, w_gate, w_up, w_down, activation)
+        p, d = cls._rows(grad)
+        a.grad, a.ld_grad, a.saved = p, d.value, saved.data_ptr()
+        for name, t in (("gx", gx), ("gw_gate", gw_gate), ("gw_up", gw_up), ("gw_down", gw_down)):
+            setattr(a, name, None if t is None else t.data_ptr())
+        cls._gated_call(a, "hs_gated_mlp_bwd", lib.hs_gated_mlp_bwd_ws_bytes(ctypes.byref(a)), x.device)
 
 
 class hsAdamState(ctypes.Structure):

@@ -1,0 +1,232 @@
+"""Operators on rows (samples, tokens, frames) beside the fused networks: learned codes looked up by index, a gated feed-forward block and
+dropout, each with its backward pass, on the kernels of csrc/embed_rows.hip, csrc/gated_mlp*.hip and csrc/dropout.hip.
+
+    codes = embedding_rows(frame_ids, table)                     # table[frame_ids], gradient by sorted indices
+    y = gated_mlp_rows(x, w_gate, w_up, w_down, "silu")          # (silu(x Wg^T) * (x Wu^T)) Wd^T
+    y = dropout_rows(y, 0.1, rng, residual=x)                    # x + dropout(y), the mask recomputed from a counter
+
+float32, bfloat16 and float16 storage, fp32 arithmetic, one rounding per result.  As everywhere in this package there is no CPU path: a tensor
+that is not on the GPU, or a type or shape the kernels do not take, raises RuntimeError.  The work runs on the current stream of the tensors' device
+and can be captured into a HIP graph; results do not depend on the launch (no floating-point atomics).  Gradients of gradients are not provided.
+"""
+import math
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from ..hashencoder import backend as _be
+
+ACTIVATIONS = tuple(_be.ROW_ACTIVATIONS)
+
+
+def _check_tensor(t, name, device=None, dtype=None, dtypes=tuple(_be.ROW_DTYPES)):
+    if not isinstance(t, torch.Tensor):
+        raise RuntimeError(f"{name} must be a tensor")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor")
+    if t.layout != torch.strided:
+        raise RuntimeError(f"{name} must be a dense tensor")
+    if device is not None and t.device != device:
+        raise RuntimeError(f"{name} is on {t.device}, expected {device}")
+    if dtype is not None and t.dtype != dtype:
+        raise RuntimeError(f"{name} must be a {dtype} tensor, got {t.dtype}")
+    if t.dtype not in dtypes:
+        raise RuntimeError(f"{name}: unsupported type {t.dtype}")
+
+
+def _as_rows(t):
+    """[..., n] -> 2-D with consecutive elements in a row: the tensor itself (any row distance >= n), else a copy."""
+    t = t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
+    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        t = t.contiguous()
+    return t
+
+
+class _embedding_rows(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, indices, table, scale, padding_idx, out_dtype):
+        rows = _as_rows(table)
+        indices = indices.contiguous()
+        out = torch.empty(*indices.shape, table.shape[1], device=table.device, dtype=out_dtype)
+        if out.numel():
+            with torch.cuda.device(table.device):
+                _be._backend.embed_fwd(indices, rows, out, scale)
+        ctx.save_for_backward(indices)
+        ctx.args = (table.shape, table.dtype, scale, -1 if padding_idx is None else padding_idx)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        indices, = ctx.saved_tensors
+        shape, dtype, scale, padding = ctx.args
+        g_table = torch.empty(shape, device=g.device, dtype=dtype)
+        if g_table.numel():
+            with torch.cuda.device(g.device):
+                _be._backend.embed_bwd(indices, _as_rows(g), g_table, scale, padding)
+        return None, g_table, None, None, None
+
+
+def embedding_rows(indices, table, scale=1.0, padding_idx=None, out_dtype=None):
+    """scale * table[indices]: indices int32 / int64 of any shape, table [V, D] -> [*indices.shape, D] of `out_dtype` (default: the table's type).
+
+    An index outside [0, V) reads zeros and takes no gradient (as a point outside the hash grid does); row `padding_idx` is read like any other and
+    takes no gradient.  The gradient is dense [V, D], summed in fp32 in the order of the positions, the same from run to run."""
+    _check_tensor(table, "table")
+    _check_tensor(indices, "indices", device=table.device, dtypes=(torch.int32, torch.int64))
+    if table.dim() != 2:
+        raise RuntimeError(f"table must be [V, D], got {tuple(table.shape)}")
+    if padding_idx is not None and not 0 <= padding_idx < table.shape[0]:
+        raise RuntimeError(f"padding_idx {padding_idx} is outside the table's {table.shape[0]} rows")
+    out_dtype = table.dtype if out_dtype is None else out_dtype
+    if out_dtype not in _be.ROW_DTYPES:
+        raise RuntimeError(f"out_dtype: unsupported type {out_dtype}")
+    return _embedding_rows.apply(indices, table, float(scale), padding_idx, out_dtype)
+
+
+class _gated_mlp_rows(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, w_down, activation):
+        lead, (hidden, dim) = x.shape[:-1], w_gate.shape
+        rows, wg, wu, wd = (_as_rows(t) for t in (x, w_gate, w_up, w_down))
+        save = any(ctx.needs_input_grad)
+        ctx.activation, ctx.lead = activation, lead
+        if rows.numel() == 0 or hidden == 0:
+            ctx.save_for_backward(x, w_gate, w_up, w_down)
+            ctx.empty = True
+            return x.new_zeros(*lead, dim)
+        ctx.empty = False
+        y = torch.empty(rows.shape[0], dim, device=x.device, dtype=x.dtype)
+        with torch.cuda.device(x.device):
+            saved = _be._backend.gated_mlp_fwd(rows, wg, wu, wd, activation, y, save)
+        if save:
+            ctx.save_for_backward(rows, wg, wu, wd, saved)
+        return y.view(*lead, dim)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        if ctx.empty:
+            return tuple(torch.zeros_like(t) if need else None for t, need in zip(ctx.saved_tensors, ctx.needs_input_grad)) + (None,)
+        rows, wg, wu, wd, saved = ctx.saved_tensors
+        gx, ggate, gup, gdown = (torch.empty(t.shape, device=t.device, dtype=t.dtype) if need else None for t, need in zip((rows, wg, wu, wd), ctx.needs_input_grad))
+        with torch.cuda.device(g.device):
+            _be._backend.gated_mlp_bwd(_as_rows(g), rows, wg, wu, wd, ctx.activation, saved, gx, ggate, gup, gdown)
+        return None if gx is None else gx.view(*ctx.lead, rows.shape[1]), ggate, gup, gdown, None
+
+
+def gated_mlp_rows(x, w_gate, w_up, w_down, activation="silu"):
+    """(act(x Wg^T) * (x Wu^T)) Wd^T for x [..., dim], w_gate and w_up [hidden, dim], w_down [dim, hidden], all of one type.
+
+    activation: "silu", "gelu" (g Phi(g)), "gelu_tanh" (its tanh form), "sigmoid", "relu".  float32 operands are multiplied as three bf16 planes each
+    (24 bits, as linear_rows under HOLOSCENE_FP32_GEMM=split3).  Rows may be strided; 16-bit operands whose rows are not 16-byte aligned are copied
+    once per call.  The forward keeps both projections and the gated product for the backward pass (3 * hidden elements a row)."""
+    _check_tensor(x, "x")
+    if x.dim() < 1:
+        raise RuntimeError("x must be [..., dim]")
+    for t, name in ((w_gate, "w_gate"), (w_up, "w_up"), (w_down, "w_down")):
+        _check_tensor(t, name, device=x.device, dtype=x.dtype)
+        if t.dim() != 2:
+            raise RuntimeError(f"{name} must be a matrix, got {tuple(t.shape)}")
+    hidden, dim = w_gate.shape
+    if x.shape[-1] != dim or w_up.shape != (hidden, dim) or w_down.shape != (dim, hidden):
+        raise RuntimeError(f"x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, w_up {tuple(w_up.shape)}, w_down {tuple(w_down.shape)}: expected [..., dim], "
+                           "[hidden, dim], [hidden, dim], [dim, hidden]")
+    if activation not in _be.ROW_ACTIVATIONS:
+        raise RuntimeError(f"activation must be one of {', '.join(ACTIVATIONS)}, got {activation!r}")
+    return _gated_mlp_rows.apply(x, w_gate, w_up, w_down, activation)
+
+
+class _dropout_rows(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, drop, rng):
+        y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        if y.numel():
+            with torch.cuda.device(x.device):
+                _be._backend.dropout_rows(x.contiguous(), None if residual is None else residual.contiguous(), y, drop, rng)
+        ctx.save_for_backward(rng)          # (autograd refuses the backward if rng has been written in the meantime)
+        ctx.drop = drop
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        rng, = ctx.saved_tensors
+        gx = None
+        if ctx.needs_input_grad[0]:
+            gx = torch.empty(g.shape, device=g.device, dtype=g.dtype)
+            if g.numel():
+                with torch.cuda.device(g.device):
+                    _be._backend.dropout_rows(g.contiguous(), None, gx, ctx.drop, rng)
+        return gx, g if ctx.needs_input_grad[1] else None, None, None
+
+
+def dropout_rows(x, p, rng, residual=None):
+    """Zeroes elements of x with probability p, scales the others by 1 / (1 - p), adds `residual` (same shape and type) if given.
+
+    rng: int64 [2] on x's device = (seed, number of the call).  The mask is a function of these two and the element's position in x (row-major,
+    whatever the strides) -- Philox-4x32-10, 16 bits an element, so p counts in steps of 2^-16 -- and is never stored: the backward pass computes it again
+    from the same rng, which therefore must not be written in between (autograd raises if it is).  Give every call its own number; inside a captured
+    graph add to rng[1] after the backward pass, so that each replay draws anew."""
+    _check_tensor(x, "x")
+    _check_tensor(rng, "rng", device=x.device, dtypes=(torch.int64,))
+    if tuple(rng.shape) != (2,) or not rng.is_contiguous():
+        raise RuntimeError("rng must be two consecutive int64 (seed, number of the call)")
+    if residual is not None:
+        _check_tensor(residual, "residual", device=x.device, dtype=x.dtype)
+        if residual.shape != x.shape:
+            raise RuntimeError(f"residual {tuple(residual.shape)} must have x's shape {tuple(x.shape)}")
+    if not 0.0 <= p <= 1.0:
+        raise RuntimeError(f"p must be in [0, 1], got {p}")
+    return _dropout_rows.apply(x, residual, math.floor(p * 65536 + 0.5), rng)
+
+
+class RowEmbedding(nn.Module):
+    """A table of `num` learned codes of `dim` elements, looked up by index (embedding_rows)."""
+
+    def __init__(self, num, dim, scale=1.0, padding_idx=None, std=1e-4):
+        super().__init__()
+        self.scale, self.padding_idx = scale, padding_idx
+        self.weight = nn.Parameter(torch.empty(num, dim).normal_(0.0, std))
+        if padding_idx is not None:
+            with torch.no_grad():
+                self.weight[padding_idx].zero_()
+
+    def forward(self, indices):
+        return embedding_rows(indices, self.weight, self.scale, self.padding_idx)
+
+
+class GatedMLP(nn.Module):
+    """The gated feed-forward block (gated_mlp_rows) with its three weights."""
+
+    def __init__(self, dim, hidden, activation="silu"):
+        super().__init__()
+        if activation not in _be.ROW_ACTIVATIONS:
+            raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}, got {activation!r}")
+        self.activation = activation
+        self.w_gate = nn.Parameter(nn.Linear(dim, hidden, bias=False).weight.detach().clone())
+        self.w_up = nn.Parameter(nn.Linear(dim, hidden, bias=False).weight.detach().clone())
+        self.w_down = nn.Parameter(nn.Linear(hidden, dim, bias=False).weight.detach().clone())
+
+    def forward(self, x):
+        return gated_mlp_rows(x, self.w_gate, self.w_up, self.w_down, self.activation)
+
+
+class RowDropout(nn.Module):
+    """Dropout (dropout_rows) with a generator state of its own: a buffer (seed, number of the next call), advanced on the device by every
+    call in training mode, so that eager calls and replays of a captured graph alike draw a new mask each time."""
+
+    def __init__(self, p, seed=0):
+        super().__init__()
+        if not 0.0 <= p <= 1.0:
+            raise ValueError(f"p must be in [0, 1], got {p}")
+        self.p = p
+        self.register_buffer("rng", torch.tensor([seed, 0], dtype=torch.int64))
+
+    def forward(self, x, residual=None):
+        if not self.training or self.p == 0.0:
+            return x if residual is None else x + residual
+        used = self.rng.clone()
+        self.rng[1:].add_(1)
+        return dropout_rows(x, self.p, used, residual)

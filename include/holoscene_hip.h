@@ -39,6 +39,7 @@ extern "C" {
 /* storage types of activation tensors */
 #define HS_F32 0
 #define HS_BF16 1
+#define HS_F16 2        /* the row operators of section 10 only */
 
 /* ------------------------------------------------------------------ 0. library info */
 /* ABI version; bumped whenever a signature below changes. */
@@ -888,6 +889,51 @@ int hs_loss_stage1(const float *rgb, const float *rgb_gt, const float *depth, co
  * depth [P], normal [P,3] (pixel-major), labels int64 [P], P = side^2.  out[0] = the loss, g_depth / g_normal = its gradient. */
 int hs_bg_smooth_loss(const float *depth, const float *normal, const int64_t *labels, int32_t side, float *out, float *g_depth, float *g_normal,
                       void *stream);
+
+/* ------------------------------------------------------------------ 10. row operators
+ *
+ * Codes looked up by index, the gated feed-forward block and counter-based dropout, in fp32 / bf16 / fp16 storage (HS_F32, HS_BF16, HS_F16) with fp32
+ * arithmetic and one rounding per result.  Work spaces and saved buffers are the caller's, 256-byte aligned; nothing in them has to be
+ * initialised and nothing is kept in them from call to call (`saved`: from a forward to its backward). */
+
+/* out [n, D] = scale * table[indices]; table [V, D] with row distance ld, indices int32 / int64 (index_bytes 4 / 8).  An index outside [0, V) reads zeros. */
+int hs_embed_fwd(const void *indices, int32_t index_bytes, const void *table, int64_t ld, void *out, int64_t n, int64_t V, int64_t D, float scale, int32_t table_dtype,
+                 int32_t out_dtype, void *stream);
+/* grad_table [V, D] (written whole, contiguous) = scale * sums of grad's rows [n, D] (row distance ldg) by index, each in the order of the positions.  Indices outside
+ * [0, V) and `padding` (-1: none) take no gradient.  ws: hs_embed_bwd_ws_bytes(n, V, D). */
+int64_t hs_embed_bwd_ws_bytes(int64_t n, int64_t V, int64_t D);
+int hs_embed_bwd(const void *indices, int32_t index_bytes, const void *grad, int64_t ldg, void *grad_table, int64_t n, int64_t V, int64_t D, float scale, int64_t padding,
+                 int32_t grad_dtype, int32_t table_dtype, void *ws, int64_t ws_bytes, void *stream);
+
+/* y_i = (u_i >= drop ? x_i * 65536 / (65536 - drop) : 0) + residual_i, u_i = 16 bits of Philox-4x32-10 with key rng[0] and counter (i / 8, rng[1]): word (i % 8) / 2, low half
+ * first.  rng: DEVICE uint64[2] (seed, number of the call), read only.  drop in [0, 65536] (65536: everything).  residual may be NULL; y may be x or residual. */
+int hs_dropout_rows(const void *x, const void *residual, void *y, int64_t n, int32_t dtype, int32_t drop, const uint64_t *rng, void *stream);
+
+/* y = (act(x Wg^T) * (x Wu^T)) Wd^T and its gradient; x [rows, dim], Wg, Wu [hidden, dim], Wd [dim, hidden], every one with a row distance of its own; y and the
+ * gradients contiguous.  All three sizes > 0. */
+#define HS_ACT_SILU 0
+#define HS_ACT_GELU 1           /* g Phi(g) */
+#define HS_ACT_GELU_TANH 2
+#define HS_ACT_SIGMOID 3
+#define HS_ACT_RELU 4
+typedef struct hsGatedMlp {
+    const void *x, *w_gate, *w_up, *w_down;
+    int64_t ldx, ld_gate, ld_up, ld_down;       /* in elements */
+    int64_t rows, dim, hidden;
+    int32_t dtype, activation;
+    void *y;                                    /* fwd: [rows, dim] */
+    void *saved;                                /* fwd: NULL, or written for the backward; bwd: as the forward left it */
+    const void *grad;                           /* bwd: dLoss/dy [rows, dim], row distance ld_grad */
+    int64_t ld_grad;
+    void *gx, *gw_gate, *gw_up, *gw_down;       /* bwd: each may be NULL (not computed) */
+    void *ws;
+    int64_t ws_bytes;
+} hsGatedMlp;
+int64_t hs_gated_mlp_saved_bytes(const hsGatedMlp *args);
+int64_t hs_gated_mlp_fwd_ws_bytes(const hsGatedMlp *args);      /* (of these very arguments: what is copied depends on their alignment) */
+int64_t hs_gated_mlp_bwd_ws_bytes(const hsGatedMlp *args);
+int hs_gated_mlp_fwd(const hsGatedMlp *args, void *stream);
+int hs_gated_mlp_bwd(const hsGatedMlp *args, void *stream);
 
 #ifdef __cplusplus
 }
