@@ -2,7 +2,8 @@
 //     G = x Wg^T, U = x Wu^T, H = act(G) U (one launch), y = H Wd^T;
 //     gH = gy Wd, gg = gH U act'(G), gu = gH act(G) (one launch), gx = gg Wg + gu Wu, gWg = gg^T x, gWu = gu^T x (one launch), gWd = gy^T H.
 // Roundings besides the results' own: H, gg and gu to the operand type, because the matrix cores multiply 16-bit operands (fp32: as three bf16 planes,
-// 24 bits); G and U to the user's type where the backward pass will read them again (the forward pass uses them unrounded).
+// 24 bits).  G and U are never rounded: the forward keeps them in fp32 for the backward pass, or the backward pass computes them again (k_gate_bwd) where that
+// moves fewer bytes than it costs products.
 #pragma once
 #include "rows_gemm.h"
 
@@ -100,6 +101,10 @@ template <typename U> int add_segments(Seg *seg, int n, const Operand &a, const 
 
 template <typename U> constexpr int planes() { return sizeof(U) == 4 ? 3 : 1; }
 
+// Up to this D the backward pass computes G and U again: 4 D operations an element against 16 bytes.  (At D = 256, 131 072 x 1 024: forward and this part of the
+// backward 660 us against 780 with G and U kept.)
+constexpr int64_t kAgainDim = 768;
+
 template <typename T, typename U> struct Block {
     const hsGatedMlp &a;
     Arena ws;
@@ -137,12 +142,15 @@ template <typename T, typename U> struct Block {
         }
     }
 
-    struct Saved { U *g, *u; Operand h; int64_t bytes; };
+    // whether the backward pass computes G and U again instead of reading them
+    bool again() const { return D <= kAgainDim; }
+
+    struct Saved { float *g, *u; Operand h; int64_t bytes; };
     Saved saved_in(char *base) const {
         Saved v = {};
-        const int64_t n = M * ldh, gu = (n * (int64_t)sizeof(U) + 255) / 256 * 256;
-        v.g = (U *)base;
-        v.u = (U *)(base + gu);
+        const int64_t n = M * ldh, gu = again() ? 0 : (n * 4 + 255) / 256 * 256;
+        v.g = gu ? (float *)base : nullptr;
+        v.u = gu ? (float *)(base + gu) : nullptr;
         v.h = Operand{base + 2 * gu, ldh, n};
         v.bytes = 2 * gu + n * 2 * planes<U>();
         return v;
@@ -207,16 +215,25 @@ template <typename T, typename U> struct Block {
             const Operand wd = operand(a.w_down, a.ld_down, D, F);
             const int64_t n = M * ldh;
             const Operand gg{ws.take(n * 2 * planes<U>()), ldh, n}, gu{ws.take(n * 2 * planes<U>()), ldh, n};
-            if (run && fits<false, true>(gy, wd)) {
+            Operand wg, wu, x;
+            if (again() || a.gx) projections(wg, wu);
+            if (again() || a.gw_gate || a.gw_up) x = operand(a.x, a.ldx, M, D);
+            if (run && fits<false, true>(gy, wd) && (!again() || fits<false, false>(x, wg))) {
                 Args p = {};
-                p.n_seg = add_segments<U>(p.seg[0], 0, gy, wd);
-                p.lda = gy.ld; p.ldb = wd.ld; p.I = M; p.J = (int)F; p.K = (int)D; p.slices = 1;
+                p.I = M; p.J = (int)F; p.K = (int)D; p.slices = 1;
                 p.g = sv.g; p.u = sv.u; p.gg = (void *)gg.p; p.gu = (void *)gu.p; p.ldh = ldh; p.plane = n; p.act = a.activation;
-                check(launch_product<T, U, false, true, EPI_GATE_BWD>(p, 1, s));
+                if (again()) {
+                    p.n_seg = add_segments<U>(p.seg[0], 0, x, wg, &wu);
+                    add_segments<U>(p.seg[1], 0, gy, wd);
+                    p.lda = x.ld; p.ldb = wg.ld; p.lda2 = gy.ld; p.ldb2 = wd.ld;
+                    check(launch_gate_bwd<T, U>(p, s));
+                } else {
+                    p.n_seg = add_segments<U>(p.seg[0], 0, gy, wd);
+                    p.lda = gy.ld; p.ldb = wd.ld;
+                    check(launch_product<T, U, false, true, EPI_GATE_BWD>(p, 1, s));
+                }
             }
             if (a.gx) {
-                Operand wg, wu;
-                projections(wg, wu);
                 if (run && fits<false, true>(gg, wg)) {
                     Args p = {};
                     p.n_seg = add_segments<U>(p.seg[0], 0, gg, wg);
@@ -227,7 +244,6 @@ template <typename T, typename U> struct Block {
                 }
             }
             if (a.gw_gate || a.gw_up) {
-                const Operand x = operand(a.x, a.ldx, M, D);
                 const Operand av[2] = {a.gw_gate ? gg : gu, gu};
                 void *const out[2] = {a.gw_gate ? a.gw_gate : a.gw_up, a.gw_up};
                 weight_gradient(av, x, out, a.gw_gate && a.gw_up ? 2 : 1, F, D);

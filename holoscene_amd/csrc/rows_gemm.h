@@ -18,6 +18,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <type_traits>
+#include <utility>
 
 #include "holoscene_hip.h"
 #include "launch_util.h"
@@ -50,78 +51,97 @@ struct Args {
     void *out[2];                                 // per problem
     int64_t ldo;
     int64_t slice_stride;                         // elements between partial results (slices > 1: fp32)
-    // gate epilogues: G, U [I, ldh] in the user's type; H or (gg, gu) as operands [planes][I][ldh]
-    void *g, *u, *h, *gg, *gu;
-    int64_t ldh, plane;                           // elements between planes
+    // gate kernels: G, U fp32 [I, ldh]; H or (gg, gu) as operands [planes][I][ldh]
+    float *g, *u;
+    void *h, *gg, *gu;
+    int64_t ldh, plane;                           // plane: elements between planes
     int32_t act;
+    // k_gate_bwd: the second product's operands are seg[1]
+    int64_t lda2, ldb2;
 };
 
-enum { EPI_STORE = 0, EPI_PARTIAL = 1, EPI_GATE = 2, EPI_GATE_BWD = 3 };
+enum { EPI_STORE = 0, EPI_PARTIAL = 1, EPI_GATE = 2, EPI_GATE_BWD = 3 };       // result; fp32 partial result; H (G, U); gg, gu from G, U
 
 // ------------------------------------------------------------------------------------------------ activations (fp32)
-// act(g) and, with `d`, act'(g).  expf / erff / tanhf are the library's fp32 functions.
-__device__ __forceinline__ float activation(int act, float g, float *d) {
-    if (act == HS_ACT_SILU || act == HS_ACT_SIGMOID) {
-        const float s = 1.f / (1.f + expf(-g));
-        if (act == HS_ACT_SIGMOID) {
-            if (d) *d = s * (1.f - s);
-            return s;
-        }
-        if (d) *d = s * (1.f + g * (1.f - s));
+// act(g) and, with D, act'(g).  The logistic function is v_exp_f32 and v_rcp_f32 (one step each): its error is |g| 2^-24 relative to s (1 - s), below the
+// rounding of g itself.  gelu_tanh: (1 + tanh z) / 2 is the logistic function of 2 z, so no difference of nearly equal numbers is formed.
+__device__ __forceinline__ float logistic(float v) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f)); }
+
+template <int ACT, bool D> __device__ __forceinline__ float activation(float g, float &d) {
+    if constexpr (ACT == HS_ACT_SILU) {
+        const float s = logistic(g);
+        if constexpr (D) d = s * (1.f + g * (1.f - s));
+        return g * s;
+    } else if constexpr (ACT == HS_ACT_SIGMOID) {
+        const float s = logistic(g);
+        if constexpr (D) d = s * (1.f - s);
+        return s;
+    } else if constexpr (ACT == HS_ACT_RELU) {
+        if constexpr (D) d = g > 0.f ? 1.f : 0.f;
+        return g > 0.f ? g : (g == g ? 0.f : g);        // (a NaN stays one)
+    } else if constexpr (ACT == HS_ACT_GELU) {
+        const float c = 0.5f * (1.f + erff(g * 0.70710678118654752f));
+        if constexpr (D) d = c + g * __builtin_amdgcn_exp2f(g * g * -0.72134752044448170f) * 0.39894228040143268f;
+        return g * c;
+    } else {                                            // HS_ACT_GELU_TANH: 2 sqrt(2 / pi) (g + 0.044715 g^3)
+        const float s = logistic(1.5957691216057308f * (g + 0.044715f * g * g * g));
+        if constexpr (D) d = s + g * s * (1.f - s) * 1.5957691216057308f * (1.f + 0.134145f * g * g);
         return g * s;
     }
-    if (act == HS_ACT_RELU) {
-        if (d) *d = g > 0.f ? 1.f : 0.f;
-        return g > 0.f ? g : (g == g ? 0.f : g);
+}
+
+// f(std::integral_constant<int, act>): the activation as a constant, one uniform branch for a whole epilogue
+template <typename F> __device__ __forceinline__ void with_activation(int act, F f) {
+    switch (act) {
+        case HS_ACT_SILU: f(std::integral_constant<int, HS_ACT_SILU>{}); break;
+        case HS_ACT_GELU: f(std::integral_constant<int, HS_ACT_GELU>{}); break;
+        case HS_ACT_GELU_TANH: f(std::integral_constant<int, HS_ACT_GELU_TANH>{}); break;
+        case HS_ACT_SIGMOID: f(std::integral_constant<int, HS_ACT_SIGMOID>{}); break;
+        default: f(std::integral_constant<int, HS_ACT_RELU>{}); break;
     }
-    if (act == HS_ACT_GELU) {
-        const float c = 0.5f * (1.f + erff(g * 0.70710678118654752f));
-        if (d) *d = c + g * expf(-0.5f * g * g) * 0.39894228040143268f;
-        return g * c;
-    }
-    const float k = 0.79788456080286536f, t = tanhf(k * (g + 0.044715f * g * g * g));       // HS_ACT_GELU_TANH
-    if (d) *d = 0.5f * (1.f + t) + 0.5f * g * (1.f - t * t) * k * (1.f + 0.134145f * g * g);
-    return 0.5f * g * (1.f + t);
 }
 
 // ------------------------------------------------------------------------------------------------ three bf16 planes of an fp32 value
 // v = p0 + p1 + p2 up to 2^-24 |v|.  A value that rounds to infinity is cut instead of rounded, an infinity or NaN stays in plane 0 alone.
 __device__ __forceinline__ void split3(float v, bf16_t (&p)[3]) {
     const uint32_t bits = __float_as_uint(v);
-    p[0] = (bf16_t)v;
-    float r = (float)p[0];
-    if (((bits >> 23) & 0xffu) == 0xffu) {
-        p[1] = p[2] = (bf16_t)0.f;
-        return;
-    }
-    if (((__float_as_uint(r) >> 23) & 0xffu) == 0xffu) {
-        r = __uint_as_float(bits & 0xffff0000u);
-        p[0] = (bf16_t)r;
-    }
-    v -= r;
-    p[1] = (bf16_t)v;
-    v -= (float)p[1];
-    p[2] = (bf16_t)v;
+    const bool finite = ((bits >> 23) & 0xffu) != 0xffu, big = (bits & 0x7fffffffu) >= 0x7f7f8000u;       // big: rounds to infinity (or is one)
+    const float first = finite && big ? __uint_as_float(bits & 0xffff0000u) : v;
+    p[0] = (bf16_t)first;
+    const float r1 = finite ? v - (float)p[0] : 0.f;
+    p[1] = (bf16_t)r1;
+    p[2] = (bf16_t)(r1 - (float)p[1]);
 }
 
-// four consecutive elements of an operand that a later product reads: one plane in the 16-bit types, three for fp32
-template <typename T, typename U> __device__ __forceinline__ void store_operand4(void *base, int64_t plane, int64_t at, const float (&v)[4]) {
+// eight consecutive elements of an operand that a later product reads: one plane in the 16-bit types, three for fp32
+template <typename U> __device__ __forceinline__ void store_operand8(void *base, int64_t plane, int64_t at, const float (&v)[8]) {
     if constexpr (sizeof(U) == 4) {
-        Pack<bf16_t, 4> o[3];
+        Pack<bf16_t, 8> o[3];
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
+        for (int e = 0; e < 8; e++) {
             bf16_t p[3];
             split3(v[e], p);
             o[0].v[e] = p[0]; o[1].v[e] = p[1]; o[2].v[e] = p[2];
         }
 #pragma unroll
-        for (int q = 0; q < 3; q++) *reinterpret_cast<Pack<bf16_t, 4> *>((bf16_t *)base + q * plane + at) = o[q];
+        for (int q = 0; q < 3; q++) *reinterpret_cast<Pack<bf16_t, 8> *>((bf16_t *)base + q * plane + at) = o[q];
     } else {
-        Pack<U, 4> o;
+        Pack<U, 8> o;
 #pragma unroll
-        for (int e = 0; e < 4; e++) o.v[e] = from_f32<U>(v[e]);
-        *reinterpret_cast<Pack<U, 4> *>((U *)base + at) = o;
+        for (int e = 0; e < 8; e++) o.v[e] = from_f32<U>(v[e]);
+        *reinterpret_cast<Pack<U, 8> *>((U *)base + at) = o;
     }
+}
+
+// eight consecutive floats
+struct F8 { float v[8]; };
+__device__ __forceinline__ F8 load8(const float *p) {
+    const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
+    return F8{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+}
+__device__ __forceinline__ void store8(float *p, const F8 &f) {
+    reinterpret_cast<float4 *>(p)[0] = make_float4(f.v[0], f.v[1], f.v[2], f.v[3]);
+    reinterpret_cast<float4 *>(p)[1] = make_float4(f.v[4], f.v[5], f.v[6], f.v[7]);
 }
 
 // ------------------------------------------------------------------------------------------------ the kernel
@@ -139,6 +159,8 @@ __device__ __forceinline__ void dma16(const i32x4 &desc, uint32_t voff, uint32_t
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to_lds), "v"(voff), "s"(desc) : "memory");
 }
 __device__ __forceinline__ void wait_and_meet() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+__device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }       // LDS only: stores to global memory stay in flight
 
 template <typename T> __device__ __forceinline__ f32x4 mfma(i16x8 a, i16x8 b, f32x4 c) {
     if constexpr (__is_same(T, bf16_t)) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -218,6 +240,57 @@ template <int R, bool KS, int WAVES, int OWN> struct Side {
     }
 };
 
+// Which tile a workgroup takes: eight contiguous ranges of tiles, one per XCD (workgroups go round the XCDs), each walked in groups of 8 row tiles so that the
+// tiles in flight on an XCD share operands in its L2.
+struct TilePlace { int i, j; };
+__device__ __forceinline__ TilePlace tile_place(int tiles_i, int tiles_j) {
+    const int n = tiles_i * tiles_j, per_xcd = n / 8, rest = n % 8, xcd = blockIdx.x % 8;
+    const int t = xcd * per_xcd + (xcd < rest ? xcd : rest) + blockIdx.x / 8;
+    const int group = t / (8 * tiles_j), in = t - group * 8 * tiles_j, rows = tiles_i - group * 8 < 8 ? tiles_i - group * 8 : 8;
+    return TilePlace{group * 8 + in % rows, in / rows};
+}
+
+// Accumulators through LDS as a tile of fp32 rows: MP of each wave's MT row groups at a time, COLS columns of fp32 a row, items of 8 of the TJ result columns.
+template <int COLS, int MT, int MP_, int WI, int WAVES, int TJ> struct Staging {
+    static constexpr int MP = MP_, kPasses = MT / MP, kLines = WI * MP * 16, kPitch = COLS + 4, kItems = kLines * (TJ / 8), kIter = kItems / (64 * WAVES);
+    static constexpr int kBytes = kLines * kPitch * 4;
+    static_assert(kItems % (64 * WAVES) == 0 && kIter >= 1, "items must fill the workgroup");
+    static __device__ __forceinline__ int line(int tid, int k) { return (tid + k * 64 * WAVES) / (TJ / 8); }
+    static __device__ __forceinline__ int col(int tid, int k) { return (tid + k * 64 * WAVES) % (TJ / 8) * 8; }
+    static __device__ __forceinline__ int row(int tid, int pass, int k) {
+        const int r = line(tid, k);
+        return r / (MP * 16) * (MT * 16) + pass * MP * 16 + r % (MP * 16);
+    }
+};
+
+template <int... I, typename F> __device__ __forceinline__ void static_for(std::integer_sequence<int, I...>, F f) { (f(std::integral_constant<int, I>{}), ...); }
+
+// One step (64 of K) of a wave's products.  Fragments are requested PF groups of matrix instructions ahead of their use, and the order written here is pinned
+// (sched_group_barrier: 0x100 LDS reads, 0x8 matrix instructions): left to itself the compiler puts every read directly in front of its use, with a wait for
+// its whole latency between.  a(m, ks), b(n, ks): the fragments; RA, RB: LDS instructions of one.  request(): the next step's LDS-DMA, issued while the
+// first fragments are on their way.
+template <typename T, int MT, int NT, int RA, int RB, typename A, typename B, typename R>
+__device__ __forceinline__ void multiply_step(A a, B b, R request, f32x4 (&acc)[MT][NT]) {
+    constexpr int G = 2 * MT, PF = MT >= 4 ? 3 : 2;
+    i16x8 fa[G], fb[2][NT];
+#pragma unroll
+    for (int n = 0; n < NT; n++) fb[0][n] = b(n, 0);
+#pragma unroll
+    for (int g = 0; g < PF; g++) fa[g] = a(g % MT, g / MT);
+    request();
+    static_for(std::make_integer_sequence<int, G>{}, [&](auto group) {
+        constexpr int g = decltype(group)::value, b0 = g < MT ? g * NT / MT : NT, b1 = g < MT ? (g + 1) * NT / MT : NT;
+        constexpr int reads = (g + PF < G ? RA : 0) + (b1 - b0) * RB;
+        if constexpr (g + PF < G) fa[g + PF] = a((g + PF) % MT, (g + PF) / MT);
+#pragma unroll
+        for (int n = b0; n < b1; n++) fb[1][n] = b(n, 1);
+#pragma unroll
+        for (int n = 0; n < NT; n++) acc[g % MT][n] = mfma<T>(fb[g / MT][n], fa[g], acc[g % MT][n]);
+        if constexpr (reads > 0) __builtin_amdgcn_sched_group_barrier(0x100, reads, 0);
+        __builtin_amdgcn_sched_group_barrier(0x8, NT, 0);
+    });
+}
+
 // T: the matrix instruction's type; U: the user's type (float: T = bf16, planes).
 template <typename T, typename U, int BM, int BN, int WI, int WJ, bool AKS, bool BKS, int EPI>
 __global__ __launch_bounds__(64 * WI * WJ) void k_rows_gemm(const Args p) {
@@ -228,13 +301,9 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_rows_gemm(const Args p) {
     using SB = Side<BN, BKS, WAVES, NT>;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wi = wave / WJ, wj = wave % WJ;
-    // tiles: eight contiguous ranges, one per XCD (workgroups go round the XCDs), each walked in groups of 8 row tiles so that the tiles in flight
-    // on an XCD share operands in its L2
-    const int n_tiles = p.tiles_i * p.tiles_j, per_xcd = n_tiles / 8, rest = n_tiles % 8, xcd = blockIdx.x % 8, nth = blockIdx.x / 8;
-    const int t = xcd * per_xcd + (xcd < rest ? xcd : rest) + nth;
-    const int group = t / (8 * p.tiles_j), in_group = t - group * 8 * p.tiles_j, gi = p.tiles_i - group * 8 < 8 ? p.tiles_i - group * 8 : 8;
-    const int64_t i0 = (int64_t)(group * 8 + in_group % gi) * BM;
-    const int j0 = (in_group / gi) * TJ;
+    const TilePlace t = tile_place(p.tiles_i, p.tiles_j);
+    const int64_t i0 = (int64_t)t.i * BM;
+    const int j0 = t.j * TJ;
     const Seg *segs = p.seg[blockIdx.z];
 
     SA sa;
@@ -248,49 +317,55 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_rows_gemm(const Args p) {
     const int s_begin = (int)((int64_t)steps * blockIdx.y / p.slices), s_end = (int)((int64_t)steps * (blockIdx.y + 1) / p.slices);
     const int64_t a_step = AKS ? BK * p.lda * 2 : BK * 2, b_step = BKS ? BK * p.ldb * 2 : BK * 2;
     const int64_t a_tile = AKS ? i0 * 2 : i0 * p.lda * 2, b_tile = BKS ? (int64_t)j0 * 2 : (int64_t)j0 * p.ldb * 2;
-    auto request = [&](int s, int buf) {
-        const int sg = s / steps_k, kk = s - sg * steps_k;
-        const char *a = (const char *)segs[sg].a + a_tile + kk * a_step, *b = (const char *)segs[sg].b + b_tile + kk * b_step;
-        const char *b1 = DUAL ? (const char *)segs[sg].b1 + b_tile + kk * b_step : b;
+    int sg = s_begin / (steps_k ? steps_k : 1), kk = s_begin - sg * steps_k;       // the next request's segment and step, and its operands' addresses
+    const char *pa, *pb, *pb1;
+    auto point = [&]() {
+        pa = (const char *)segs[sg].a + a_tile + kk * a_step;
+        pb = (const char *)segs[sg].b + b_tile + kk * b_step;
+        pb1 = DUAL ? (const char *)segs[sg].b1 + b_tile + kk * b_step : pb;
+    };
+    auto request = [&](int buf) {
         const int64_t left = p.K - (int64_t)kk * BK;
         const uint32_t at = lds0 + (uint32_t)buf * (SA::kBytes + SB::kBytes);
-        sa.request(wave, a, a, left, at);
-        sb.request(wave, b, b1, left, at + SA::kBytes);
+        sa.request(wave, pa, pa, left, at);
+        sb.request(wave, pb, DUAL ? pb1 : pb, left, at + SA::kBytes);
+        pa += a_step;
+        pb += b_step;
+        if constexpr (DUAL) pb1 += b_step;
+        if (++kk == steps_k) {
+            kk = 0;
+            if (++sg < p.n_seg) point();
+        }
     };
     f32x4 acc[MT][NT];
 #pragma unroll
     for (int m = 0; m < MT; m++)
 #pragma unroll
         for (int n = 0; n < NT; n++) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (s_begin < s_end) request(s_begin, 0);
+    if (s_begin < s_end) {
+        point();
+        request(0);
+    }
     int buf = 0;
     for (int s = s_begin; s < s_end; s++) {
         wait_and_meet();            // step s has landed for every wave; every wave is done with the other buffer
-        if (s + 1 < s_end) request(s + 1, buf ^ 1);
         const uint32_t at = lds0 + (uint32_t)buf * (SA::kBytes + SB::kBytes);
-#pragma unroll
-        for (int ks = 0; ks < 2; ks++) {
-            i16x8 fa[MT], fb[NT];
-#pragma unroll
-            for (int n = 0; n < NT; n++)         // (the tile's upper half: the up projection's rows)
-                fb[n] = DUAL && n >= NT / 2 ? sb.fragment(at + SA::kBytes, n - NT / 2, ks, BN / 2) : sb.fragment(at + SA::kBytes, n, ks);
-#pragma unroll
-            for (int m = 0; m < MT; m++) fa[m] = sa.fragment(at, m, ks);
-#pragma unroll
-            for (int m = 0; m < MT; m++)
-#pragma unroll
-                for (int n = 0; n < NT; n++) acc[m][n] = mfma<T>(fb[n], fa[m], acc[m][n]);
-        }
+        multiply_step<T, MT, NT, AKS ? 2 : 1, BKS ? 2 : 1>(
+            [&](int m, int ks) { return sa.fragment(at, m, ks); },
+            [&](int n, int ks) {         // (EPI_GATE: the tile's upper half is the up projection's rows)
+                return DUAL && n >= NT / 2 ? sb.fragment(at + SA::kBytes, n - NT / 2, ks, BN / 2) : sb.fragment(at + SA::kBytes, n, ks);
+            },
+            [&]() { if (s + 1 < s_end) request(buf ^ 1); }, acc);
         buf ^= 1;
     }
 
     // ---- epilogue: acc[m][n][r] is row i0 + 16 (wi MT + m) + (lane & 15), column 16 unit + 4 (lane >> 4) + r
     const int li = lane & 15, lq = lane >> 4;
+    if constexpr (EPI == EPI_STORE || EPI == EPI_PARTIAL) {
 #pragma unroll
-    for (int m = 0; m < MT; m++) {
-        const int64_t i = i0 + (wi * MT + m) * 16 + li;
-        if (i >= p.I) continue;
-        if constexpr (EPI == EPI_STORE || EPI == EPI_PARTIAL) {
+        for (int m = 0; m < MT; m++) {
+            const int64_t i = i0 + (wi * MT + m) * 16 + li;
+            if (i >= p.I) continue;
             using O = typename std::conditional<EPI == EPI_PARTIAL, float, U>::type;
             O *row = (O *)p.out[blockIdx.z] + (EPI == EPI_PARTIAL ? (int64_t)blockIdx.y * p.slice_stride : 0) + i * p.ldo;
             const bool wide = p.ldo % 4 == 0 && (uintptr_t)p.out[blockIdx.z] % (4 * sizeof(O)) == 0;
@@ -306,47 +381,74 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_rows_gemm(const Args p) {
                     for (int r = 0; r < 4; r++)
                         if (j + r < p.J) row[j + r] = o.v[r];
             }
-        } else if constexpr (EPI == EPI_GATE) {
-            // columns up to ldh are written: behind J both projections are zero (nothing was read), so the padding of G, U and H is zero
-#pragma unroll
-            for (int n = 0; n < NT / 2; n++) {
-                const int j = j0 + (wj * (NT / 2) + n) * 16 + lq * 4;
-                if (j >= p.ldh) continue;
-                float h[4];
-                Pack<U, 4> go, uo;
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const float g = acc[m][n][r], u = acc[m][n + NT / 2][r];
-                    go.v[r] = from_f32<U>(g);
-                    uo.v[r] = from_f32<U>(u);
-                    h[r] = activation(p.act, g, nullptr) * u;
-                }
-                const int64_t at = i * p.ldh + j;
-                if (p.g) {
-                    *reinterpret_cast<Pack<U, 4> *>((U *)p.g + at) = go;
-                    *reinterpret_cast<Pack<U, 4> *>((U *)p.u + at) = uo;
-                }
-                store_operand4<T, U>(p.h, p.plane, at, h);
-            }
-        } else {
-#pragma unroll
-            for (int n = 0; n < NT; n++) {
-                const int j = j0 + (wj * NT + n) * 16 + lq * 4;
-                if (j >= p.ldh) continue;
-                const int64_t at = i * p.ldh + j;
-                const Pack<U, 4> gi_ = *reinterpret_cast<const Pack<U, 4> *>((const U *)p.g + at), ui_ = *reinterpret_cast<const Pack<U, 4> *>((const U *)p.u + at);
-                float gg[4], gu[4];
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    float d;
-                    const float a = activation(p.act, to_f32(gi_.v[r]), &d), gh = acc[m][n][r];
-                    gg[r] = gh * to_f32(ui_.v[r]) * d;
-                    gu[r] = gh * a;
-                }
-                store_operand4<T, U>(p.gg, p.plane, at, gg);
-                store_operand4<T, U>(p.gu, p.plane, at, gu);
-            }
         }
+    } else {
+        // Through LDS, MP row groups of every wave at a time, so that the elementwise part is a short loop over 8 consecutive columns a thread (full lines of
+        // global memory, one copy of the activation's code: unrolled over the accumulators it did not fit the instruction cache and took longer than
+        // the products).  Columns up to ldh are written: behind J nothing was read, so the padding of G, U, H, gg and gu is zero.
+        using St = Staging<BN, MT, EPI == EPI_GATE_BWD ? 1 : 2, WI, WAVES, TJ>;     // (G and U of a whole pass are in registers: 16 a thread and item)
+        F8 gq[St::kIter], uq[St::kIter];
+        auto fetch = [&](int pass, int k) {                 // (clamped: nothing branches between the requests)
+            int64_t i = i0 + St::row(tid, pass, k), j = j0 + St::col(tid, k);
+            i = i < p.I ? i : p.I - 1;
+            j = j < p.ldh ? j : p.ldh - 8;
+            gq[k] = load8(p.g + i * p.ldh + j);
+            uq[k] = load8(p.u + i * p.ldh + j);
+        };
+        if constexpr (EPI == EPI_GATE_BWD) {
+#pragma unroll
+            for (int k = 0; k < St::kIter; k++) fetch(0, k);
+        }
+        float *stage = reinterpret_cast<float *>(lds);
+        with_activation(p.act, [&](auto act) {
+            constexpr int ACT = decltype(act)::value;
+#pragma unroll
+            for (int pass = 0; pass < St::kPasses; pass++) {
+                meet();
+#pragma unroll
+                for (int m = 0; m < St::MP; m++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        const int col = DUAL ? (n < NT / 2 ? (wj * (NT / 2) + n) * 16 : BN / 2 + (wj * (NT / 2) + n - NT / 2) * 16) : (wj * NT + n) * 16;
+                        *reinterpret_cast<f32x4 *>(stage + ((wi * St::MP + m) * 16 + li) * St::kPitch + col + lq * 4) = acc[pass * St::MP + m][n];
+                    }
+                meet();
+#pragma unroll
+                for (int k = 0; k < St::kIter; k++) {
+                    const int64_t i = i0 + St::row(tid, pass, k), at = i * p.ldh + j0 + St::col(tid, k);
+                    const bool in = i < p.I && j0 + St::col(tid, k) < p.ldh;
+                    const float *s = stage + St::line(tid, k) * St::kPitch + St::col(tid, k);
+                    const F8 a = load8(s);
+                    float unused;
+                    if constexpr (EPI == EPI_GATE) {
+                        const F8 u = load8(s + BN / 2);
+                        F8 h;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) h.v[e] = activation<ACT, false>(a.v[e], unused) * u.v[e];
+                        if (in) {
+                            if (p.g) {
+                                store8(p.g + at, a);
+                                store8(p.u + at, u);
+                            }
+                            store_operand8<U>(p.h, p.plane, at, h.v);
+                        }
+                    } else {
+                        F8 gg, gu;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            float d;
+                            gu.v[e] = a.v[e] * activation<ACT, true>(gq[k].v[e], d);
+                            gg.v[e] = a.v[e] * uq[k].v[e] * d;
+                        }
+                        if (pass + 1 < St::kPasses) fetch(pass + 1, k);
+                        if (in) {
+                            store_operand8<U>(p.gg, p.plane, at, gg.v);
+                            store_operand8<U>(p.gu, p.plane, at, gu.v);
+                        }
+                    }
+                }
+            }
+        });
     }
 }
 
@@ -360,10 +462,143 @@ inline int launch_tile(Args &p, int problems, hipStream_t s) {
     p.tiles_i = (int)ti;
     p.tiles_j = (int)tj;
     constexpr int lds = 2 * (BM + BN) * BK * 2;
+    static_assert(Staging<BN, BM / WI / 16, 2, WI, WI * WJ, TJ>::kBytes <= lds, "the epilogue's tile must fit");
     static hsLdsAttrOnce attr;
     const void *fn = (const void *)k_rows_gemm<T, U, BM, BN, WI, WJ, AKS, BKS, EPI>;
     attr.set(fn, lds);
     k_rows_gemm<T, U, BM, BN, WI, WJ, AKS, BKS, EPI><<<dim3((unsigned)(ti * tj), (unsigned)p.slices, (unsigned)problems), 64 * WI * WJ, lds, s>>>(p);
+    return hipGetLastError() == hipSuccess ? HS_OK : HS_ERR_LAUNCH;
+}
+
+// ------------------------------------------------------------------------------------------------ gg and gu without G and U
+// gH = gy Wd, G = x Wg^T, U = x Wu^T over the same K = D in one workgroup: 4 D operations an element of H more than reading G and U back, 16 bytes less written
+// and read (fp32: 16-bit G and U would add two roundings to every gradient).  Tile 128 x 64 of each of the three, four waves, two workgroups a CU.
+constexpr int kAgainM = 128, kAgainJ = 64;
+
+template <typename T, typename U>
+__global__ __launch_bounds__(256, 2) void k_gate_bwd(const Args p) {
+    constexpr int BM = kAgainM, TJ = kAgainJ, WAVES = 4, WI = 2, WJ = 2, MT = BM / WI / 16, N2 = TJ / WJ / 16, N1 = 2 * N2;
+    using SA = Side<BM, false, WAVES, MT>;
+    using S1 = Side<2 * TJ, false, WAVES, N1>;
+    using S2 = Side<TJ, true, WAVES, N2>;
+    constexpr uint32_t kBuf = SA::kBytes + S1::kBytes;
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wi = wave / WJ, wj = wave % WJ;
+    const TilePlace t = tile_place(p.tiles_i, p.tiles_j);
+    const int64_t i0 = (int64_t)t.i * BM;
+    const int j0 = t.j * TJ;
+    SA sx, sg;
+    S1 s1;
+    S2 s2;
+    sx.init(wave, lane, p.I - i0, p.lda, false);
+    sg.init(wave, lane, p.I - i0, p.lda2, false);
+    s1.init(wave, lane, (int64_t)p.J - j0, p.ldb, true);
+    s2.init(wave, lane, (int64_t)p.J - j0, p.ldb2, false);
+    sx.init_frags(lane, wi * MT);
+    s1.init_frags(lane, wj * N2);
+    s2.init_frags(lane, wj * N2);
+    const uint32_t lds0 = lds_addr(lds);
+    const int steps_k = (p.K + BK - 1) / BK, steps = steps_k * p.n_seg;
+    int sgm = 0, kk = 0;
+    auto advance = [&]() { if (++kk == steps_k) { kk = 0; sgm++; } };
+    auto request1 = [&](int buf) {
+        const Seg &sg_ = p.seg[0][sgm];
+        const int64_t left = p.K - (int64_t)kk * BK, b = (int64_t)j0 * p.ldb * 2 + kk * (BK * 2);
+        const char *a = (const char *)sg_.a + i0 * p.lda * 2 + kk * (BK * 2);
+        sx.request(wave, a, a, left, lds0 + buf * kBuf);
+        s1.request(wave, (const char *)sg_.b + b, (const char *)sg_.b1 + b, left, lds0 + buf * kBuf + SA::kBytes);
+        advance();
+    };
+    auto request2 = [&](int buf) {
+        const Seg &sg_ = p.seg[1][sgm];
+        const int64_t left = p.K - (int64_t)kk * BK;
+        const char *a = (const char *)sg_.a + i0 * p.lda2 * 2 + kk * (BK * 2), *b = (const char *)sg_.b + (int64_t)j0 * 2 + kk * (BK * p.ldb2 * 2);
+        sg.request(wave, a, a, left, lds0 + buf * kBuf);
+        s2.request(wave, b, b, left, lds0 + buf * kBuf + SA::kBytes);
+        advance();
+    };
+    f32x4 acc[MT][N1], acc2[MT][N2];
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
+#pragma unroll
+        for (int n = 0; n < N1; n++) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int n = 0; n < N2; n++) acc2[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    request1(0);
+    int buf = 0;
+    for (int s = 0; s < steps; s++) {
+        wait_and_meet();
+        const uint32_t at = lds0 + buf * kBuf;
+        multiply_step<T, MT, N1, 1, 1>([&](int m, int ks) { return sx.fragment(at, m, ks); },
+                                       [&](int n, int ks) { return n < N2 ? s1.fragment(at + SA::kBytes, n, ks) : s1.fragment(at + SA::kBytes, n - N2, ks, TJ); },
+                                       [&]() {
+                                           if (s + 1 < steps) request1(buf ^ 1);
+                                           else {
+                                               sgm = kk = 0;
+                                               request2(buf ^ 1);
+                                           }
+                                       },
+                                       acc);
+        buf ^= 1;
+    }
+    for (int s = 0; s < steps; s++) {
+        wait_and_meet();
+        const uint32_t at = lds0 + buf * kBuf;
+        multiply_step<T, MT, N2, 1, 2>([&](int m, int ks) { return sx.fragment(at, m, ks); }, [&](int n, int ks) { return s2.fragment(at + SA::kBytes, n, ks); },
+                                       [&]() { if (s + 1 < steps) request2(buf ^ 1); }, acc2);
+        buf ^= 1;
+    }
+    using St = Staging<3 * TJ, MT, 2, WI, WAVES, TJ>;
+    static_assert(St::kBytes <= 2 * kBuf, "the epilogue's tile must fit");
+    const int li = lane & 15, lq = lane >> 4;
+    float *stage = reinterpret_cast<float *>(lds);
+    with_activation(p.act, [&](auto act) {
+        constexpr int ACT = decltype(act)::value;
+#pragma unroll
+        for (int pass = 0; pass < St::kPasses; pass++) {
+            meet();
+#pragma unroll
+            for (int m = 0; m < St::MP; m++) {
+                float *row = stage + ((wi * St::MP + m) * 16 + li) * St::kPitch + wj * N2 * 16 + lq * 4;
+#pragma unroll
+                for (int n = 0; n < N2; n++) {
+                    *reinterpret_cast<f32x4 *>(row + n * 16) = acc[pass * St::MP + m][n];
+                    *reinterpret_cast<f32x4 *>(row + TJ + n * 16) = acc[pass * St::MP + m][n + N2];
+                    *reinterpret_cast<f32x4 *>(row + 2 * TJ + n * 16) = acc2[pass * St::MP + m][n];
+                }
+            }
+            meet();
+#pragma unroll
+            for (int k = 0; k < St::kIter; k++) {
+                const int64_t i = i0 + St::row(tid, pass, k), at = i * p.ldh + j0 + St::col(tid, k);
+                const float *s = stage + St::line(tid, k) * St::kPitch + St::col(tid, k);
+                const F8 g = load8(s), u = load8(s + TJ), gh = load8(s + 2 * TJ);
+                F8 gg, gu;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    float d;
+                    gu.v[e] = gh.v[e] * activation<ACT, true>(g.v[e], d);
+                    gg.v[e] = gh.v[e] * u.v[e] * d;
+                }
+                if (i < p.I && j0 + St::col(tid, k) < p.ldh) {
+                    store_operand8<U>(p.gg, p.plane, at, gg.v);
+                    store_operand8<U>(p.gu, p.plane, at, gu.v);
+                }
+            }
+        }
+    });
+}
+
+template <typename T, typename U> inline int launch_gate_bwd(Args &p, hipStream_t s) {
+    const int64_t ti = (p.I + kAgainM - 1) / kAgainM, tj = (p.ldh + kAgainJ - 1) / kAgainJ;
+    if (ti * tj > 0x7fffffff / 8) return HS_ERR_ARG;
+    p.tiles_i = (int)ti;
+    p.tiles_j = (int)tj;
+    constexpr int lds = 2 * (kAgainM + 2 * kAgainJ) * BK * 2;
+    static hsLdsAttrOnce attr;
+    attr.set((const void *)k_gate_bwd<T, U>, lds);
+    k_gate_bwd<T, U><<<dim3((unsigned)(ti * tj)), 256, lds, s>>>(p);
     return hipGetLastError() == hipSuccess ? HS_OK : HS_ERR_LAUNCH;
 }
 
