@@ -6,6 +6,7 @@
 // moves fewer bytes than it costs products.
 #pragma once
 #include "rows_gemm.h"
+#include "rows_small.h"
 
 namespace hs_gemm {
 
@@ -78,12 +79,35 @@ __global__ __launch_bounds__(256) void k_rows_reduce(const float *__restrict__ p
 }
 
 // ------------------------------------------------------------------------------------------------ products
-// Tile by the number of workgroups: 256 CUs want at least one each; the larger tile reads less per product.
-template <typename T, typename U, bool AKS, bool BKS, int EPI> int launch_product(Args &p, int problems, hipStream_t s) {
-    const int64_t cols = EPI == EPI_GATE ? 2 * p.ldh : EPI == EPI_GATE_BWD ? p.ldh : p.J;
-    auto tiles = [&](int64_t b) { return (p.I + b - 1) / b * ((cols + b - 1) / b) * problems * p.slices; };
-    if (tiles(256) >= 192) return launch_tile<T, U, 256, 256, 2, 4, AKS, BKS, EPI>(p, problems, s);
-    if (tiles(128) >= 192) return launch_tile<T, U, 128, 128, 2, 2, AKS, BKS, EPI>(p, problems, s);
+// Which tile, and into how many slices K is cut, by what a step of 64 of K costs (microseconds, measured at 8 192 x 4 096 x 12 288 and 1 021 x 1 000 x 2 730):
+// a lone workgroup on a CU waits for its requests (`first`), every further one of the `fit` that LDS admits adds its own work (`more`).  The 256 x 256
+// tile reads the least per product and has the highest rate (1.1 PFLOP/s against 0.93 and 0.6); with few tiles of the result the smaller ones, or
+// slices whose fp32 partial results are added up by another launch, fill the device.  E.g. 1 021 x 1 000 over K = 5 460: 52 us in 64 x 64 tiles,
+// 72 in 128 x 128, 31 in 128 x 128 and four slices.
+struct Plan { int tile, slices; };
+struct TileCost { int size, fit; float first, more; };
+inline Plan plan_product(int64_t I, int64_t cols, int64_t steps, int problems, bool sliceable, int64_t out_bytes) {
+    static const TileCost kinds[3] = {{256, 1, 1.9f, 0.f}, {128, 2, 0.75f, 0.41f}, {64, 5, 0.5f, 0.15f}};
+    Plan best = {256, 1};
+    float least = 0.f;
+    for (const TileCost &t : kinds)
+        for (int slices = 1; slices <= (sliceable ? 64 : 1); slices *= 2) {
+            if (slices > 1 && steps / slices < 4) break;
+            const int64_t groups = ((I + t.size - 1) / t.size) * ((cols + t.size - 1) / t.size) * problems * slices;
+            const int64_t each = (groups + 255) / 256, together = each < t.fit ? each : t.fit, rounds = (groups + 256 * together - 1) / (256 * together);
+            float us = (float)rounds * ((float)((steps + slices - 1) / slices) * (t.first + t.more * (float)(together - 1)) + 3.f);
+            if (slices > 1) us += 4.f + (float)out_bytes * (float)(2 * slices) * 2.5e-7f;        // partial results written and read at 4 TB/s, one launch more
+            if (least == 0.f || us < least) {
+                least = us;
+                best = Plan{t.size, slices};
+            }
+        }
+    return best;
+}
+
+template <typename T, typename U, bool AKS, bool BKS, int EPI> int launch_product(Args &p, int tile, int problems, hipStream_t s) {
+    if (tile == 256) return launch_tile<T, U, 256, 256, 2, 4, AKS, BKS, EPI>(p, problems, s);
+    if (tile == 128) return launch_tile<T, U, 128, 128, 2, 2, AKS, BKS, EPI>(p, problems, s);
     return launch_tile<T, U, 64, 64, 2, 2, AKS, BKS, EPI>(p, problems, s);
 }
 
@@ -104,6 +128,10 @@ template <typename U> constexpr int planes() { return sizeof(U) == 4 ? 3 : 1; }
 // Up to this D the backward pass computes G and U again: 4 D operations an element against 16 bytes.  (At D = 256, 131 072 x 1 024: forward and this part of the
 // backward 660 us against 780 with G and U kept.)
 constexpr int64_t kAgainDim = 768;
+
+// Up to this many rows the forward products read the weights in place (rows_small.h).  4 096 x 12 288 bf16: 105 us at 33 rows, 145 at 64, where the tiles take
+// 104 at 65; fp32, whose tiles need copies in planes: 392 at 64 against 738 at 65.
+template <typename U> constexpr int64_t small_rows() { return sizeof(U) == 4 ? 64 : 32; }
 
 template <typename T, typename U> struct Block {
     const hsGatedMlp &a;
@@ -162,7 +190,25 @@ template <typename T, typename U> struct Block {
         return rc == HS_OK;
     }
 
+    void fwd_small() {
+        Saved sv = saved_in((char *)a.saved);
+        if (!a.saved) {
+            sv.g = sv.u = nullptr;
+            sv.h = Operand{ws.take(M * ldh * 2 * planes<U>()), ldh, M * ldh};
+        }
+        if (!run || rc != HS_OK) return;
+        SmallArgs p = {};
+        p.x = a.x; p.w = a.w_gate; p.w1 = a.w_up; p.ldx = a.ldx; p.ldw = a.ld_gate; p.ldw1 = a.ld_up; p.M = (int)M; p.N = (int)F; p.K = (int)D; p.act = a.activation;
+        p.g = sv.g; p.u = sv.u; p.h = (void *)sv.h.p; p.ldh = ldh; p.plane = sv.h.plane;
+        check(launch_small<T, U, EPI_GATE>(p, s));
+        SmallArgs q = {};
+        q.x = sv.h.p; q.w = q.w1 = a.w_down; q.ldx = ldh; q.ldw = q.ldw1 = a.ld_down; q.M = (int)M; q.N = (int)D; q.K = (int)F; q.plane = sv.h.plane;
+        q.y = a.y; q.ldy = D;
+        if (rc == HS_OK) check(launch_small<T, U, EPI_STORE>(q, s));
+    }
+
     void fwd() {
+        if (M <= small_rows<U>()) return fwd_small();
         const Operand x = operand(a.x, a.ldx, M, D);
         Operand wg, wu;
         projections(wg, wu);
@@ -172,40 +218,47 @@ template <typename T, typename U> struct Block {
             sv.g = sv.u = nullptr;
             sv.h = Operand{ws.take(M * ldh * 2 * planes<U>()), ldh, M * ldh};
         }
-        if (!run || !fits<false, false>(x, wg) || !fits<false, false>(wd, sv.h)) return;
+        if (!fits<false, false>(x, wg) || !fits<false, false>(wd, sv.h)) return;
         Args p = {};
         p.n_seg = add_segments<U>(p.seg[0], 0, x, wg, &wu);
         p.lda = x.ld; p.ldb = wg.ld; p.I = M; p.J = (int)F; p.K = (int)D; p.slices = 1;
         p.g = sv.g; p.u = sv.u; p.h = (void *)sv.h.p; p.ldh = ldh; p.plane = sv.h.plane; p.act = a.activation;
-        check(launch_product<T, U, false, false, EPI_GATE>(p, 1, s));
+        if (run && rc == HS_OK) check(launch_product<T, U, false, false, EPI_GATE>(p, plan_product(M, 2 * ldh, (D + BK - 1) / BK * p.n_seg, 1, false, 0).tile, 1, s));
         Args q = {};
         q.n_seg = add_segments<U>(q.seg[0], 0, sv.h, wd);
-        q.lda = ldh; q.ldb = wd.ld; q.I = M; q.J = (int)D; q.K = (int)F; q.slices = 1;
-        q.out[0] = a.y; q.ldo = D;
-        if (rc == HS_OK) check(launch_product<T, U, false, false, EPI_STORE>(q, 1, s));
+        q.lda = ldh; q.ldb = wd.ld; q.I = M; q.J = (int)D; q.K = (int)F;
+        result<false, false>(q, &a.y, 1);
     }
 
-    // C_z [I, J] = A_z^T B over the rows, z < problems: sliced along them when the result alone does not fill the device
-    void weight_gradient(const Operand *av, const Operand &b, void *const *out, int problems, int64_t I, int64_t J) {
-        const int64_t tiles = (I + 127) / 128 * ((J + 127) / 128) * problems, steps = (M + BK - 1) / BK * (sizeof(U) == 4 ? 6 : 1);
-        int64_t slices = 1;
-        while (slices < 64 && tiles * slices < 512 && steps / (slices * 2) >= 8) slices *= 2;
-        const int64_t n = I * J, stride = (n + 3) / 4 * 4;
-        float *parts = slices > 1 ? (float *)ws.take(stride * 4 * slices * problems) : nullptr;
-        if (!run || !fits<true, true>(av[0], b)) return;
-        Args p = {};
-        for (int z = 0; z < problems; z++) p.n_seg = add_segments<U>(p.seg[z], 0, av[z], b);
-        p.lda = av[0].ld; p.ldb = b.ld; p.I = I; p.J = (int)J; p.K = (int)M; p.slices = (int)slices; p.ldo = J; p.slice_stride = stride;
-        for (int z = 0; z < problems; z++) p.out[z] = slices > 1 ? (void *)(parts + z * slices * stride) : out[z];
-        if (slices == 1) {
-            check(launch_product<T, U, true, true, EPI_STORE>(p, problems, s));
+    // The results of up to two products of one shape (p holds everything but the outputs): out[z] [I, J], contiguous.
+    template <bool AKS, bool BKS> void result(Args &p, void *const *out, int problems) {
+        const int64_t n = p.I * p.J, stride = (n + 3) / 4 * 4, steps = (p.K + BK - 1) / BK * (int64_t)p.n_seg;
+        const Plan plan = plan_product(p.I, p.J, steps, problems, true, 4 * n * problems);
+        float *parts = plan.slices > 1 ? (float *)ws.take(stride * 4 * plan.slices * problems) : nullptr;
+        if (!run || rc != HS_OK) return;
+        p.ldo = p.J;
+        p.slices = plan.slices;
+        p.slice_stride = stride;
+        for (int z = 0; z < problems; z++) p.out[z] = parts ? (void *)(parts + z * plan.slices * stride) : out[z];
+        if (!parts) {
+            check(launch_product<T, U, AKS, BKS, EPI_STORE>(p, plan.tile, problems, s));
             return;
         }
-        check(launch_product<T, U, true, true, EPI_PARTIAL>(p, problems, s));
-        if (rc != HS_OK) return;
+        check(launch_product<T, U, AKS, BKS, EPI_PARTIAL>(p, plan.tile, problems, s));
         const int64_t blocks = (n + 1023) / 1024;
-        k_rows_reduce<U><<<dim3((unsigned)blocks, problems), 256, 0, s>>>(parts, parts + (problems - 1) * slices * stride, n, (int)slices, (U *)out[0], (U *)out[problems - 1]);
+        if (rc != HS_OK || blocks > 0x7fffffff) { check(HS_ERR_ARG); return; }
+        k_rows_reduce<U><<<dim3((unsigned)blocks, problems), 256, 0, s>>>(parts, parts + (problems - 1) * plan.slices * stride, n, plan.slices, (U *)out[0],
+                                                                          (U *)out[problems - 1]);
         check(hipGetLastError() == hipSuccess ? HS_OK : HS_ERR_LAUNCH);
+    }
+
+    // C_z [I, J] = A_z^T B over the rows
+    void weight_gradient(const Operand *av, const Operand &b, void *const *out, int problems, int64_t I, int64_t J) {
+        if (!fits<true, true>(av[0], b)) return;
+        Args p = {};
+        for (int z = 0; z < problems; z++) p.n_seg = add_segments<U>(p.seg[z], 0, av[z], b);
+        p.lda = av[0].ld; p.ldb = b.ld; p.I = I; p.J = (int)J; p.K = (int)M;
+        result<true, true>(p, out, problems);
     }
 
     void bwd() {
@@ -218,7 +271,7 @@ template <typename T, typename U> struct Block {
             Operand wg, wu, x;
             if (again() || a.gx) projections(wg, wu);
             if (again() || a.gw_gate || a.gw_up) x = operand(a.x, a.ldx, M, D);
-            if (run && fits<false, true>(gy, wd) && (!again() || fits<false, false>(x, wg))) {
+            if (fits<false, true>(gy, wd) && (!again() || fits<false, false>(x, wg)) && run) {
                 Args p = {};
                 p.I = M; p.J = (int)F; p.K = (int)D; p.slices = 1;
                 p.g = sv.g; p.u = sv.u; p.gg = (void *)gg.p; p.gu = (void *)gu.p; p.ldh = ldh; p.plane = n; p.act = a.activation;
@@ -230,17 +283,16 @@ template <typename T, typename U> struct Block {
                 } else {
                     p.n_seg = add_segments<U>(p.seg[0], 0, gy, wd);
                     p.lda = gy.ld; p.ldb = wd.ld;
-                    check(launch_product<T, U, false, true, EPI_GATE_BWD>(p, 1, s));
+                    check(launch_product<T, U, false, true, EPI_GATE_BWD>(p, plan_product(M, ldh, (D + BK - 1) / BK * p.n_seg, 1, false, 0).tile, 1, s));
                 }
             }
             if (a.gx) {
-                if (run && fits<false, true>(gg, wg)) {
+                if (fits<false, true>(gg, wg)) {
                     Args p = {};
                     p.n_seg = add_segments<U>(p.seg[0], 0, gg, wg);
                     p.n_seg = add_segments<U>(p.seg[0], p.n_seg, gu, wu);
-                    p.lda = ldh; p.ldb = wg.ld; p.I = M; p.J = (int)D; p.K = (int)F; p.slices = 1;
-                    p.out[0] = a.gx; p.ldo = D;
-                    check(launch_product<T, U, false, true, EPI_STORE>(p, 1, s));
+                    p.lda = ldh; p.ldb = wg.ld; p.I = M; p.J = (int)D; p.K = (int)F;
+                    result<false, true>(p, &a.gx, 1);
                 }
             }
             if (a.gw_gate || a.gw_up) {

@@ -152,6 +152,10 @@ def _gate(gate):
 
 _lib = None
 _ROW_BYTES = ("hs_embed_bwd_ws_bytes", "hs_gated_mlp_saved_bytes", "hs_gated_mlp_fwd_ws_bytes", "hs_gated_mlp_bwd_ws_bytes")      # sizes, or a negative error
+_p, _i, _l, _f = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
+# (declared once: a call then takes plain integers -- the smallest calls are bound by the host)
+_ROW_ARGTYPES = {"hs_embed_fwd": (_p, _i, _p, _l, _p, _l, _l, _l, _f, _i, _i, _p), "hs_embed_bwd_ws_bytes": (_l, _l, _l),
+                 "hs_embed_bwd": (_p, _i, _p, _l, _p, _l, _l, _l, _f, _l, _i, _i, _p, _l, _p), "hs_dropout_rows": (_p, _p, _p, _l, _i, _i, _p, _p)}
 ROW_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}        # HS_F32 / HS_BF16 / HS_F16: section 10 (row operators)
 ROW_ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "sigmoid": 3, "relu": 4}       # HS_ACT_*
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}  # HS_F32 / HS_BF16
@@ -169,6 +173,8 @@ def load_library():
         for name in dir_symbols():
             if name != "hs_target_arch":
                 getattr(_lib, name).restype = ctypes.c_int64 if name in _ROW_BYTES else ctypes.c_int
+        for name, types in _ROW_ARGTYPES.items():
+            getattr(_lib, name).argtypes = types
         if _lib.hs_abi_version() != ABI_VERSION:
             raise RuntimeError(f"{LIB_PATH}: ABI version {_lib.hs_abi_version()}, this package needs {ABI_VERSION} -- rebuild "
                                "(python -m holoscene_amd.csrc.build)")
@@ -210,6 +216,11 @@ def _dev_at(t, name, elem_offset, dtype=torch.float32):
 
 def _stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def _row_stream(t):
+    """The current stream of t's device, as an integer (the row operators' calls)."""
+    return torch.cuda.current_stream(t.device).cuda_stream
 
 
 SCHEDULE = int(os.environ.get("HOLOSCENE_HASH_SCHEDULE", "1"))
@@ -1595,50 +1606,44 @@ class _HipBackend:
     # ---- row operators (include/holoscene_hip.h section 10).  Callers (model/row_ops.py) have checked shapes, types and devices and made the
     # tensors' device current; rows may be strided, elements of a row are consecutive.
     @staticmethod
-    def _rows(t):
-        """(pointer, row distance) of a 2-D tensor; a matrix of one row (or none) may carry any stride."""
-        return ctypes.c_void_p(t.data_ptr()), ctypes.c_int64(t.stride(0) if t.shape[0] > 1 else t.shape[1])
+    def _ld(t):
+        """Row distance of a 2-D tensor; a matrix of one row (or none) may carry any stride."""
+        return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
     @classmethod
     def embed_fwd(cls, indices, table, out, scale):
         lib = load_library()
-        tp, ld = cls._rows(table)
-        _check(lib.hs_embed_fwd(ctypes.c_void_p(indices.data_ptr()), indices.element_size(), tp, ld, ctypes.c_void_p(out.data_ptr()), ctypes.c_int64(indices.numel()),
-                                ctypes.c_int64(table.shape[0]), ctypes.c_int64(table.shape[1]), ctypes.c_float(scale), ROW_DTYPES[table.dtype], ROW_DTYPES[out.dtype],
-                                _stream()), "hs_embed_fwd")
+        V, D = table.shape
+        _check(lib.hs_embed_fwd(indices.data_ptr(), indices.element_size(), table.data_ptr(), cls._ld(table), out.data_ptr(), indices.numel(), V, D, scale,
+                                ROW_DTYPES[table.dtype], ROW_DTYPES[out.dtype], _row_stream(out)), "hs_embed_fwd")
 
     @classmethod
     def embed_bwd(cls, indices, grad, grad_table, scale, padding):
         lib = load_library()
-        n, V, D = ctypes.c_int64(indices.numel()), ctypes.c_int64(grad_table.shape[0]), ctypes.c_int64(grad_table.shape[1])
+        n, (V, D) = indices.numel(), grad_table.shape
         nbytes = lib.hs_embed_bwd_ws_bytes(n, V, D)
         _check(min(nbytes, 0), "hs_embed_bwd")
         ws = torch.empty(nbytes, device=grad.device, dtype=torch.uint8)
-        gp, ldg = cls._rows(grad)
-        _check(lib.hs_embed_bwd(ctypes.c_void_p(indices.data_ptr()), indices.element_size(), gp, ldg, ctypes.c_void_p(grad_table.data_ptr()), n, V, D, ctypes.c_float(scale),
-                                ctypes.c_int64(padding), ROW_DTYPES[grad.dtype], ROW_DTYPES[grad_table.dtype], ctypes.c_void_p(ws.data_ptr()), ctypes.c_int64(nbytes), _stream()), "hs_embed_bwd")
+        _check(lib.hs_embed_bwd(indices.data_ptr(), indices.element_size(), grad.data_ptr(), cls._ld(grad), grad_table.data_ptr(), n, V, D, scale, padding,
+                                ROW_DTYPES[grad.dtype], ROW_DTYPES[grad_table.dtype], ws.data_ptr(), nbytes, _row_stream(grad)), "hs_embed_bwd")
 
     @staticmethod
     def dropout_rows(x, residual, y, drop, rng):
-        lib = load_library()
-        _check(lib.hs_dropout_rows(ctypes.c_void_p(x.data_ptr()), None if residual is None else ctypes.c_void_p(residual.data_ptr()), ctypes.c_void_p(y.data_ptr()),
-                                   ctypes.c_int64(x.numel()), ROW_DTYPES[x.dtype], int(drop), ctypes.c_void_p(rng.data_ptr()), _stream()), "hs_dropout_rows")
+        _check(load_library().hs_dropout_rows(x.data_ptr(), None if residual is None else residual.data_ptr(), y.data_ptr(), x.numel(), ROW_DTYPES[x.dtype], drop,
+                                              rng.data_ptr(), _row_stream(x)), "hs_dropout_rows")
 
     @classmethod
     def _gated_args(cls, x, w_gate, w_up, w_down, activation):
-        a = hsGatedMlp(rows=x.shape[0], dim=x.shape[1], hidden=w_gate.shape[0], dtype=ROW_DTYPES[x.dtype], activation=ROW_ACTIVATIONS[activation])
-        for name, ld, t in (("x", "ldx", x), ("w_gate", "ld_gate", w_gate), ("w_up", "ld_up", w_up), ("w_down", "ld_down", w_down)):
-            p, d = cls._rows(t)
-            setattr(a, name, p)
-            setattr(a, ld, d.value)
-        return a
+        return hsGatedMlp(x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), cls._ld(x), cls._ld(w_gate), cls._ld(w_up), cls._ld(w_down), x.shape[0],
+                          x.shape[1], w_gate.shape[0], ROW_DTYPES[x.dtype], ROW_ACTIVATIONS[activation])
 
     @staticmethod
-    def _gated_call(a, fn, nbytes, device):
+    def _gated_call(a, fn, nbytes, x):
         _check(min(nbytes, 0), fn)
-        ws = torch.empty(nbytes, device=device, dtype=torch.uint8)
-        a.ws, a.ws_bytes = ws.data_ptr(), nbytes
-        _check(getattr(load_library(), fn)(ctypes.byref(a), _stream()), fn)
+        if nbytes:
+            ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
+            a.ws, a.ws_bytes = ws.data_ptr(), nbytes
+        _check(getattr(load_library(), fn)(ctypes.byref(a), ctypes.c_void_p(_row_stream(x))), fn)
 
     @classmethod
     def gated_mlp_fwd(cls, x, w_gate, w_up, w_down, activation, y, save):
@@ -1652,7 +1657,7 @@ class _HipBackend:
             saved = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
             a.saved = saved.data_ptr()
         a.y = y.data_ptr()
-        cls._gated_call(a, "hs_gated_mlp_fwd", lib.hs_gated_mlp_fwd_ws_bytes(ctypes.byref(a)), x.device)
+        cls._gated_call(a, "hs_gated_mlp_fwd", lib.hs_gated_mlp_fwd_ws_bytes(ctypes.byref(a)), x)
         return saved
 
     @classmethod
@@ -1660,11 +1665,9 @@ class _HipBackend:
         """gx, gw_*: written, None = not wanted."""
         lib = load_library()
         a = cls._gated_args(x, w_gate, w_up, w_down, activation)
-        p, d = cls._rows(grad)
-        a.grad, a.ld_grad, a.saved = p, d.value, saved.data_ptr()
-        for name, t in (("gx", gx), ("gw_gate", gw_gate), ("gw_up", gw_up), ("gw_down", gw_down)):
-            setattr(a, name, None if t is None else t.data_ptr())
-        cls._gated_call(a, "hs_gated_mlp_bwd", lib.hs_gated_mlp_bwd_ws_bytes(ctypes.byref(a)), x.device)
+        a.grad, a.ld_grad, a.saved = grad.data_ptr(), cls._ld(grad), saved.data_ptr()
+        a.gx, a.gw_gate, a.gw_up, a.gw_down = (None if t is None else t.data_ptr() for t in (gx, gw_gate, gw_up, gw_down))
+        cls._gated_call(a, "hs_gated_mlp_bwd", lib.hs_gated_mlp_bwd_ws_bytes(ctypes.byref(a)), x)
 
 
 class hsAdamState(ctypes.Structure):

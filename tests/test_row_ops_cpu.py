@@ -80,10 +80,13 @@ def test_gated_mlp_refusals():
 
 def test_gated_mlp_work_space_counts_the_copies():
     ws = lib().hs_gated_mlp_fwd_ws_bytes
-    assert ws(gated()) == 0                                                  # aligned 16-bit operands are read where they are
-    assert ws(gated(x=258)) >= 4 * 16 * 2                                    # ... others are copied
-    assert ws(gated(dtype=0)) >= 3 * 2 * (4 * 16 + 3 * 16 * 32)              # fp32: three planes of every operand
-    assert lib().hs_gated_mlp_saved_bytes(gated()) >= 3 * 4 * 32 * 2
+    assert ws(gated()) == 0 and ws(gated(x=258)) == 0                        # few rows: everything is read where it is
+    plain = ws(gated(rows=100))
+    assert ws(gated(rows=100, x=258)) - plain >= 100 * 16 * 2                # more: an operand that is not aligned is copied
+    assert ws(gated(rows=100, w_down=264)) - plain >= 16 * 32 * 2
+    assert ws(gated(rows=100, dtype=0)) >= 3 * 2 * (100 * 16 + 3 * 16 * 32)  # fp32: three planes of every operand
+    assert lib().hs_gated_mlp_saved_bytes(gated()) >= 4 * 32 * 2             # the gated product; with wide rows both projections in fp32 too
+    assert lib().hs_gated_mlp_saved_bytes(gated(dim=2048, ldx=2048, ld_gate=2048, ld_up=2048)) >= 4 * 32 * (2 + 8)
     assert lib().hs_gated_mlp_bwd_ws_bytes(gated(gx=256)) >= 2 * 4 * 32 * 2
 
 
