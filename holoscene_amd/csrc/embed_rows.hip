@@ -5,12 +5,13 @@
 //
 // The gradient sums each row's run in the order of the positions, so it is the same from run to run: (index, position) pairs are sorted by
 // index with a stable counting sort, and the table's gradient is then written row by row, once, zeros included -- no fill, no atomics on it.
-//   sort    N <= 16 384: one workgroup, the pairs in registers, one pass per <= 8 bits of the index through LDS (one launch);
-//           longer: passes of <= 11 bits, two launches each (block histograms; ranks, every workgroup adding up the histograms itself).
-//   chunks  sorted positions in chunks of 64: a chunk that lies inside one run is summed to fp32 partials (a run of one index may be the whole batch).
-//   rows    bounds of a row's run by bisection in the sorted indices; head and tail of the run from g, its whole chunks from the partials.
+//   sort    N <= 4 096: one workgroup, the pairs in registers, one pass per <= 8 bits of the index through LDS (one launch);
+//           longer: passes of <= 9 bits, two launches each (block histograms; ranks, every workgroup adding up the histograms itself).
+//   chunks  sorted positions in chunks of 32: a chunk that lies inside one run is summed to fp32 partials (a run of one index may be the whole batch).
+//   bounds  of every row's run, by bisection in the sorted indices, in the same launch.
+//   rows    head and tail of the run from g, its whole chunks from the partials.
 //           Short runs: a wave per row.  Long ones: all four waves of the workgroup on one row, joined through LDS in a fixed order.
-// fp32 sums: 64 terms per chunk, then the partials; the last operation rounds to the table's type.
+// fp32 sums: 32 terms per chunk, then the partials; the last operation rounds to the table's type.
 #include "holoscene_hip.h"
 #include "launch_util.h"
 #include "row_types.h"
@@ -56,19 +57,24 @@ template <typename I> __device__ __forceinline__ uint32_t sort_key(const I *__re
 }
 
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
-constexpr int kTile = 4096;                         // pairs per tile of the multi-block sort: 4 per thread
-constexpr int kOneMax = 16384, kOneDigit = 8;       // the one-workgroup sort
-constexpr int kMultiDigit = 11;
+constexpr int kOneMax = 4096, kOneDigit = 8;        // the one-workgroup sort (16 384 pairs in it: 37 us, bound by one CU's vector instructions; over 16 CUs 24)
+constexpr int kMultiDigit = 9;                     // the multi-block sort: tiles of 1, 2 or 4 pairs per thread
 constexpr int kMaxBlocks = 64;                      // workgroups of the multi-block sort (each adds up all their histograms)
 
-// Lanes of this wave whose digit equals mine, among those with `on`.
+// Lanes of this wave whose digit equals mine, among those with `on`.  (Per bit: a mask of the bit, a ballot, and the lanes that agree with it.)
 __device__ __forceinline__ uint64_t same_digit(uint32_t digit, int bits, bool on) {
-    uint64_t m = __ballot(on);
-    for (int b = 0; b < bits; b++) {
-        const uint64_t set = __ballot((digit >> b) & 1u);
-        m &= ((digit >> b) & 1u) ? set : ~set;
+    const uint64_t all = __ballot(on);
+    uint32_t lo = (uint32_t)all, hi = (uint32_t)(all >> 32);
+#pragma unroll
+    for (int b = 0; b < kMultiDigit; b++) {
+        if (b < bits) {         // (uniform)
+            const uint32_t mine = (uint32_t)((int32_t)(digit << (31 - b)) >> 31);
+            const uint64_t set = __ballot(mine != 0u);
+            lo &= ~((uint32_t)set ^ mine);
+            hi &= ~((uint32_t)(set >> 32) ^ mine);
+        }
     }
-    return m;
+    return ((uint64_t)hi << 32) | lo;
 }
 
 // Ranks of a tile's pairs among those of equal digit in front of them.  Wave w holds pairs [w * 64 * R, (w + 1) * 64 * R) of the tile, round r lane l
@@ -156,20 +162,24 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_one(const I *__restrict__
         tile_ranks<R>(digit, on, rank, nb, bins, cnt, total);
         __syncthreads();
         scan_exclusive(total, bins, wave_sums);
-        const bool last = p + 1 == passes;
 #pragma unroll
         for (int r = 0; r < R; r++) {
             if (!on[r]) continue;
             const uint32_t to = total[digit[r]] + rank[r];
-            (last ? keys : lk)[to] = key[r];
-            (last ? pos : lp)[to] = at[r];
+            lk[to] = key[r];
+            lp[to] = at[r];
         }
         __syncthreads();
-        if (!last) {
+        if (p + 1 < passes) {
 #pragma unroll
             for (int r = 0; r < R; r++) {
                 const int i = (wave * R + r) * 64 + lane;
                 if (on[r]) { key[r] = lk[i]; at[r] = lp[i]; }
+            }
+        } else {
+            for (int i = tid; i < n; i += kSortThreads) {       // (from LDS: written where the ranks point, every store instruction would touch 64 lines)
+                keys[i] = lk[i];
+                pos[i] = lp[i];
             }
         }
         shift += nb;
@@ -194,33 +204,36 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_hist(const I *__restrict_
 }
 
 // second launch: ranks.  A workgroup's first place for a digit = all pairs of smaller digits + the pairs of this digit in earlier workgroups.
-template <typename I>
+template <typename I, int R>
 __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(const I *__restrict__ idx, const uint32_t *__restrict__ keys_in, const uint32_t *__restrict__ pos_in, int64_t n,
                                                                int64_t per, int64_t V, int64_t padding, int shift, int nb, const uint32_t *__restrict__ hist,
                                                                uint32_t *__restrict__ keys, uint32_t *__restrict__ pos) {
-    constexpr int R = kTile / kSortThreads;
+    constexpr int kTile = R * kSortThreads;
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
     const int bins = 1 << nb, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    uint32_t *place = lds, *tile_total = lds + bins, *wave_sums = lds + 2 * bins;
-    uint16_t *cnt = reinterpret_cast<uint16_t *>(wave_sums + kSortWaves);
-    uint32_t before[2] = {0, 0};
-#pragma unroll
-    for (int q = 0; q < 2; q++) {
-        const int d = 2 * tid + q;          // (the layout scan_exclusive works on: the pair 2 tid, 2 tid + 1 stays with the thread)
-        if (d >= bins) continue;
-        uint32_t all = 0;
-        for (int b = 0; b < (int)gridDim.x; b++) {
-            const uint32_t c = hist[(size_t)b * bins + d];
-            if (b < (int)blockIdx.x) before[q] += c;
-            all += c;
+    uint32_t *place = lds, *tile_total = lds + bins, *tile_first = lds + 2 * bins, *wave_sums = lds + 3 * bins, *lk = wave_sums + kSortWaves, *lp = lk + kTile;
+    uint16_t *cnt = reinterpret_cast<uint16_t *>(lp + kTile);
+    // all pairs of a digit, and those in earlier workgroups: 2048 / bins threads a pair of digits, each a share of the workgroups' histograms
+    uint32_t *before = tile_first;
+    for (int d = tid; d < bins; d += kSortThreads) place[d] = before[d] = 0;
+    __syncthreads();
+    {
+        const int half = bins / 2, d = tid % half, share = kSortThreads / half;
+#pragma unroll 4
+        for (int b = tid / half; b < (int)gridDim.x; b += share) {
+            const uint2 c = reinterpret_cast<const uint2 *>(hist + (size_t)b * bins)[d];
+            atomicAdd(&place[2 * d], c.x);              // (counts in LDS: their order does not matter)
+            atomicAdd(&place[2 * d + 1], c.y);
+            if (b < (int)blockIdx.x) {
+                atomicAdd(&before[2 * d], c.x);
+                atomicAdd(&before[2 * d + 1], c.y);
+            }
         }
-        place[d] = all;
     }
     __syncthreads();
     scan_exclusive(place, bins, wave_sums);
-#pragma unroll
-    for (int q = 0; q < 2; q++)
-        if (2 * tid + q < bins) place[2 * tid + q] += before[q];
+    for (int d = tid; d < bins; d += kSortThreads) place[d] += before[d];
+    __syncthreads();
     const int64_t begin = blockIdx.x * per, end = begin + per < n ? begin + per : n;
     for (int64_t t0 = begin; t0 < end; t0 += kTile) {
         for (int i = tid; i < kSortWaves * bins; i += kSortThreads) cnt[i] = 0;
@@ -236,12 +249,23 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(const I *__restri
         }
         __syncthreads();
         tile_ranks<R>(digit, on, rank, nb, bins, cnt, tile_total);
+        // the tile in its own order through LDS, then out: neighbours go to neighbouring places
+        for (int d = tid; d < bins; d += kSortThreads) tile_first[d] = tile_total[d];
+        __syncthreads();
+        scan_exclusive(tile_first, bins, wave_sums);
 #pragma unroll
         for (int r = 0; r < R; r++) {
             if (!on[r]) continue;
-            const uint32_t to = place[digit[r]] + rank[r];
-            keys[to] = key[r];
-            pos[to] = at[r];
+            const uint32_t to = tile_first[digit[r]] + rank[r];
+            lk[to] = key[r];
+            lp[to] = at[r];
+        }
+        __syncthreads();
+        const int in_tile = end - t0 < kTile ? (int)(end - t0) : kTile;
+        for (int i = tid; i < in_tile; i += kSortThreads) {
+            const uint32_t k = lk[i], d = (k >> shift) & (uint32_t)(bins - 1), to = place[d] + (uint32_t)i - tile_first[d];
+            keys[to] = k;
+            pos[to] = lp[i];
         }
         __syncthreads();
         for (int d = tid; d < bins; d += kSortThreads) place[d] += tile_total[d];
@@ -250,51 +274,28 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(const I *__restri
 }
 
 // ------------------------------------------------------------------------------------------------ sums
-constexpr int kChunk = 64;
+constexpr int kChunk = 32;
 
-// VEC elements of a row at any alignment of the row, zeros behind column `cols`
-template <typename T, int VEC> __device__ __forceinline__ void add_row(const T *__restrict__ p, int cols, float (&acc)[VEC]) {
+// acc += the entries first, first + step, .. < end, in that order.  row(j): where entry j's element `col` lies.  BATCH entries are requested together, the missing
+// ones of the last batch at the first entry's address and not added (a branch between the requests would wait for each of them).
+template <int BATCH, typename T, int VEC, typename R>
+__device__ __forceinline__ void add_entries(int64_t first, int64_t end, int step, int cols, R row, float (&acc)[VEC]) {
     if (cols >= VEC) {
-        const Loose<T, VEC> t = *reinterpret_cast<const Loose<T, VEC> *>(p);
+        for (int64_t j = first; j < end; j += BATCH * step) {
+            Loose<T, VEC> t[BATCH];
 #pragma unroll
-        for (int e = 0; e < VEC; e++) acc[e] += to_f32(t.v[e]);
-    } else {
+            for (int b = 0; b < BATCH; b++) t[b] = *reinterpret_cast<const Loose<T, VEC> *>(row(j + b * step < end ? j + b * step : first));
 #pragma unroll
-        for (int e = 0; e < VEC; e++)
-            if (e < cols) acc[e] += to_f32(p[e]);
+            for (int b = 0; b < BATCH; b++)
+#pragma unroll
+                for (int e = 0; e < VEC; e++) acc[e] += j + b * step < end ? to_f32(t[b].v[e]) : 0.f;
+        }
+    } else {                    // a row's last columns
+        for (int64_t j = first; j < end; j += step)
+#pragma unroll
+            for (int e = 0; e < VEC; e++)
+                if (e < cols) acc[e] += to_f32(row(j)[e]);
     }
-}
-
-// Column layout of the two kernels below: a workgroup covers `lanes` * VEC columns (blockIdx.y the column block), lanes = a power of two <= 64; the
-// 256 / lanes groups of lanes are slots that take entries in turn.
-
-// partial[c][D] of the chunks that lie inside one run
-template <typename T, int VEC>
-__global__ __launch_bounds__(256) void k_embed_chunks(const uint32_t *__restrict__ keys, const uint32_t *__restrict__ pos, const T *__restrict__ grad, int64_t ldg,
-                                                      int64_t n, uint32_t V, int D, int lanes, float *__restrict__ partial) {
-    __shared__ float join[256 * VEC];
-    const int64_t c0 = (int64_t)blockIdx.x * kChunk;
-    const uint32_t first = keys[c0];
-    if (c0 + kChunk > n || first == V || first != keys[c0 + kChunk - 1]) return;        // (uniform in the workgroup)
-    const int tid = threadIdx.x, col = ((int)blockIdx.y * lanes + (tid & (lanes - 1))) * VEC, slot = tid / lanes, slots = 256 / lanes;
-    float acc[VEC];
-#pragma unroll
-    for (int e = 0; e < VEC; e++) acc[e] = 0.f;
-    if (col < D) {
-#pragma unroll 4
-        for (int j = slot; j < kChunk; j += slots) add_row<T, VEC>(grad + (int64_t)pos[c0 + j] * ldg + col, D - col, acc);
-    }
-#pragma unroll
-    for (int e = 0; e < VEC; e++) join[e * 256 + tid] = acc[e];
-    __syncthreads();
-    if (slot != 0 || col >= D) return;
-    for (int s = 1; s < slots; s++)
-#pragma unroll
-        for (int e = 0; e < VEC; e++) acc[e] += join[e * 256 + s * lanes + tid];
-    float *out = partial + (int64_t)blockIdx.x * D + col;
-#pragma unroll
-    for (int e = 0; e < VEC; e++)
-        if (col + e < D) out[e] = acc[e];
 }
 
 // first place in keys[0, n) that is >= v
@@ -307,20 +308,61 @@ __device__ __forceinline__ int64_t lower_bound(const uint32_t *__restrict__ keys
     return lo;
 }
 
-constexpr int kRowsPerGroup = 16, kShort = 8;       // rows per workgroup; runs up to kShort entries are summed by one slot
+// Column layout of the two kernels below: a group of `lanes` (a power of two <= 64) covers lanes * VEC columns at a time; the 256 / lanes groups of a
+// workgroup are slots that take entries (short runs: rows) in turn.  k_embed_chunks: blockIdx.y is the column block.
 
-template <typename T, typename O, int VEC>
-__global__ __launch_bounds__(256) void k_embed_rows(const uint32_t *__restrict__ keys, const uint32_t *__restrict__ pos, const T *__restrict__ grad, int64_t ldg, int64_t n,
-                                                    int64_t V, int D, int lanes, const float *__restrict__ partial, float scale, O *__restrict__ gtable) {
-    __shared__ int64_t bound[kRowsPerGroup + 1];
+// Two jobs that only need the sorted pairs, in one launch: the first bound_blocks workgroups find the first entry of every row's run (a thread per row and a
+// chain of ~log2 n dependent loads: as part of the rows' kernel it was most of its time), the others sum the chunks that lie inside one run.
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void k_embed_chunks(const uint32_t *__restrict__ keys, const uint32_t *__restrict__ pos, const T *__restrict__ grad, int64_t ldg,
+                                                      int64_t n, uint32_t V, int D, int lanes, float *__restrict__ partial, uint2 *__restrict__ bounds, unsigned bound_blocks) {
     __shared__ float join[256 * VEC];
-    const int tid = threadIdx.x, lane = tid & (lanes - 1), slot = tid / lanes, slots = 256 / lanes, col = ((int)blockIdx.y * lanes + lane) * VEC;
-    const int64_t v0 = (int64_t)blockIdx.x * kRowsPerGroup;
-    const int rows = V - v0 < kRowsPerGroup ? (int)(V - v0) : kRowsPerGroup;
-    if (tid <= rows) bound[tid] = lower_bound(keys, n, (uint32_t)(v0 + tid));
+    const int tid = threadIdx.x;
+    if (blockIdx.x < bound_blocks) {
+        const int64_t v = (int64_t)blockIdx.x * 256 + tid;
+        if (blockIdx.y == 0 && v <= V) {
+            const int64_t at = lower_bound(keys, n, (uint32_t)v);
+            bounds[v] = make_uint2((uint32_t)at, at < n ? pos[at] : 0u);        // .y: the first entry's position, a load less in the rows' chain
+        }
+        return;
+    }
+    const int64_t c = blockIdx.x - bound_blocks, c0 = c * kChunk;
+    const uint32_t first = keys[c0];
+    if (first == V || first != keys[c0 + kChunk - 1]) return;        // (uniform in the workgroup)
+    const int col = ((int)blockIdx.y * lanes + (tid & (lanes - 1))) * VEC, slot = tid / lanes, slots = 256 / lanes;
+    float acc[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; e++) acc[e] = 0.f;
+    if (col < D) add_entries<8, T, VEC>(c0 + slot, c0 + kChunk, slots, D - col, [&](int64_t j) { return grad + (int64_t)pos[j] * ldg + col; }, acc);
+#pragma unroll
+    for (int e = 0; e < VEC; e++) join[e * 256 + tid] = acc[e];
     __syncthreads();
-    auto write = [&](int r, const float (&acc)[VEC]) {
-        O *out = gtable + (v0 + r) * D + col;
+    if (slot != 0 || col >= D) return;
+    for (int s = 1; s < slots; s++)
+#pragma unroll
+        for (int e = 0; e < VEC; e++) acc[e] += join[e * 256 + s * lanes + tid];
+    float *out = partial + c * D + col;
+#pragma unroll
+    for (int e = 0; e < VEC; e++)
+        if (col + e < D) out[e] = acc[e];
+}
+
+constexpr int kShort = 8, kWide = 4;        // runs up to kShort entries are summed by one slot, kWide * VEC columns a lane at a time
+
+// A slot per row: the chain bounds -> position -> gradient is paid once per row, not once per row and 1 KB of it, and with short runs there are
+// few bytes to wait for otherwise.
+template <typename T, typename O, int VEC>
+__global__ __launch_bounds__(256) void k_embed_rows(const uint2 *__restrict__ bounds, const uint32_t *__restrict__ pos, const T *__restrict__ grad, int64_t ldg, int64_t V, int D,
+                                                    int lanes, const float *__restrict__ partial, float scale, O *__restrict__ gtable) {
+    __shared__ int64_t run[256][2];
+    __shared__ float join[256 * VEC];
+    const int tid = threadIdx.x, lane = tid & (lanes - 1), slot = tid / lanes, slots = 256 / lanes;
+    const int64_t v0 = (int64_t)blockIdx.x * slots, v = v0 + slot;
+    const uint2 own = v < V ? bounds[v] : make_uint2(0, 0);
+    const int64_t s = own.x, e_ = v < V ? bounds[v + 1].x : 0;
+    const bool is_long = e_ - s > kShort;
+    auto write = [&](int64_t row, int col, const float *acc) {
+        O *out = gtable + row * D + col;
         Loose<O, VEC> o;
 #pragma unroll
         for (int e = 0; e < VEC; e++) o.v[e] = from_f32<O>(acc[e] * scale);
@@ -330,49 +372,74 @@ __global__ __launch_bounds__(256) void k_embed_rows(const uint32_t *__restrict__
             for (int e = 0; e < VEC; e++)
                 if (col + e < D) out[e] = o.v[e];
     };
-    for (int r = slot; r < rows; r += slots) {              // short runs: a slot each
-        const int64_t s = bound[r], e_ = bound[r + 1];
-        if (e_ - s > kShort || col >= D) continue;
-        float acc[VEC];
+    if (v < V && !is_long) {
+        for (int c0 = lane * VEC; c0 < D; c0 += kWide * lanes * VEC) {
+            float acc[kWide][VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; e++) acc[e] = 0.f;
-        for (int64_t j = s; j < e_; j++) add_row<T, VEC>(grad + (int64_t)pos[j] * ldg + col, D - col, acc);
-        write(r, acc);
+            for (int k = 0; k < kWide; k++)
+#pragma unroll
+                for (int e = 0; e < VEC; e++) acc[k][e] = 0.f;
+            for (int64_t j = s; j < e_; j++) {
+                const T *row = grad + (int64_t)(j == s ? own.y : pos[j]) * ldg;
+#pragma unroll
+                for (int k = 0; k < kWide; k++) {
+                    const int col = c0 + k * lanes * VEC;
+                    if (col + VEC <= D) {
+                        const Loose<T, VEC> t = *reinterpret_cast<const Loose<T, VEC> *>(row + col);
+#pragma unroll
+                        for (int e = 0; e < VEC; e++) acc[k][e] += to_f32(t.v[e]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < VEC; e++)
+                            if (col + e < D) acc[k][e] += to_f32(row[col + e]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < kWide; k++)
+                if (c0 + k * lanes * VEC < D) write(v, c0 + k * lanes * VEC, acc[k]);
+        }
     }
-    for (int r = 0; r < rows; r++) {                        // long runs: all slots, joined in the order of the slots
-        const int64_t s = bound[r], e_ = bound[r + 1];
-        if (e_ - s <= kShort) continue;                     // (uniform)
-        const int64_t c_first = (s + kChunk - 1) / kChunk, c_last = e_ / kChunk;      // whole chunks [c_first, c_last)
-        const int64_t head = c_first < c_last ? c_first * kChunk : e_, tail = c_first < c_last ? c_last * kChunk : e_;
-        float acc[VEC];
+    if (!__syncthreads_or(is_long)) return;
+    if (lane == 0) {
+        run[slot][0] = s;
+        run[slot][1] = e_;
+    }
+    __syncthreads();
+    for (int q = 0; q < slots; q++) {                       // long runs: all slots on one row, joined in the order of the slots
+        const int64_t rs = run[q][0], re = run[q][1];
+        if (re - rs <= kShort) continue;                    // (uniform)
+        const int64_t c_first = (rs + kChunk - 1) / kChunk, c_last = re / kChunk;      // whole chunks [c_first, c_last)
+        const int64_t head = c_first < c_last ? c_first * kChunk : re, tail = c_first < c_last ? c_last * kChunk : re;
+        for (int c0 = 0; c0 < D; c0 += lanes * VEC) {
+            const int col = c0 + lane * VEC;
+            float acc[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; e++) acc[e] = 0.f;
-        if (col < D) {
-#pragma unroll 4
-            for (int64_t j = s + slot; j < head; j += slots) add_row<T, VEC>(grad + (int64_t)pos[j] * ldg + col, D - col, acc);
-#pragma unroll 4
-            for (int64_t j = tail + slot; j < e_; j += slots) add_row<T, VEC>(grad + (int64_t)pos[j] * ldg + col, D - col, acc);
-#pragma unroll 4
-            for (int64_t c = c_first + slot; c < c_last; c += slots) add_row<float, VEC>(partial + c * D + col, D - col, acc);
+            for (int e = 0; e < VEC; e++) acc[e] = 0.f;
+            if (col < D) {
+                const int64_t skip = tail - head;           // head and tail as one sequence
+                add_entries<4, T, VEC>(rs + slot, re - skip, slots, D - col, [&](int64_t j) { return grad + (int64_t)pos[j < head ? j : j + skip] * ldg + col; }, acc);
+                add_entries<4, float, VEC>(c_first + slot, c_last, slots, D - col, [&](int64_t c) { return partial + c * D + col; }, acc);
+            }
+#pragma unroll
+            for (int e = 0; e < VEC; e++) join[e * 256 + tid] = acc[e];
+            __syncthreads();
+            if (slot == 0 && col < D) {
+                for (int o = 1; o < slots; o++)
+#pragma unroll
+                    for (int e = 0; e < VEC; e++) acc[e] += join[e * 256 + o * lanes + lane];
+                write(v0 + q, col, acc);
+            }
+            __syncthreads();
         }
-#pragma unroll
-        for (int e = 0; e < VEC; e++) join[e * 256 + tid] = acc[e];
-        __syncthreads();
-        if (slot == 0 && col < D) {
-            for (int q = 1; q < slots; q++)
-#pragma unroll
-                for (int e = 0; e < VEC; e++) acc[e] += join[e * 256 + q * lanes + lane];
-            write(r, acc);
-        }
-        __syncthreads();
     }
 }
 
 // ------------------------------------------------------------------------------------------------ host
 struct BwdPlan {
-    int bits, passes, nb_max;
+    int bits, passes, nb_max, tile;
     int64_t blocks, per;            // multi-block sort
-    int64_t off_keys[2], off_pos[2], off_hist, off_partial, bytes;
+    int64_t off_keys[2], off_pos[2], off_hist, off_partial, off_bounds, bytes;
 };
 
 int64_t up256(int64_t b) { return (b + 255) / 256 * 256; }
@@ -384,8 +451,9 @@ BwdPlan plan_bwd(int64_t n, int64_t V, int64_t D) {
     const int digit = one ? kOneDigit : kMultiDigit;
     p.passes = (p.bits + digit - 1) / digit;
     p.nb_max = (p.bits + p.passes - 1) / p.passes;
-    const int64_t tiles = (n + kTile - 1) / kTile;
-    p.per = ((tiles + kMaxBlocks - 1) / kMaxBlocks) * kTile;
+    p.tile = kSortThreads * (n <= kMaxBlocks * 1024 ? 1 : n <= kMaxBlocks * 2048 ? 2 : 4);
+    const int64_t tiles = (n + p.tile - 1) / p.tile;
+    p.per = ((tiles + kMaxBlocks - 1) / kMaxBlocks) * p.tile;
     p.blocks = one ? 1 : (n + p.per - 1) / p.per;
     int64_t at = 0;
     auto take = [&](int64_t b) { const int64_t r = at; at += up256(b); return r; };
@@ -396,6 +464,7 @@ BwdPlan plan_bwd(int64_t n, int64_t V, int64_t D) {
     }
     p.off_hist = one ? 0 : take(p.blocks * 4ll << p.nb_max);
     p.off_partial = take((n / kChunk) * D * 4);
+    p.off_bounds = take(8 * (V + 1));
     p.bytes = at;
     return p;
 }
@@ -408,27 +477,34 @@ void launch_one(const I *idx, int n, int64_t V, int64_t padding, const BwdPlan &
     k_sort_one<I, R><<<1, kSortThreads, lds, s>>>(idx, n, V, padding, p.bits, p.passes, keys, pos);
 }
 
+template <typename I, int R>
+void launch_scatter(const I *idx, const uint32_t *k_in, const uint32_t *p_in, int64_t n, int64_t V, int64_t padding, const BwdPlan &p, int shift, int nb, const uint32_t *hist,
+                    uint32_t *keys, uint32_t *pos, hipStream_t s) {
+    auto lds = [](int bins) { return 4 * (3 * bins + kSortWaves + 2 * R * kSortThreads) + 2 * kSortWaves * bins; };
+    static hsLdsAttrOnce attr;
+    attr.set((const void *)k_sort_scatter<I, R>, lds(1 << kMultiDigit));
+    k_sort_scatter<I, R><<<(unsigned)p.blocks, kSortThreads, lds(1 << nb), s>>>(idx, k_in, p_in, n, p.per, V, padding, shift, nb, hist, keys, pos);
+}
+
 template <typename I>
 void launch_sort(const I *idx, int64_t n, int64_t V, int64_t padding, const BwdPlan &p, char *ws, uint32_t *&keys, uint32_t *&pos, hipStream_t s) {
     if (n <= kOneMax) {
         keys = (uint32_t *)(ws + p.off_keys[0]);
         pos = (uint32_t *)(ws + p.off_pos[0]);
         if (n <= 1024) launch_one<I, 1>(idx, (int)n, V, padding, p, keys, pos, s);
-        else if (n <= 4096) launch_one<I, 4>(idx, (int)n, V, padding, p, keys, pos, s);
-        else launch_one<I, 16>(idx, (int)n, V, padding, p, keys, pos, s);
+        else launch_one<I, 4>(idx, (int)n, V, padding, p, keys, pos, s);
         return;
     }
-    static hsLdsAttrOnce attr;
-    attr.set((const void *)k_sort_scatter<I>, 4 * (2 * 2048 + kSortWaves) + 2 * kSortWaves * 2048);
     uint32_t *hist = (uint32_t *)(ws + p.off_hist), *k_in = nullptr, *p_in = nullptr;
     int shift = 0;
     for (int pass = 0; pass < p.passes; pass++) {
-        const int nb = (p.bits - shift + p.passes - pass - 1) / (p.passes - pass), bins = 1 << nb;
+        const int nb = (p.bits - shift + p.passes - pass - 1) / (p.passes - pass);
         keys = (uint32_t *)(ws + p.off_keys[pass & 1]);
         pos = (uint32_t *)(ws + p.off_pos[pass & 1]);
         k_sort_hist<I><<<(unsigned)p.blocks, kSortThreads, 0, s>>>(idx, k_in, n, p.per, V, padding, shift, nb, hist);
-        k_sort_scatter<I><<<(unsigned)p.blocks, kSortThreads, 4 * (2 * bins + kSortWaves) + 2 * kSortWaves * bins, s>>>(idx, k_in, p_in, n, p.per, V, padding, shift, nb,
-                                                                                                                     hist, keys, pos);
+        if (p.tile == 1024) launch_scatter<I, 1>(idx, k_in, p_in, n, V, padding, p, shift, nb, hist, keys, pos, s);
+        else if (p.tile == 2048) launch_scatter<I, 2>(idx, k_in, p_in, n, V, padding, p, shift, nb, hist, keys, pos, s);
+        else launch_scatter<I, 4>(idx, k_in, p_in, n, V, padding, p, shift, nb, hist, keys, pos, s);
         k_in = keys;
         p_in = pos;
         shift += nb;
@@ -476,7 +552,7 @@ int hs_embed_bwd(const void *indices, int32_t index_bytes, const void *grad, int
                  int32_t grad_dtype, int32_t table_dtype, void *ws, int64_t ws_bytes, void *stream) {
     if (!sizes_ok(n, V, D) || (index_bytes != 4 && index_bytes != 8) || !known_dtype(grad_dtype) || !known_dtype(table_dtype) || ldg < D) return HS_ERR_ARG;
     if (V == 0 || D == 0) return HS_OK;
-    if (!grad_table || (n > 0 && (!indices || !grad || !ws))) return HS_ERR_NULL;
+    if (!grad_table || !ws || (n > 0 && (!indices || !grad))) return HS_ERR_NULL;
     const BwdPlan p = plan_bwd(n, V, D);
     if (ws_bytes < p.bytes) return HS_ERR_ARG;
     hipStream_t s = (hipStream_t)stream;
@@ -490,13 +566,15 @@ int hs_embed_bwd(const void *indices, int32_t index_bytes, const void *grad, int
     int lanes = pow2_at_least((int)((D + VEC - 1) / VEC));
     lanes = lanes > 64 ? 64 : lanes;
     const unsigned col_blocks = (unsigned)((D + (int64_t)lanes * VEC - 1) / ((int64_t)lanes * VEC));
-    const int64_t row_blocks = (V + kRowsPerGroup - 1) / kRowsPerGroup;
+    const int64_t row_blocks = (V + 256 / lanes - 1) / (256 / lanes);
+    const unsigned bound_blocks = (unsigned)(V / 256 + 1);
+    uint2 *bounds = (uint2 *)((char *)ws + p.off_bounds);
     HS_BY_DTYPE(grad_dtype, {
         using G = T;
         constexpr int W = sizeof(T) == 4 ? 4 : 8;
-        if (n >= kChunk)
-            k_embed_chunks<G, W><<<dim3((unsigned)(n / kChunk), col_blocks), 256, 0, s>>>(keys, pos, (const G *)grad, ldg, n, (uint32_t)V, (int)D, lanes, partial);
-        HS_BY_DTYPE(table_dtype, (k_embed_rows<G, T, W><<<dim3((unsigned)row_blocks, col_blocks), 256, 0, s>>>(keys, pos, (const G *)grad, ldg, n, V, (int)D, lanes, partial,
+        k_embed_chunks<G, W><<<dim3(bound_blocks + (unsigned)(n / kChunk), col_blocks), 256, 0, s>>>(keys, pos, (const G *)grad, ldg, n, (uint32_t)V, (int)D, lanes, partial,
+                                                                                                  bounds, bound_blocks);
+        HS_BY_DTYPE(table_dtype, (k_embed_rows<G, T, W><<<(unsigned)row_blocks, 256, 0, s>>>(bounds, pos, (const G *)grad, ldg, V, (int)D, lanes, partial,
                                                                                                            scale, (T *)grad_table)));
     });
     return hipGetLastError() == hipSuccess ? HS_OK : HS_ERR_LAUNCH;

@@ -40,10 +40,10 @@ def test_embed_work_space_grows_with_its_parts():
     f = lib().hs_embed_bwd_ws_bytes
     assert f(I64(-1), I64(1), I64(1)) == -1
     assert f(I64(1), I64(1), I64(1)) >= 8
-    for n, V, D in ((16384, 50021, 2048), (16385, 100, 7), (131072, 1024, 32), (1 << 20, 1 << 22, 64)):
-        multi = n > 16384
-        passes = -(-V.bit_length() // 11)
-        assert f(I64(n), I64(V), I64(D)) >= 8 * n * (2 if multi and passes > 1 else 1) + (n // 64) * D * 4
+    for n, V, D in ((4096, 50021, 2048), (4097, 100, 7), (131072, 1024, 32), (1 << 20, 1 << 22, 64)):
+        multi = n > 4096
+        passes = -(-V.bit_length() // 9)
+        assert f(I64(n), I64(V), I64(D)) >= 8 * n * (2 if multi and passes > 1 else 1) + (n // 32) * D * 4
 
 
 def test_dropout_refusals():
