@@ -81,49 +81,40 @@ __global__ __launch_bounds__(256) void k_rows_reduce(const float *__restrict__ p
 // ------------------------------------------------------------------------------------------------ products
 // Which tile, and into how many slices K is cut, by what a step of 64 of K costs (microseconds, measured at 8 192 x 4 096 x 12 288 and 1 021 x 1 000 x 2 730):
 // a lone workgroup on a CU waits for its requests (`first`), every further one of the `fit` that LDS admits adds its own work (`more`).  The 256 x 256
-// tile reads the least per product and has the highest rate (1.1 PFLOP/s against 0.93 and 0.6); with few tiles of the result the smaller ones, or
+// tile reads the least per product and has the highest rate (1.2 PFLOP/s against 0.93 and 0.6); with few tiles of the result the smaller ones, or
 // slices whose fp32 partial results are added up by another launch, fill the device.  E.g. 1 021 x 1 000 over K = 5 460: 52 us in 64 x 64 tiles,
-// 72 in 128 x 128, 31 in 128 x 128 and four slices.
+// 72 in 128 x 128, 31 in 128 x 128 and four slices.  fp32 (six plane products): the large tile in
+// six passes, 200 TFLOP/s; small tiles with the planes in LDS, one workgroup a CU.
 struct Plan { int tile, slices; };
-struct TileCost { int size, fit; float first, more; };
-inline Plan plan_product(int64_t I, int64_t cols, int64_t steps, int problems, bool sliceable, int64_t out_bytes) {
-    static const TileCost kinds[3] = {{256, 1, 1.9f, 0.f}, {128, 2, 0.75f, 0.41f}, {64, 5, 0.5f, 0.15f}};
-    Plan best = {256, 1};
+struct TileCost { int rows, cols, fit; float first, more; };
+constexpr TileCost kTiles16[3] = {{256, 256, 1, 1.9f, 0.f}, {128, 128, 2, 0.75f, 0.41f}, {64, 64, 5, 0.5f, 0.15f}};
+constexpr TileCost kTiles32[3] = {{256, 256, 1, 11.4f, 0.f}, {128, 64, 1, 2.1f, 0.f}, {64, 64, 1, 1.15f, 0.f}};
+template <typename U> Plan plan_product(int64_t I, int64_t cols, int64_t steps, int problems, bool sliceable) {
+    const TileCost *kinds = sizeof(U) == 4 ? kTiles32 : kTiles16;
+    Plan best = {0, 1};
     float least = 0.f;
-    for (const TileCost &t : kinds)
+    for (int k = 0; k < 3; k++)
         for (int slices = 1; slices <= (sliceable ? 64 : 1); slices *= 2) {
             if (slices > 1 && steps / slices < 4) break;
-            const int64_t groups = ((I + t.size - 1) / t.size) * ((cols + t.size - 1) / t.size) * problems * slices;
+            const TileCost &t = kinds[k];
+            const int64_t groups = ((I + t.rows - 1) / t.rows) * ((cols + t.cols - 1) / t.cols) * problems * slices;
             const int64_t each = (groups + 255) / 256, together = each < t.fit ? each : t.fit, rounds = (groups + 256 * together - 1) / (256 * together);
             float us = (float)rounds * ((float)((steps + slices - 1) / slices) * (t.first + t.more * (float)(together - 1)) + 3.f);
-            if (slices > 1) us += 4.f + (float)out_bytes * (float)(2 * slices) * 2.5e-7f;        // partial results written and read at 4 TB/s, one launch more
+            if (slices > 1) us += 4.f + (float)(I * cols * problems) * (float)slices * 2e-6f;        // partial results written and read at 4 TB/s, one launch more
             if (least == 0.f || us < least) {
                 least = us;
-                best = Plan{t.size, slices};
+                best = Plan{k, slices};
             }
         }
     return best;
 }
 
 template <typename T, typename U, bool AKS, bool BKS, int EPI> int launch_product(Args &p, int tile, int problems, hipStream_t s) {
-    if (tile == 256) return launch_tile<T, U, 256, 256, 2, 4, AKS, BKS, EPI>(p, problems, s);
-    if (tile == 128) return launch_tile<T, U, 128, 128, 2, 2, AKS, BKS, EPI>(p, problems, s);
-    return launch_tile<T, U, 64, 64, 2, 2, AKS, BKS, EPI>(p, problems, s);
+    constexpr int P = planes<U>();
+    if (tile == 0) return launch_tile<T, U, 1, 256, 256, 2, 4, AKS, BKS, EPI>(p, problems, s);
+    if (tile == 1) return launch_tile<T, U, P, 128, P == 3 ? 64 : 128, 2, 2, AKS, BKS, EPI>(p, problems, s);
+    return launch_tile<T, U, P, 64, 64, 2, 2, AKS, BKS, EPI>(p, problems, s);
 }
-
-// the segments of one product: one pair, or the six plane products of an fp32 one
-template <typename U> int add_segments(Seg *seg, int n, const Operand &a, const Operand &b, const Operand *b1 = nullptr) {
-    if constexpr (sizeof(U) == 4) {
-        static const int pa[6] = {0, 1, 2, 0, 1, 0}, pb[6] = {2, 1, 0, 1, 0, 0};
-        for (int t = 0; t < 6; t++)
-            seg[n++] = Seg{(const bf16_t *)a.p + pa[t] * a.plane, (const bf16_t *)b.p + pb[t] * b.plane, b1 ? (const void *)((const bf16_t *)b1->p + pb[t] * b1->plane) : nullptr};
-    } else {
-        seg[n++] = Seg{a.p, b.p, b1 ? b1->p : nullptr};
-    }
-    return n;
-}
-
-template <typename U> constexpr int planes() { return sizeof(U) == 4 ? 3 : 1; }
 
 // Up to this D the backward pass computes G and U again: 4 D operations an element against 16 bytes.  (At D = 256, 131 072 x 1 024: forward and this part of the
 // backward 660 us against 780 with G and U kept.)
@@ -139,10 +130,10 @@ template <typename T, typename U> struct Block {
     hipStream_t s;
     bool run;
     int rc = HS_OK;
-    int64_t M, D, F, ldh, ldd;
+    int64_t M, D, F, ldh;
 
     Block(const hsGatedMlp &args, bool run_, hipStream_t stream) : a(args), ws{run_ ? (char *)args.ws : nullptr}, s(stream), run(run_), M(args.rows), D(args.dim), F(args.hidden),
-                                                                  ldh(up8(args.hidden)), ldd(up8(args.dim)) {}
+                                                                  ldh(up8(args.hidden)) {}
 
     void check(int r) { if (rc == HS_OK) rc = r; }
 
@@ -219,21 +210,30 @@ template <typename T, typename U> struct Block {
             sv.h = Operand{ws.take(M * ldh * 2 * planes<U>()), ldh, M * ldh};
         }
         if (!fits<false, false>(x, wg) || !fits<false, false>(wd, sv.h)) return;
-        Args p = {};
-        p.n_seg = add_segments<U>(p.seg[0], 0, x, wg, &wu);
-        p.lda = x.ld; p.ldb = wg.ld; p.I = M; p.J = (int)F; p.K = (int)D; p.slices = 1;
+        Args p = product(x, wg, M, F, D);
+        p.seg[0][0].b1 = wu.p;
         p.g = sv.g; p.u = sv.u; p.h = (void *)sv.h.p; p.ldh = ldh; p.plane = sv.h.plane; p.act = a.activation;
-        if (run && rc == HS_OK) check(launch_product<T, U, false, false, EPI_GATE>(p, plan_product(M, 2 * ldh, (D + BK - 1) / BK * p.n_seg, 1, false, 0).tile, 1, s));
-        Args q = {};
-        q.n_seg = add_segments<U>(q.seg[0], 0, sv.h, wd);
-        q.lda = ldh; q.ldb = wd.ld; q.I = M; q.J = (int)D; q.K = (int)F;
+        if (run && rc == HS_OK) check(launch_product<T, U, false, false, EPI_GATE>(p, plan_product<U>(M, 2 * ldh, steps(D), 1, false).tile, 1, s));
+        Args q = product(sv.h, wd, M, D, F);
         result<false, false>(q, &a.y, 1);
+    }
+
+    static int64_t steps(int64_t k) { return (k + BK - 1) / BK; }
+
+    // C [I, J] = a b^T over K, everything but where it goes
+    static Args product(const Operand &a, const Operand &b, int64_t I, int64_t J, int64_t K) {
+        Args p = {};
+        p.seg[0][0] = Seg{a.p, b.p, nullptr};
+        p.n_seg = 1;
+        p.lda = a.ld; p.ldb = b.ld; p.plane_a = a.plane * 2; p.plane_b = b.plane * 2;
+        p.I = I; p.J = (int)J; p.K = (int)K; p.slices = 1;
+        return p;
     }
 
     // The results of up to two products of one shape (p holds everything but the outputs): out[z] [I, J], contiguous.
     template <bool AKS, bool BKS> void result(Args &p, void *const *out, int problems) {
-        const int64_t n = p.I * p.J, stride = (n + 3) / 4 * 4, steps = (p.K + BK - 1) / BK * (int64_t)p.n_seg;
-        const Plan plan = plan_product(p.I, p.J, steps, problems, true, 4 * n * problems);
+        const int64_t n = p.I * p.J, stride = (n + 3) / 4 * 4;
+        const Plan plan = plan_product<U>(p.I, p.J, steps(p.K) * p.n_seg, problems, true);
         float *parts = plan.slices > 1 ? (float *)ws.take(stride * 4 * plan.slices * problems) : nullptr;
         if (!run || rc != HS_OK) return;
         p.ldo = p.J;
@@ -255,9 +255,8 @@ template <typename T, typename U> struct Block {
     // C_z [I, J] = A_z^T B over the rows
     void weight_gradient(const Operand *av, const Operand &b, void *const *out, int problems, int64_t I, int64_t J) {
         if (!fits<true, true>(av[0], b)) return;
-        Args p = {};
-        for (int z = 0; z < problems; z++) p.n_seg = add_segments<U>(p.seg[z], 0, av[z], b);
-        p.lda = av[0].ld; p.ldb = b.ld; p.I = I; p.J = (int)J; p.K = (int)M;
+        Args p = product(av[0], b, I, J, M);
+        if (problems == 2) p.seg[1][0] = Seg{av[1].p, b.p, nullptr};
         result<true, true>(p, out, problems);
     }
 
@@ -272,26 +271,22 @@ template <typename T, typename U> struct Block {
             if (again() || a.gx) projections(wg, wu);
             if (again() || a.gw_gate || a.gw_up) x = operand(a.x, a.ldx, M, D);
             if (fits<false, true>(gy, wd) && (!again() || fits<false, false>(x, wg)) && run) {
-                Args p = {};
-                p.I = M; p.J = (int)F; p.K = (int)D; p.slices = 1;
+                Args p = again() ? product(x, wg, M, F, D) : product(gy, wd, M, F, D);
                 p.g = sv.g; p.u = sv.u; p.gg = (void *)gg.p; p.gu = (void *)gu.p; p.ldh = ldh; p.plane = n; p.act = a.activation;
                 if (again()) {
-                    p.n_seg = add_segments<U>(p.seg[0], 0, x, wg, &wu);
-                    add_segments<U>(p.seg[1], 0, gy, wd);
-                    p.lda = x.ld; p.ldb = wg.ld; p.lda2 = gy.ld; p.ldb2 = wd.ld;
+                    p.seg[0][0].b1 = wu.p;
+                    p.seg[1][0] = Seg{gy.p, wd.p, nullptr};
+                    p.lda2 = gy.ld; p.ldb2 = wd.ld; p.plane_a2 = gy.plane * 2; p.plane_b2 = wd.plane * 2;
                     check(launch_gate_bwd<T, U>(p, s));
                 } else {
-                    p.n_seg = add_segments<U>(p.seg[0], 0, gy, wd);
-                    p.lda = gy.ld; p.ldb = wd.ld;
-                    check(launch_product<T, U, false, true, EPI_GATE_BWD>(p, plan_product(M, ldh, (D + BK - 1) / BK * p.n_seg, 1, false, 0).tile, 1, s));
+                    check(launch_product<T, U, false, true, EPI_GATE_BWD>(p, plan_product<U>(M, ldh, steps(D), 1, false).tile, 1, s));
                 }
             }
             if (a.gx) {
                 if (fits<false, true>(gg, wg)) {
-                    Args p = {};
-                    p.n_seg = add_segments<U>(p.seg[0], 0, gg, wg);
-                    p.n_seg = add_segments<U>(p.seg[0], p.n_seg, gu, wu);
-                    p.lda = ldh; p.ldb = wg.ld; p.I = M; p.J = (int)D; p.K = (int)F;
+                    Args p = product(gg, wg, M, D, F);
+                    p.seg[0][1] = Seg{gu.p, wu.p, nullptr};
+                    p.n_seg = 2;
                     result<false, true>(p, &a.gx, 1);
                 }
             }

@@ -2,8 +2,10 @@
 //
 //     C [I, J] = sum over segments of  A_s [I, K] . B_s [J, K]^T,   fp32 accumulators
 //
-// A segment is one pair of operands.  One: a plain product.  Two: gx = gg Wg + gu Wu in one pass.  Six: an fp32 product, whose operands
-// are sums of three bf16 planes each (gemm_split.hip has the arithmetic: the plane products of combined weight >= 2^-16, smallest first).
+// A segment is one pair of operands.  One: a plain product.  Two: gx = gg Wg + gu Wu in one pass.  An operand of the 16-bit types is one matrix; an fp32
+// one is the sum of three bf16 planes, and its product six plane products (those of combined weight >= 2^-16, smallest first; gemm_split.hip has the
+// arithmetic).  Small tiles have all planes in LDS together (P = 3): a step is 64 of K, each fragment takes part in up to three products.  The large tile has no
+// room for that and takes the six as segments, one after the other (P = 1): it reads every plane twice, and still less per product.
 // Either operand may have K as its contiguous index ([rows, K], ld) or as its strided one ([K, rows], ld); all four products of the
 // block and its gradient are of that form, so nothing is ever transposed in memory.
 //
@@ -38,12 +40,15 @@ typedef short i16x8 __attribute__((ext_vector_type(8)));
 constexpr int BK = 64;
 constexpr int kMaxSeg = 12;
 
+template <typename U> constexpr int planes() { return sizeof(U) == 4 ? 3 : 1; }
+
 struct Seg { const void *a, *b, *b1; };          // b1: the up projection's weights beside the gate's (EPI_GATE)
 
 struct Args {
     Seg seg[2][kMaxSeg];                          // [problem][segment]
     int32_t n_seg;
     int64_t lda, ldb;                             // in elements, multiples of 8
+    int64_t plane_a, plane_b;                     // bytes between planes
     int64_t I;
     int32_t J, K;
     int32_t tiles_i, tiles_j, slices;
@@ -57,7 +62,7 @@ struct Args {
     int64_t ldh, plane;                           // plane: elements between planes
     int32_t act;
     // k_gate_bwd: the second product's operands are seg[1]
-    int64_t lda2, ldb2;
+    int64_t lda2, ldb2, plane_a2, plane_b2;
 };
 
 enum { EPI_STORE = 0, EPI_PARTIAL = 1, EPI_GATE = 2, EPI_GATE_BWD = 3 };       // result; fp32 partial result; H (G, U); gg, gu from G, U
@@ -265,34 +270,51 @@ template <int COLS, int MT, int MP_, int WI, int WAVES, int TJ> struct Staging {
 
 template <int... I, typename F> __device__ __forceinline__ void static_for(std::integer_sequence<int, I...>, F f) { (f(std::integral_constant<int, I>{}), ...); }
 
+// c += the product of two fragments of P planes, the smallest plane products first
+template <typename T, int P> __device__ __forceinline__ f32x4 plane_product(int term, const i16x8 (&w)[P], const i16x8 (&x)[P], f32x4 c) {
+    constexpr int pw[6] = {0, 1, 2, 0, 1, 0}, px[6] = {2, 1, 0, 1, 0, 0};        // (which side is called the first does not matter)
+    return P == 1 ? mfma<T>(w[0], x[0], c) : mfma<T>(w[pw[term]], x[px[term]], c);
+}
+
 // One step (64 of K) of a wave's products.  Fragments are requested PF groups of matrix instructions ahead of their use, and the order written here is pinned
 // (sched_group_barrier: 0x100 LDS reads, 0x8 matrix instructions): left to itself the compiler puts every read directly in front of its use, with a wait for
-// its whole latency between.  a(m, ks), b(n, ks): the fragments; RA, RB: LDS instructions of one.  request(): the next step's LDS-DMA, issued while the
-// first fragments are on their way.
-template <typename T, int MT, int NT, int RA, int RB, typename A, typename B, typename R>
+// its whole latency between (8 192 x 4 096 x 12 288: 774 -> 699 us).  a(m, ks, plane), b(n, ks, plane): the fragments; RA, RB: LDS instructions of one.
+// request(): the next step's LDS-DMA, issued while the first fragments are on their way.
+template <typename T, int MT, int NT, int P, int RA, int RB, typename A, typename B, typename R>
 __device__ __forceinline__ void multiply_step(A a, B b, R request, f32x4 (&acc)[MT][NT]) {
-    constexpr int G = 2 * MT, PF = MT >= 4 ? 3 : 2;
-    i16x8 fa[G], fb[2][NT];
+    constexpr int G = 2 * MT, PF = P == 3 ? 1 : MT >= 4 ? 3 : 2, TERMS = P == 3 ? 6 : 1;
+    i16x8 fa[G][P], fb[2][NT][P];
 #pragma unroll
-    for (int n = 0; n < NT; n++) fb[0][n] = b(n, 0);
+    for (int n = 0; n < NT; n++)
 #pragma unroll
-    for (int g = 0; g < PF; g++) fa[g] = a(g % MT, g / MT);
+        for (int q = 0; q < P; q++) fb[0][n][q] = b(n, 0, q);
+#pragma unroll
+    for (int g = 0; g < PF; g++)
+#pragma unroll
+        for (int q = 0; q < P; q++) fa[g][q] = a(g % MT, g / MT, q);
     request();
     static_for(std::make_integer_sequence<int, G>{}, [&](auto group) {
         constexpr int g = decltype(group)::value, b0 = g < MT ? g * NT / MT : NT, b1 = g < MT ? (g + 1) * NT / MT : NT;
-        constexpr int reads = (g + PF < G ? RA : 0) + (b1 - b0) * RB;
-        if constexpr (g + PF < G) fa[g + PF] = a((g + PF) % MT, (g + PF) / MT);
+        constexpr int reads = P * ((g + PF < G ? RA : 0) + (b1 - b0) * RB);
+        if constexpr (g + PF < G) {
 #pragma unroll
-        for (int n = b0; n < b1; n++) fb[1][n] = b(n, 1);
+            for (int q = 0; q < P; q++) fa[g + PF][q] = a((g + PF) % MT, (g + PF) / MT, q);
+        }
 #pragma unroll
-        for (int n = 0; n < NT; n++) acc[g % MT][n] = mfma<T>(fb[g / MT][n], fa[g], acc[g % MT][n]);
+        for (int n = b0; n < b1; n++)
+#pragma unroll
+            for (int q = 0; q < P; q++) fb[1][n][q] = b(n, 1, q);
+#pragma unroll
+        for (int t = 0; t < TERMS; t++)
+#pragma unroll
+            for (int n = 0; n < NT; n++) acc[g % MT][n] = plane_product<T, P>(t, fb[g / MT][n], fa[g], acc[g % MT][n]);
         if constexpr (reads > 0) __builtin_amdgcn_sched_group_barrier(0x100, reads, 0);
-        __builtin_amdgcn_sched_group_barrier(0x8, NT, 0);
+        __builtin_amdgcn_sched_group_barrier(0x8, NT * TERMS, 0);
     });
 }
 
-// T: the matrix instruction's type; U: the user's type (float: T = bf16, planes).
-template <typename T, typename U, int BM, int BN, int WI, int WJ, bool AKS, bool BKS, int EPI>
+// T: the matrix instruction's type; U: the user's type (float: T = bf16, planes); P: planes in LDS.
+template <typename T, typename U, int P, int BM, int BN, int WI, int WJ, bool AKS, bool BKS, int EPI>
 __global__ __launch_bounds__(64 * WI * WJ) void k_rows_gemm(const Args p) {
     constexpr int WAVES = WI * WJ, MT = BM / WI / 16, NT = BN / WJ / 16;
     constexpr bool DUAL = EPI == EPI_GATE;
@@ -312,6 +334,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_rows_gemm(const Args p) {
     sb.init(wave, lane, (int64_t)p.J - j0, p.ldb, DUAL);
     sa.init_frags(lane, wi * MT);
     sb.init_frags(lane, DUAL ? wj * (NT / 2) : wj * NT);
+    constexpr uint32_t kBuf = P * (SA::kBytes + SB::kBytes);
     const uint32_t lds0 = lds_addr(lds);
     const int steps_k = (p.K + BK - 1) / BK, steps = steps_k * p.n_seg;
     const int s_begin = (int)((int64_t)steps * blockIdx.y / p.slices), s_end = (int)((int64_t)steps * (blockIdx.y + 1) / p.slices);
@@ -326,9 +349,13 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_rows_gemm(const Args p) {
     };
     auto request = [&](int buf) {
         const int64_t left = p.K - (int64_t)kk * BK;
-        const uint32_t at = lds0 + (uint32_t)buf * (SA::kBytes + SB::kBytes);
-        sa.request(wave, pa, pa, left, at);
-        sb.request(wave, pb, DUAL ? pb1 : pb, left, at + SA::kBytes);
+        const uint32_t at = lds0 + (uint32_t)buf * kBuf;
+#pragma unroll
+        for (int q = 0; q < P; q++) {
+            const char *a = pa + q * p.plane_a, *b = pb + q * p.plane_b, *b1 = DUAL ? pb1 + q * p.plane_b : b;
+            sa.request(wave, a, a, left, at + q * SA::kBytes);
+            sb.request(wave, b, b1, left, at + P * SA::kBytes + q * SB::kBytes);
+        }
         pa += a_step;
         pb += b_step;
         if constexpr (DUAL) pb1 += b_step;
@@ -349,11 +376,11 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_rows_gemm(const Args p) {
     int buf = 0;
     for (int s = s_begin; s < s_end; s++) {
         wait_and_meet();            // step s has landed for every wave; every wave is done with the other buffer
-        const uint32_t at = lds0 + (uint32_t)buf * (SA::kBytes + SB::kBytes);
-        multiply_step<T, MT, NT, AKS ? 2 : 1, BKS ? 2 : 1>(
-            [&](int m, int ks) { return sa.fragment(at, m, ks); },
-            [&](int n, int ks) {         // (EPI_GATE: the tile's upper half is the up projection's rows)
-                return DUAL && n >= NT / 2 ? sb.fragment(at + SA::kBytes, n - NT / 2, ks, BN / 2) : sb.fragment(at + SA::kBytes, n, ks);
+        const uint32_t at = lds0 + (uint32_t)buf * kBuf, at_b = at + P * SA::kBytes;
+        multiply_step<T, MT, NT, P, AKS ? 2 : 1, BKS ? 2 : 1>(
+            [&](int m, int ks, int q) { return sa.fragment(at + q * SA::kBytes, m, ks); },
+            [&](int n, int ks, int q) {         // (EPI_GATE: the tile's upper half is the up projection's rows)
+                return DUAL && n >= NT / 2 ? sb.fragment(at_b + q * SB::kBytes, n - NT / 2, ks, BN / 2) : sb.fragment(at_b + q * SB::kBytes, n, ks);
             },
             [&]() { if (s + 1 < s_end) request(buf ^ 1); }, acc);
         buf ^= 1;
@@ -452,8 +479,22 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_rows_gemm(const Args p) {
     }
 }
 
-template <typename T, typename U, int BM, int BN, int WI, int WJ, bool AKS, bool BKS, int EPI>
-inline int launch_tile(Args &p, int problems, hipStream_t s) {
+constexpr int kPlaneA[6] = {0, 1, 2, 0, 1, 0}, kPlaneB[6] = {2, 1, 0, 1, 0, 0};      // the six plane products, smallest first
+
+// every pair of fp32 operands as six pairs of planes
+inline void as_segments(Args &p) {
+    for (int z = 0; z < 2; z++)
+        for (int s = p.n_seg - 1; s >= 0; s--) {
+            const Seg pair = p.seg[z][s];
+            const int64_t a = z && p.plane_a2 ? p.plane_a2 : p.plane_a, b = z && p.plane_b2 ? p.plane_b2 : p.plane_b;        // (k_gate_bwd's second product)
+            for (int t = 0; t < 6; t++)
+                p.seg[z][6 * s + t] = Seg{(const char *)pair.a + kPlaneA[t] * a, (const char *)pair.b + kPlaneB[t] * b, (const char *)pair.b1 + kPlaneB[t] * b};
+        }
+    p.n_seg *= 6;
+}
+
+template <typename T, typename U, int P, int BM, int BN, int WI, int WJ, bool AKS, bool BKS, int EPI>
+inline int launch_tile(Args p, int problems, hipStream_t s) {
     constexpr int TJ = EPI == EPI_GATE ? BN / 2 : BN;
     // the gate epilogues also write the padding columns up to ldh (< J + 8)
     const int64_t cols = EPI == EPI_GATE || EPI == EPI_GATE_BWD ? p.ldh : p.J;
@@ -461,22 +502,26 @@ inline int launch_tile(Args &p, int problems, hipStream_t s) {
     if (ti * tj > 0x7fffffff / 8 || p.slices > 65535) return HS_ERR_ARG;
     p.tiles_i = (int)ti;
     p.tiles_j = (int)tj;
-    constexpr int lds = 2 * (BM + BN) * BK * 2;
+    if constexpr (planes<U>() != P) as_segments(p);
+    constexpr int lds = 2 * P * (BM + BN) * BK * 2;
     static_assert(Staging<BN, BM / WI / 16, 2, WI, WI * WJ, TJ>::kBytes <= lds, "the epilogue's tile must fit");
     static hsLdsAttrOnce attr;
-    const void *fn = (const void *)k_rows_gemm<T, U, BM, BN, WI, WJ, AKS, BKS, EPI>;
+    const void *fn = (const void *)k_rows_gemm<T, U, P, BM, BN, WI, WJ, AKS, BKS, EPI>;
     attr.set(fn, lds);
-    k_rows_gemm<T, U, BM, BN, WI, WJ, AKS, BKS, EPI><<<dim3((unsigned)(ti * tj), (unsigned)p.slices, (unsigned)problems), 64 * WI * WJ, lds, s>>>(p);
+    k_rows_gemm<T, U, P, BM, BN, WI, WJ, AKS, BKS, EPI><<<dim3((unsigned)(ti * tj), (unsigned)p.slices, (unsigned)problems), 64 * WI * WJ, lds, s>>>(p);
     return hipGetLastError() == hipSuccess ? HS_OK : HS_ERR_LAUNCH;
 }
 
 // ------------------------------------------------------------------------------------------------ gg and gu without G and U
 // gH = gy Wd, G = x Wg^T, U = x Wu^T over the same K = D in one workgroup: 4 D operations an element of H more than reading G and U back, 16 bytes less written
-// and read (fp32: 16-bit G and U would add two roundings to every gradient).  Tile 128 x 64 of each of the three, four waves, two workgroups a CU.
+// and read (fp32: 16-bit G and U would add two roundings to every gradient).  Tile 128 x 64 of each of the three, four waves, two workgroups a CU
+// (fp32: plane products as segments).  Larger tiles read less and were slower: with K this short half the time is the beginnings and the ends of tiles, and a second
+// workgroup is what fills them (131 072 x 256 x 1 024: 383 us; 128 x 128 435, 256 x 64 435, 256 x 128 413; 24 % of the cycles in the matrix cores, 37 % in
+// the vector units).
 constexpr int kAgainM = 128, kAgainJ = 64;
 
 template <typename T, typename U>
-__global__ __launch_bounds__(256, 2) void k_gate_bwd(const Args p) {
+__global__ __launch_bounds__(256) void k_gate_bwd(const Args p) {
     constexpr int BM = kAgainM, TJ = kAgainJ, WAVES = 4, WI = 2, WJ = 2, MT = BM / WI / 16, N2 = TJ / WJ / 16, N1 = 2 * N2;
     using SA = Side<BM, false, WAVES, MT>;
     using S1 = Side<2 * TJ, false, WAVES, N1>;
@@ -530,8 +575,8 @@ __global__ __launch_bounds__(256, 2) void k_gate_bwd(const Args p) {
     for (int s = 0; s < steps; s++) {
         wait_and_meet();
         const uint32_t at = lds0 + buf * kBuf;
-        multiply_step<T, MT, N1, 1, 1>([&](int m, int ks) { return sx.fragment(at, m, ks); },
-                                       [&](int n, int ks) { return n < N2 ? s1.fragment(at + SA::kBytes, n, ks) : s1.fragment(at + SA::kBytes, n - N2, ks, TJ); },
+        multiply_step<T, MT, N1, 1, 1, 1>([&](int m, int ks, int) { return sx.fragment(at, m, ks); },
+                                       [&](int n, int ks, int) { return n < N2 ? s1.fragment(at + SA::kBytes, n, ks) : s1.fragment(at + SA::kBytes, n - N2, ks, TJ); },
                                        [&]() {
                                            if (s + 1 < steps) request1(buf ^ 1);
                                            else {
@@ -545,7 +590,7 @@ __global__ __launch_bounds__(256, 2) void k_gate_bwd(const Args p) {
     for (int s = 0; s < steps; s++) {
         wait_and_meet();
         const uint32_t at = lds0 + buf * kBuf;
-        multiply_step<T, MT, N2, 1, 2>([&](int m, int ks) { return sx.fragment(at, m, ks); }, [&](int n, int ks) { return s2.fragment(at + SA::kBytes, n, ks); },
+        multiply_step<T, MT, N2, 1, 1, 2>([&](int m, int ks, int) { return sx.fragment(at, m, ks); }, [&](int n, int ks, int) { return s2.fragment(at + SA::kBytes, n, ks); },
                                        [&]() { if (s + 1 < steps) request2(buf ^ 1); }, acc2);
         buf ^= 1;
     }
@@ -590,7 +635,8 @@ __global__ __launch_bounds__(256, 2) void k_gate_bwd(const Args p) {
     });
 }
 
-template <typename T, typename U> inline int launch_gate_bwd(Args &p, hipStream_t s) {
+template <typename T, typename U> inline int launch_gate_bwd(Args p, hipStream_t s) {
+    if constexpr (planes<U>() == 3) as_segments(p);
     const int64_t ti = (p.I + kAgainM - 1) / kAgainM, tj = (p.ldh + kAgainJ - 1) / kAgainJ;
     if (ti * tj > 0x7fffffff / 8) return HS_ERR_ARG;
     p.tiles_i = (int)ti;

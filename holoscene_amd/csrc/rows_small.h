@@ -47,15 +47,9 @@ template <typename T, typename U, int P> __device__ __forceinline__ void small_f
 }
 
 template <typename T, int P> __device__ __forceinline__ f32x4 small_product(const i16x8 (&w)[P], const i16x8 (&x)[P], f32x4 c) {
-    if constexpr (P == 1) return mfma<T>(w[0], x[0], c);
-    else {
-        c = mfma<T>(w[0], x[2], c);
-        c = mfma<T>(w[1], x[1], c);
-        c = mfma<T>(w[2], x[0], c);
-        c = mfma<T>(w[0], x[1], c);
-        c = mfma<T>(w[1], x[0], c);
-        return mfma<T>(w[0], x[0], c);
-    }
+#pragma unroll
+    for (int t = 0; t < (P == 3 ? 6 : 1); t++) c = plane_product<T, P>(t, w, x, c);
+    return c;
 }
 
 // the same of H as EPI_GATE left it: planes of whole fragments
