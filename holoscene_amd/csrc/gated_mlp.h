@@ -83,17 +83,18 @@ __global__ __launch_bounds__(256) void k_rows_reduce(const float *__restrict__ p
 // a lone workgroup on a CU waits for its requests (`first`), every further one of the `fit` that LDS admits adds its own work (`more`).  The 256 x 256
 // tile reads the least per product and has the highest rate (1.2 PFLOP/s against 0.93 and 0.6); with few tiles of the result the smaller ones, or
 // slices whose fp32 partial results are added up by another launch, fill the device.  E.g. 1 021 x 1 000 over K = 5 460: 52 us in 64 x 64 tiles,
-// 72 in 128 x 128, 31 in 128 x 128 and four slices.  fp32 (six plane products): the large tile in
+// 72 in 128 x 128, 29 in 128 x 128 and four slices, 22 with the requests three steps ahead (eight waves, four buffers, so one workgroup a CU: with
+// many tiles two workgroups of two buffers are faster, 228 us against 343 for G and U of 131 072 x 256 x 1 024).  fp32 (six plane products): the large tile in
 // six passes, 200 TFLOP/s; small tiles with the planes in LDS, one workgroup a CU.
 struct Plan { int tile, slices; };
 struct TileCost { int rows, cols, fit; float first, more; };
-constexpr TileCost kTiles16[3] = {{256, 256, 1, 1.9f, 0.f}, {128, 128, 2, 0.75f, 0.41f}, {64, 64, 5, 0.5f, 0.15f}};
+constexpr TileCost kTiles16[4] = {{256, 256, 1, 1.9f, 0.f}, {128, 128, 2, 0.8f, 0.38f}, {64, 64, 5, 0.5f, 0.15f}, {128, 128, 1, 0.66f, 0.f}};
 constexpr TileCost kTiles32[3] = {{256, 256, 1, 11.4f, 0.f}, {128, 64, 1, 2.1f, 0.f}, {64, 64, 1, 1.15f, 0.f}};
 template <typename U> Plan plan_product(int64_t I, int64_t cols, int64_t steps, int problems, bool sliceable) {
     const TileCost *kinds = sizeof(U) == 4 ? kTiles32 : kTiles16;
     Plan best = {0, 1};
     float least = 0.f;
-    for (int k = 0; k < 3; k++)
+    for (int k = 0; k < (sizeof(U) == 4 ? 3 : 4); k++)
         for (int slices = 1; slices <= (sliceable ? 64 : 1); slices *= 2) {
             if (slices > 1 && steps / slices < 4) break;
             const TileCost &t = kinds[k];
@@ -111,9 +112,12 @@ template <typename U> Plan plan_product(int64_t I, int64_t cols, int64_t steps, 
 
 template <typename T, typename U, bool AKS, bool BKS, int EPI> int launch_product(Args &p, int tile, int problems, hipStream_t s) {
     constexpr int P = planes<U>();
-    if (tile == 0) return launch_tile<T, U, 1, 256, 256, 2, 4, AKS, BKS, EPI>(p, problems, s);
-    if (tile == 1) return launch_tile<T, U, P, 128, P == 3 ? 64 : 128, 2, 2, AKS, BKS, EPI>(p, problems, s);
-    return launch_tile<T, U, P, 64, 64, 2, 2, AKS, BKS, EPI>(p, problems, s);
+    if (tile == 0) return launch_tile<T, U, 1, 2, 256, 256, 2, 4, AKS, BKS, EPI>(p, problems, s);
+    if (tile == 1) return launch_tile<T, U, P, 2, 128, P == 3 ? 64 : 128, 2, 2, AKS, BKS, EPI>(p, problems, s);
+    if constexpr (P == 1) {
+        if (tile == 3) return launch_tile<T, U, P, 4, 128, 128, 2, 4, AKS, BKS, EPI>(p, problems, s);
+    }
+    return launch_tile<T, U, P, 2, 64, 64, 2, 2, AKS, BKS, EPI>(p, problems, s);
 }
 
 // Up to this D the backward pass computes G and U again: 4 D operations an element against 16 bytes.  (At D = 256, 131 072 x 1 024: forward and this part of the

@@ -163,7 +163,8 @@ __device__ __forceinline__ i32x4 descriptor(const void *p) {
 __device__ __forceinline__ void dma16(const i32x4 &desc, uint32_t voff, uint32_t to_lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to_lds), "v"(voff), "s"(desc) : "memory");
 }
-__device__ __forceinline__ void wait_and_meet() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// everybody has this step's data (N of this wave's requests, for later steps, may still be under way) and is done with the previous step's
+template <int N> __device__ __forceinline__ void wait_and_meet() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
 
 __device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }       // LDS only: stores to global memory stay in flight
 
@@ -314,7 +315,7 @@ __device__ __forceinline__ void multiply_step(A a, B b, R request, f32x4 (&acc)[
 }
 
 // T: the matrix instruction's type; U: the user's type (float: T = bf16, planes); P: planes in LDS.
-template <typename T, typename U, int P, int BM, int BN, int WI, int WJ, bool AKS, bool BKS, int EPI>
+template <typename T, typename U, int P, int BUFS, int BM, int BN, int WI, int WJ, bool AKS, bool BKS, int EPI>
 __global__ __launch_bounds__(64 * WI * WJ) void k_rows_gemm(const Args p) {
     constexpr int WAVES = WI * WJ, MT = BM / WI / 16, NT = BN / WJ / 16;
     constexpr bool DUAL = EPI == EPI_GATE;
@@ -369,21 +370,25 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_rows_gemm(const Args p) {
     for (int m = 0; m < MT; m++)
 #pragma unroll
         for (int n = 0; n < NT; n++) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (s_begin < s_end) {
-        point();
-        request(0);
-    }
+    // BUFS buffers: a step's requests are made BUFS - 1 steps ahead, into the buffer that the step before the current one has just left
+    if (s_begin < s_end) point();
+#pragma unroll
+    for (int b = 0; b < BUFS - 1; b++)
+        if (s_begin + b < s_end) request(b);
+    constexpr int kAhead = (BUFS - 2) * P * (SA::kReq + SB::kReq);       // a wave's requests for the steps after this one
+    static_assert(kAhead < 64, "the wait counts to 63");
     int buf = 0;
     for (int s = s_begin; s < s_end; s++) {
-        wait_and_meet();            // step s has landed for every wave; every wave is done with the other buffer
+        if (s + BUFS - 2 < s_end) wait_and_meet<kAhead>();
+        else wait_and_meet<0>();
         const uint32_t at = lds0 + (uint32_t)buf * kBuf, at_b = at + P * SA::kBytes;
         multiply_step<T, MT, NT, P, AKS ? 2 : 1, BKS ? 2 : 1>(
             [&](int m, int ks, int q) { return sa.fragment(at + q * SA::kBytes, m, ks); },
             [&](int n, int ks, int q) {         // (EPI_GATE: the tile's upper half is the up projection's rows)
                 return DUAL && n >= NT / 2 ? sb.fragment(at_b + q * SB::kBytes, n - NT / 2, ks, BN / 2) : sb.fragment(at_b + q * SB::kBytes, n, ks);
             },
-            [&]() { if (s + 1 < s_end) request(buf ^ 1); }, acc);
-        buf ^= 1;
+            [&]() { if (s + BUFS - 1 < s_end) request(buf == 0 ? BUFS - 1 : buf - 1); }, acc);
+        buf = buf + 1 == BUFS ? 0 : buf + 1;
     }
 
     // ---- epilogue: acc[m][n][r] is row i0 + 16 (wi MT + m) + (lane & 15), column 16 unit + 4 (lane >> 4) + r
@@ -493,7 +498,7 @@ inline void as_segments(Args &p) {
     p.n_seg *= 6;
 }
 
-template <typename T, typename U, int P, int BM, int BN, int WI, int WJ, bool AKS, bool BKS, int EPI>
+template <typename T, typename U, int P, int BUFS, int BM, int BN, int WI, int WJ, bool AKS, bool BKS, int EPI>
 inline int launch_tile(Args p, int problems, hipStream_t s) {
     constexpr int TJ = EPI == EPI_GATE ? BN / 2 : BN;
     // the gate epilogues also write the padding columns up to ldh (< J + 8)
@@ -503,12 +508,12 @@ inline int launch_tile(Args p, int problems, hipStream_t s) {
     p.tiles_i = (int)ti;
     p.tiles_j = (int)tj;
     if constexpr (planes<U>() != P) as_segments(p);
-    constexpr int lds = 2 * P * (BM + BN) * BK * 2;
+    constexpr int lds = BUFS * P * (BM + BN) * BK * 2;
     static_assert(Staging<BN, BM / WI / 16, 2, WI, WI * WJ, TJ>::kBytes <= lds, "the epilogue's tile must fit");
     static hsLdsAttrOnce attr;
-    const void *fn = (const void *)k_rows_gemm<T, U, P, BM, BN, WI, WJ, AKS, BKS, EPI>;
+    const void *fn = (const void *)k_rows_gemm<T, U, P, BUFS, BM, BN, WI, WJ, AKS, BKS, EPI>;
     attr.set(fn, lds);
-    k_rows_gemm<T, U, P, BM, BN, WI, WJ, AKS, BKS, EPI><<<dim3((unsigned)(ti * tj), (unsigned)p.slices, (unsigned)problems), 64 * WI * WJ, lds, s>>>(p);
+    k_rows_gemm<T, U, P, BUFS, BM, BN, WI, WJ, AKS, BKS, EPI><<<dim3((unsigned)(ti * tj), (unsigned)p.slices, (unsigned)problems), 64 * WI * WJ, lds, s>>>(p);
     return hipGetLastError() == hipSuccess ? HS_OK : HS_ERR_LAUNCH;
 }
 
@@ -573,7 +578,7 @@ __global__ __launch_bounds__(256) void k_gate_bwd(const Args p) {
     request1(0);
     int buf = 0;
     for (int s = 0; s < steps; s++) {
-        wait_and_meet();
+        wait_and_meet<0>();
         const uint32_t at = lds0 + buf * kBuf;
         multiply_step<T, MT, N1, 1, 1, 1>([&](int m, int ks, int) { return sx.fragment(at, m, ks); },
                                        [&](int n, int ks, int) { return n < N2 ? s1.fragment(at + SA::kBytes, n, ks) : s1.fragment(at + SA::kBytes, n - N2, ks, TJ); },
@@ -588,7 +593,7 @@ __global__ __launch_bounds__(256) void k_gate_bwd(const Args p) {
         buf ^= 1;
     }
     for (int s = 0; s < steps; s++) {
-        wait_and_meet();
+        wait_and_meet<0>();
         const uint32_t at = lds0 + buf * kBuf;
         multiply_step<T, MT, N2, 1, 1, 2>([&](int m, int ks, int) { return sx.fragment(at, m, ks); }, [&](int n, int ks, int) { return s2.fragment(at + SA::kBytes, n, ks); },
                                        [&]() { if (s + 1 < steps) request2(buf ^ 1); }, acc2);
