@@ -29,18 +29,26 @@ struct Arena {
 
 inline int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
 
-// src [rows, cols] -> dst [planes][rows][ldp], ldp = up8(cols), zeros behind cols
+// Operands that are not in that form, copied into it: src [rows, cols] -> dst [planes][rows][8 chunks], zeros behind cols.  All of a pass in one launch (fp32
+// has every operand in it; a launch each cost more than the copies).
+constexpr int kMaxPack = 6;
+struct PackJob { const void *src; void *dst; int64_t ld, rows, cols, chunks, plane; unsigned first; };      // first: the job's first workgroup
+struct PackJobs { PackJob j[kMaxPack]; int n; unsigned blocks; };
+
 template <typename U>
-__global__ __launch_bounds__(256) void k_rows_pack(const U *__restrict__ src, int64_t ld, int64_t rows, int64_t cols, int64_t chunks, void *__restrict__ dst, int64_t plane) {
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (id >= rows * chunks) return;
-    const int64_t r = id / chunks, c = (id - r * chunks) * 8;
-    const U *s = src + r * ld + c;
+__global__ __launch_bounds__(256) void k_rows_pack(const PackJobs jobs) {
+    int k = 0;
+    while (k + 1 < jobs.n && blockIdx.x >= jobs.j[k + 1].first) k++;
+    const PackJob &job = jobs.j[k];
+    const int64_t id = (int64_t)(blockIdx.x - job.first) * 256 + threadIdx.x;
+    if (id >= job.rows * job.chunks) return;
+    const int64_t r = id / job.chunks, c = (id - r * job.chunks) * 8;
+    const U *s = (const U *)job.src + r * job.ld + c;
     Loose<U, 8> v;
-    if (c + 8 <= cols) v = *reinterpret_cast<const Loose<U, 8> *>(s);
+    if (c + 8 <= job.cols) v = *reinterpret_cast<const Loose<U, 8> *>(s);
     else
 #pragma unroll
-        for (int e = 0; e < 8; e++) v.v[e] = c + e < cols ? s[e] : (U)0.f;
+        for (int e = 0; e < 8; e++) v.v[e] = c + e < job.cols ? s[e] : (U)0.f;
     if constexpr (sizeof(U) == 4) {
         Pack<bf16_t, 8> o[3];
 #pragma unroll
@@ -50,12 +58,12 @@ __global__ __launch_bounds__(256) void k_rows_pack(const U *__restrict__ src, in
             o[0].v[e] = q[0]; o[1].v[e] = q[1]; o[2].v[e] = q[2];
         }
 #pragma unroll
-        for (int q = 0; q < 3; q++) *reinterpret_cast<Pack<bf16_t, 8> *>((bf16_t *)dst + q * plane + id * 8) = o[q];
+        for (int q = 0; q < 3; q++) *reinterpret_cast<Pack<bf16_t, 8> *>((bf16_t *)job.dst + q * job.plane + id * 8) = o[q];
     } else {
         Pack<U, 8> o;
 #pragma unroll
         for (int e = 0; e < 8; e++) o.v[e] = v.v[e];
-        *reinterpret_cast<Pack<U, 8> *>((U *)dst + id * 8) = o;
+        *reinterpret_cast<Pack<U, 8> *>((U *)job.dst + id * 8) = o;
     }
 }
 
@@ -141,17 +149,25 @@ template <typename T, typename U> struct Block {
 
     void check(int r) { if (rc == HS_OK) rc = r; }
 
+    // The operand itself, or the copy of it that the next pack() makes.
+    PackJobs jobs = {};
     Operand operand(const void *p, int64_t ld, int64_t rows, int64_t cols, bool force = false) {
         if (sizeof(U) == 2 && !force && (uintptr_t)p % 16 == 0 && ld % 8 == 0 && cols % 8 == 0) return Operand{p, ld, 0};
-        const int64_t ldp = up8(cols), n = rows * ldp;
+        const int64_t ldp = up8(cols), n = rows * ldp, blocks = (n / 8 + 255) / 256;
         void *dst = ws.take(n * 2 * planes<U>());
-        if (run && rc == HS_OK) {
-            const int64_t blocks = (n / 8 + 255) / 256;
-            if (blocks > 0x7fffffff) { check(HS_ERR_ARG); return Operand{}; }
-            k_rows_pack<U><<<(unsigned)blocks, 256, 0, s>>>((const U *)p, ld, rows, cols, ldp / 8, dst, n);
-            check(hipGetLastError() == hipSuccess ? HS_OK : HS_ERR_LAUNCH);
+        if (jobs.n == kMaxPack || jobs.blocks + blocks > 0x7fffffff) check(HS_ERR_ARG);
+        else {
+            jobs.j[jobs.n++] = PackJob{p, dst, ld, rows, cols, ldp / 8, n, jobs.blocks};
+            jobs.blocks += (unsigned)blocks;
         }
         return Operand{dst, ldp, n};
+    }
+    void pack() {
+        if (run && rc == HS_OK && jobs.n > 0) {
+            k_rows_pack<U><<<jobs.blocks, 256, 0, s>>>(jobs);
+            check(hipGetLastError() == hipSuccess ? HS_OK : HS_ERR_LAUNCH);
+        }
+        jobs = {};
     }
 
     // both projections' weights with one row distance
@@ -214,6 +230,7 @@ template <typename T, typename U> struct Block {
             sv.h = Operand{ws.take(M * ldh * 2 * planes<U>()), ldh, M * ldh};
         }
         if (!fits<false, false>(x, wg) || !fits<false, false>(wd, sv.h)) return;
+        pack();
         Args p = product(x, wg, M, F, D);
         p.seg[0][0].b1 = wu.p;
         p.g = sv.g; p.u = sv.u; p.h = (void *)sv.h.p; p.ldh = ldh; p.plane = sv.h.plane; p.act = a.activation;
@@ -265,15 +282,17 @@ template <typename T, typename U> struct Block {
     }
 
     void bwd() {
-        const Operand gy = operand(a.grad, a.ld_grad, M, D);
         const Saved sv = saved_in((char *)a.saved);
-        if (a.gx || a.gw_gate || a.gw_up) {
-            const Operand wd = operand(a.w_down, a.ld_down, D, F);
+        const bool inner = a.gx || a.gw_gate || a.gw_up, xw = a.gw_gate || a.gw_up;
+        const Operand gy = operand(a.grad, a.ld_grad, M, D);
+        Operand wd, wg, wu, x;
+        if (inner) wd = operand(a.w_down, a.ld_down, D, F);
+        if (inner && (again() || a.gx)) projections(wg, wu);
+        if (inner && (again() || xw)) x = operand(a.x, a.ldx, M, D);
+        pack();
+        if (inner) {
             const int64_t n = M * ldh;
             const Operand gg{ws.take(n * 2 * planes<U>()), ldh, n}, gu{ws.take(n * 2 * planes<U>()), ldh, n};
-            Operand wg, wu, x;
-            if (again() || a.gx) projections(wg, wu);
-            if (again() || a.gw_gate || a.gw_up) x = operand(a.x, a.ldx, M, D);
             if (fits<false, true>(gy, wd) && (!again() || fits<false, false>(x, wg)) && run) {
                 Args p = again() ? product(x, wg, M, F, D) : product(gy, wd, M, F, D);
                 p.g = sv.g; p.u = sv.u; p.gg = (void *)gg.p; p.gu = (void *)gu.p; p.ldh = ldh; p.plane = n; p.act = a.activation;
@@ -294,7 +313,7 @@ template <typename T, typename U> struct Block {
                     result<false, true>(p, &a.gx, 1);
                 }
             }
-            if (a.gw_gate || a.gw_up) {
+            if (xw) {
                 const Operand av[2] = {a.gw_gate ? gg : gu, gu};
                 void *const out[2] = {a.gw_gate ? a.gw_gate : a.gw_up, a.gw_up};
                 weight_gradient(av, x, out, a.gw_gate && a.gw_up ? 2 : 1, F, D);
