@@ -41,7 +41,7 @@ __global__ __launch_bounds__(256) void k_dropout(const T *__restrict__ x, const 
 }  // namespace
 
 extern "C" int hs_dropout_rows(const void *x, const void *residual, void *y, int64_t n, int32_t dtype, int32_t drop, const uint64_t *rng, void *stream) {
-    if (n < 0 || !hs_row::known_dtype(dtype) || drop < 0 || drop > 65536 || n / 2048 >= 0x7fffffff) return HS_ERR_ARG;
+    if (n < 0 || !hs_row::known_dtype(dtype) || drop < 0 || drop > 65536 || n / 2048 >= 0xffffff) return HS_ERR_ARG;
     if (n == 0) return HS_OK;
     if (!x || !y || !rng) return HS_ERR_NULL;
     const float scale = drop < 65536 ? (float)(65536.0 / (65536 - drop)) : 0.f;

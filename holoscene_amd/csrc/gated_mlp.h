@@ -10,7 +10,8 @@
 
 namespace hs_gemm {
 
-// An operand as the products read it: 16-byte aligned rows whose contiguous extent is a multiple of 8 (zeros behind the matrix's own).
+// An operand as the products read it: 16-byte aligned rows whose contiguous extent is a multiple of 8 (zeros behind the matrix's own), at most 2^21 elements
+// apart (offsets inside a tile have 32 bits).
 struct Operand {
     const void *p;
     int64_t ld, plane;
@@ -152,10 +153,10 @@ template <typename T, typename U> struct Block {
     // The operand itself, or the copy of it that the next pack() makes.
     PackJobs jobs = {};
     Operand operand(const void *p, int64_t ld, int64_t rows, int64_t cols, bool force = false) {
-        if (sizeof(U) == 2 && !force && (uintptr_t)p % 16 == 0 && ld % 8 == 0 && cols % 8 == 0) return Operand{p, ld, 0};
+        if (sizeof(U) == 2 && !force && (uintptr_t)p % 16 == 0 && ld % 8 == 0 && cols % 8 == 0 && ld <= (1 << 21)) return Operand{p, ld, 0};
         const int64_t ldp = up8(cols), n = rows * ldp, blocks = (n / 8 + 255) / 256;
         void *dst = ws.take(n * 2 * planes<U>());
-        if (jobs.n == kMaxPack || jobs.blocks + blocks > 0x7fffffff) check(HS_ERR_ARG);
+        if (jobs.n == kMaxPack || jobs.blocks + blocks > kMaxGrid / 256) check(HS_ERR_ARG);
         else {
             jobs.j[jobs.n++] = PackJob{p, dst, ld, rows, cols, ldp / 8, n, jobs.blocks};
             jobs.blocks += (unsigned)blocks;
@@ -195,12 +196,6 @@ template <typename T, typename U> struct Block {
         return v;
     }
 
-    template <bool AKS, bool BKS> bool fits(const Operand &x, const Operand &y) {       // 32-bit offsets inside a tile's step
-        const int64_t most = 0x7fffffffll - 4096;
-        if (256 * x.ld * 2 > most || 256 * y.ld * 2 > most) { check(HS_ERR_ARG); return false; }
-        return rc == HS_OK;
-    }
-
     void fwd_small() {
         Saved sv = saved_in((char *)a.saved);
         if (!a.saved) {
@@ -229,7 +224,6 @@ template <typename T, typename U> struct Block {
             sv.g = sv.u = nullptr;
             sv.h = Operand{ws.take(M * ldh * 2 * planes<U>()), ldh, M * ldh};
         }
-        if (!fits<false, false>(x, wg) || !fits<false, false>(wd, sv.h)) return;
         pack();
         Args p = product(x, wg, M, F, D);
         p.seg[0][0].b1 = wu.p;
@@ -267,7 +261,7 @@ template <typename T, typename U> struct Block {
         }
         check(launch_product<T, U, AKS, BKS, EPI_PARTIAL>(p, plan.tile, problems, s));
         const int64_t blocks = (n + 1023) / 1024;
-        if (rc != HS_OK || blocks > 0x7fffffff) { check(HS_ERR_ARG); return; }
+        if (rc != HS_OK || blocks > kMaxGrid / 256) { check(HS_ERR_ARG); return; }
         k_rows_reduce<U><<<dim3((unsigned)blocks, problems), 256, 0, s>>>(parts, parts + (problems - 1) * plan.slices * stride, n, plan.slices, (U *)out[0],
                                                                           (U *)out[problems - 1]);
         check(hipGetLastError() == hipSuccess ? HS_OK : HS_ERR_LAUNCH);
@@ -275,7 +269,6 @@ template <typename T, typename U> struct Block {
 
     // C_z [I, J] = A_z^T B over the rows
     void weight_gradient(const Operand *av, const Operand &b, void *const *out, int problems, int64_t I, int64_t J) {
-        if (!fits<true, true>(av[0], b)) return;
         Args p = product(av[0], b, I, J, M);
         if (problems == 2) p.seg[1][0] = Seg{av[1].p, b.p, nullptr};
         result<true, true>(p, out, problems);
@@ -293,7 +286,7 @@ template <typename T, typename U> struct Block {
         if (inner) {
             const int64_t n = M * ldh;
             const Operand gg{ws.take(n * 2 * planes<U>()), ldh, n}, gu{ws.take(n * 2 * planes<U>()), ldh, n};
-            if (fits<false, true>(gy, wd) && (!again() || fits<false, false>(x, wg)) && run) {
+            if (run && rc == HS_OK) {
                 Args p = again() ? product(x, wg, M, F, D) : product(gy, wd, M, F, D);
                 p.g = sv.g; p.u = sv.u; p.gg = (void *)gg.p; p.gu = (void *)gu.p; p.ldh = ldh; p.plane = n; p.act = a.activation;
                 if (again()) {
@@ -306,12 +299,10 @@ template <typename T, typename U> struct Block {
                 }
             }
             if (a.gx) {
-                if (fits<false, true>(gg, wg)) {
-                    Args p = product(gg, wg, M, D, F);
-                    p.seg[0][1] = Seg{gu.p, wu.p, nullptr};
-                    p.n_seg = 2;
-                    result<false, true>(p, &a.gx, 1);
-                }
+                Args p = product(gg, wg, M, D, F);
+                p.seg[0][1] = Seg{gu.p, wu.p, nullptr};
+                p.n_seg = 2;
+                result<false, true>(p, &a.gx, 1);
             }
             if (xw) {
                 const Operand av[2] = {a.gw_gate ? gg : gu, gu};

@@ -39,6 +39,7 @@ typedef short i16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int BK = 64;
 constexpr int kMaxSeg = 12;
+constexpr int64_t kMaxGrid = 0xffffffffll;        // threads along x in a launch
 
 template <typename U> constexpr int planes() { return sizeof(U) == 4 ? 3 : 1; }
 
@@ -504,7 +505,7 @@ inline int launch_tile(Args p, int problems, hipStream_t s) {
     // the gate epilogues also write the padding columns up to ldh (< J + 8)
     const int64_t cols = EPI == EPI_GATE || EPI == EPI_GATE_BWD ? p.ldh : p.J;
     const int64_t ti = (p.I + BM - 1) / BM, tj = (cols + TJ - 1) / TJ;
-    if (ti * tj > 0x7fffffff / 8 || p.slices > 65535) return HS_ERR_ARG;
+    if (ti * tj > kMaxGrid / (64 * WI * WJ) || p.slices > 65535) return HS_ERR_ARG;
     p.tiles_i = (int)ti;
     p.tiles_j = (int)tj;
     if constexpr (planes<U>() != P) as_segments(p);
@@ -643,7 +644,7 @@ __global__ __launch_bounds__(256) void k_gate_bwd(const Args p) {
 template <typename T, typename U> inline int launch_gate_bwd(Args p, hipStream_t s) {
     if constexpr (planes<U>() == 3) as_segments(p);
     const int64_t ti = (p.I + kAgainM - 1) / kAgainM, tj = (p.ldh + kAgainJ - 1) / kAgainJ;
-    if (ti * tj > 0x7fffffff / 8) return HS_ERR_ARG;
+    if (ti * tj > kMaxGrid / 256) return HS_ERR_ARG;
     p.tiles_i = (int)ti;
     p.tiles_j = (int)tj;
     constexpr int lds = 2 * (kAgainM + 2 * kAgainJ) * BK * 2;

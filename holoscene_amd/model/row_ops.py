@@ -7,7 +7,8 @@ dropout, each with its backward pass, on the kernels of csrc/embed_rows.hip, csr
 
 float32, bfloat16 and float16 storage, fp32 arithmetic, one rounding per result.  As everywhere in this package there is no CPU path: a tensor
 that is not on the GPU, or a type or shape the kernels do not take, raises RuntimeError.  The work runs on the current stream of the tensors' device
-and can be captured into a HIP graph; results do not depend on the launch (no floating-point atomics).  Gradients of gradients are not provided.
+and can be captured into a HIP graph (with a backward pass: capture before an eager graph of the same leaves is built, or drop it first -- its
+gradient accumulators belong to the eager stream); results do not depend on the launch (no floating-point atomics).  Gradients of gradients are not provided.
 """
 import contextlib
 import math
@@ -142,9 +143,9 @@ class _gated_mlp_rows(torch.autograd.Function):
 def gated_mlp_rows(x, w_gate, w_up, w_down, activation="silu"):
     """(act(x Wg^T) * (x Wu^T)) Wd^T for x [..., dim], w_gate and w_up [hidden, dim], w_down [dim, hidden], all of one type.
 
-    activation: "silu", "gelu" (g Phi(g)), "gelu_tanh" (its tanh form), "sigmoid", "relu".  float32 operands are multiplied as three bf16 planes each
-    (24 bits, as linear_rows under HOLOSCENE_FP32_GEMM=split3).  Rows may be strided; 16-bit operands whose rows are not 16-byte aligned are copied
-    once per call.  The forward keeps both projections and the gated product for the backward pass (3 * hidden elements a row)."""
+    dim and hidden are at most 2^21.  activation: "silu", "gelu" (g Phi(g)), "gelu_tanh" (its tanh form), "sigmoid", "relu".  float32 operands are multiplied as three bf16 planes each
+    (24 bits, as linear_rows under HOLOSCENE_FP32_GEMM=split3; an infinity among them gives NaN).  Rows may be strided; 16-bit operands whose
+    rows are not 16-byte aligned are copied once per call.  The forward keeps the gated product for the backward pass, with dim > 768 both projections in fp32 as well."""
     _check_tensor(x, "x")
     if x.dim() < 1:
         raise RuntimeError("x must be [..., dim]")
@@ -156,6 +157,8 @@ def gated_mlp_rows(x, w_gate, w_up, w_down, activation="silu"):
     if x.shape[-1] != dim or w_up.shape != (hidden, dim) or w_down.shape != (dim, hidden):
         raise RuntimeError(f"x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, w_up {tuple(w_up.shape)}, w_down {tuple(w_down.shape)}: expected [..., dim], "
                            "[hidden, dim], [hidden, dim], [dim, hidden]")
+    if max(hidden, dim) > 1 << 21:
+        raise RuntimeError(f"dim {dim} and hidden {hidden} must be at most {1 << 21}")
     if activation not in _be.ROW_ACTIVATIONS:
         raise RuntimeError(f"activation must be one of {', '.join(ACTIVATIONS)}, got {activation!r}")
     if _recorded(x, w_gate, w_up, w_down):
@@ -242,7 +245,9 @@ class GatedMLP(nn.Module):
 
 class RowDropout(nn.Module):
     """Dropout (dropout_rows) with a generator state of its own: a buffer (seed, number of the next call), advanced on the device by every
-    call in training mode, so that eager calls and replays of a captured graph alike draw a new mask each time."""
+    call in training mode, so that eager calls and replays of a captured graph alike draw a new mask each time.  A pass that is run twice
+    (activation checkpointing) draws twice: call dropout_rows with a state of your own there.  Give every rank its own seed, and keep
+    DistributedDataParallel from copying rank 0's buffer (broadcast_buffers=False)."""
 
     def __init__(self, p, seed=0):
         super().__init__()

@@ -906,11 +906,12 @@ int hs_embed_bwd(const void *indices, int32_t index_bytes, const void *grad, int
                  int32_t grad_dtype, int32_t table_dtype, void *ws, int64_t ws_bytes, void *stream);
 
 /* y_i = (u_i >= drop ? x_i * 65536 / (65536 - drop) : 0) + residual_i, u_i = 16 bits of Philox-4x32-10 with key rng[0] and counter (i / 8, rng[1]): word (i % 8) / 2, low half
- * first.  rng: DEVICE uint64[2] (seed, number of the call), read only.  drop in [0, 65536] (65536: everything).  residual may be NULL; y may be x or residual. */
+ * first.  rng: DEVICE uint64[2] (seed, number of the call), read only.  drop in [0, 65536] (65536: everything).  residual may be NULL.
+ * n < 2^35 - 2048 (one launch). */
 int hs_dropout_rows(const void *x, const void *residual, void *y, int64_t n, int32_t dtype, int32_t drop, const uint64_t *rng, void *stream);
 
 /* y = (act(x Wg^T) * (x Wu^T)) Wd^T and its gradient; x [rows, dim], Wg, Wu [hidden, dim], Wd [dim, hidden], every one with a row distance of its own; y and the
- * gradients contiguous.  All three sizes > 0. */
+ * gradients contiguous.  All three sizes > 0, dim and hidden <= 2^21.  fp32: an infinite operand gives NaN (infinity times a plane that is zero). */
 #define HS_ACT_SILU 0
 #define HS_ACT_GELU 1           /* g Phi(g) */
 #define HS_ACT_GELU_TANH 2

@@ -67,7 +67,7 @@ def test_gated_mlp_refusals():
     for fn in (fwd, bwd):
         assert fn(None, None) == -3
         for bad in (dict(rows=0), dict(dim=0), dict(hidden=0), dict(rows=-1), dict(ldx=15), dict(ld_gate=1), dict(ld_up=1), dict(ld_down=31), dict(activation=5),
-                    dict(activation=-1), dict(dtype=3), dict(hidden=1 << 23, ld_down=1 << 23)):
+                    dict(activation=-1), dict(dtype=3), dict(hidden=(1 << 21) + 1, ld_down=1 << 23)):
             assert fn(gated(**bad), None) == -1, bad
         for name in ("x", "w_gate", "w_up", "w_down"):
             assert fn(gated(**{name: None}), None) == -3

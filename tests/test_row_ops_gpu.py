@@ -120,6 +120,29 @@ def test_embedding_gradient_of_broadcast_and_strided_results():
     assert torch.equal(a, b)
 
 
+def test_embedding_beyond_32_bits():
+    """More result elements than a grid has threads, gradients behind 4 GiB."""
+    n, V, D = 65600, 5, 65537
+    gen = torch.Generator().manual_seed(8)
+    idx = torch.randint(-1, V, (n,), generator=gen).to(DEV)
+    table = torch.randn(V, D, generator=gen).to(torch.bfloat16).to(DEV).requires_grad_()
+    out = ops().embedding_rows(idx, table)
+    assert out.numel() > 1 << 32
+    for v in range(V):
+        at = (idx == v).nonzero()[:, 0]
+        assert all(torch.equal(out[i], table[v]) for i in (int(at[0]), int(at[len(at) // 2]), int(at[-1])))
+    for i in range(0, n, 4100):
+        part = idx[i:i + 4100, None]
+        assert torch.equal(out[i:i + 4100], torch.where(part >= 0, table.detach()[part[:, 0].clamp(min=0)], torch.zeros((), dtype=table.dtype, device=DEV)))
+    # whole numbers below 2^24: the sums are exact; every row ends in a value of its own
+    g = torch.ones_like(out)
+    g[:, -1] = (torch.arange(n, device=DEV) % 3).to(g.dtype)
+    gt, = torch.autograd.grad(out, table, g)
+    want = torch.stack([(idx == v).sum() for v in range(V)]).float().to(gt.dtype)[:, None].expand(V, D).clone()
+    want[:, -1] = torch.stack([(torch.arange(n, device=DEV) % 3)[idx == v].sum() for v in range(V)]).float().to(gt.dtype)
+    assert torch.equal(gt, want)
+
+
 def test_embedding_refusals():
     f, table, idx = ops().embedding_rows, torch.zeros(4, 8, device=DEV), torch.zeros(3, dtype=torch.long, device=DEV)
     for bad in (dict(indices=idx.float()), dict(indices=idx.short()), dict(table=table[0]), dict(table=table.double()), dict(padding_idx=4), dict(padding_idx=-1),
@@ -129,10 +152,10 @@ def test_embedding_refusals():
 
 
 # ------------------------------------------------------------------------------------------------ dropout
-def keep_reference(n, drop, seed, call):
-    """Philox-4x32-10 in Python integers."""
+def keep_reference(n, drop, seed, call, first=0):
+    """Philox-4x32-10 in Python integers: elements 8 first, 8 first + 1, .. n of them."""
     out = []
-    for grp in range((n + 7) // 8):
+    for grp in range(first, first + (n + 7) // 8):
         c, k = [grp & 0xffffffff, grp >> 32, call & 0xffffffff, call >> 32], [seed & 0xffffffff, seed >> 32]
         for _ in range(10):
             a, b = 0xD2511F53 * c[0], 0xCD9E8D57 * c[2]
@@ -197,6 +220,15 @@ def test_dropout_dropped_infinities_strides_and_shares():
     other = ops().dropout_rows(base, 0.5, torch.tensor([11, 3], device=DEV))
     assert not torch.equal(other == 0, ops().dropout_rows(base, 0.5, rng) == 0), "another call, another mask"
     assert ops().dropout_rows(base[:0], 0.5, rng).shape == (0, 70)
+
+
+def test_dropout_beyond_32_bits():
+    n = (1 << 33) + 2051                   # the last groups' counters have more than 30 bits, their elements more than 33
+    x = torch.ones(n, dtype=torch.bfloat16, device=DEV)
+    y = ops().dropout_rows(x, 0.5, torch.tensor([9, 4], device=DEV))
+    for first, count in ((0, 64), ((1 << 29) - 4, 64), (1 << 29, 2051)):
+        want = keep_reference(count, 32768, 9, 4, first)
+        assert torch.equal(y[8 * first:8 * first + count].cpu(), want.to(torch.bfloat16) * 2)
 
 
 def test_dropout_refusals():
@@ -340,6 +372,26 @@ def test_gated_partial_gradients():
         some = [t.detach().requires_grad_(i in pick) for i, t in enumerate((x, wg, wu, wd))]
         got = torch.autograd.grad(ops().gated_mlp_rows(*some), [some[i] for i in pick], gy)
         assert all(torch.equal(a, want[i]) for a, i in zip(got, pick))
+
+
+def test_gated_beyond_32_bits():
+    """A hidden layer of more than 2^32 elements: rows at its start, behind 2^31 and at its end."""
+    M, D, F = (1 << 20) + 77, 64, 4104
+    x, wg, wu, wd, _ = gated_inputs(200, D, F, torch.bfloat16)
+    at = torch.cat([torch.arange(64), torch.arange(64) + M // 2 + 100, torch.arange(72) + M - 72]).to(DEV)
+    rows, gy = torch.zeros(M, D, dtype=x.dtype, device=DEV), torch.zeros(M, D, dtype=x.dtype, device=DEV)
+    rows[at] = x
+    gy[at] = torch.randn(200, D, generator=torch.Generator().manual_seed(9)).to(x.dtype).to(DEV)
+    leaves = [t.requires_grad_() for t in (rows, wg, wu, wd)]
+    y = ops().gated_mlp_rows(*leaves)
+    grads = torch.autograd.grad(y, leaves, gy)
+    # rows of zeros give zeros everywhere: the sums over the rows have 200 terms
+    ref = gated_reference(x, wg, wu, wd, "silu", gy[at])
+    for got, (want, bound), what in zip((y[at], grads[0][at], *grads[1:]), ref, ("y", "gx", "gw_gate", "gw_up", "gw_down")):
+        within(got, want, bound, what)
+    rest = torch.ones(M, dtype=torch.bool, device=DEV)
+    rest[at] = False
+    assert not bool(y[rest].any()) and not bool(grads[0][rest].any())
 
 
 @pytest.mark.parametrize("M,D,F", [(0, 8, 16), (4, 8, 0), (0, 0, 0), (3, 0, 5)])
