@@ -51,6 +51,12 @@ def _recorded(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def _once(backward):
+    """once_differentiable, without its guard where gradients are off anyway (every backward pass but create_graph=True; the guard is 5 us of the host)."""
+    guarded = once_differentiable(backward)
+    return lambda ctx, g: guarded(ctx, g) if torch.is_grad_enabled() else backward(ctx, g)
+
+
 def _as_rows(t):
     """[..., n] -> 2-D with consecutive elements in a row: the tensor itself (any row distance >= n), else a copy."""
     if t.dim() != 2:
@@ -76,7 +82,7 @@ class _embedding_rows(torch.autograd.Function):
         return _embed(indices, table, scale, out_dtype)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g):
         indices, = ctx.saved_tensors
         shape, dtype, scale, padding = ctx.args
@@ -128,7 +134,7 @@ class _gated_mlp_rows(torch.autograd.Function):
         return y.view(x.shape)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g):
         if ctx.empty:
             return tuple(torch.zeros_like(t) if need else None for t, need in zip(ctx.saved_tensors, ctx.needs_input_grad)) + (None,)
@@ -185,7 +191,7 @@ class _dropout_rows(torch.autograd.Function):
         return _dropout(x, residual, drop, rng)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g):
         rng, = ctx.saved_tensors
         return _dropout(g, None, ctx.drop, rng) if ctx.needs_input_grad[0] else None, g if ctx.needs_input_grad[1] else None, None, None
