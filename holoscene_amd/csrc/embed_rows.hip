@@ -58,7 +58,7 @@ template <typename I> __device__ __forceinline__ uint32_t sort_key(const I *__re
 
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
 constexpr int kOneMax = 4096, kOneDigit = 8;        // the one-workgroup sort (16 384 pairs in it: 37 us, bound by one CU's vector instructions; over 16 CUs 24)
-constexpr int kMultiDigit = 9;                     // the multi-block sort: tiles of 1, 2 or 4 pairs per thread
+constexpr int kMultiDigit = 9, kOnlyDigit = 11;    // the multi-block sort: tiles of 1, 2 or 4 pairs per thread; up to 11 bits in a single pass
 constexpr int kMaxBlocks = 64;                      // workgroups of the multi-block sort (each adds up all their histograms)
 
 // Lanes of this wave whose digit equals mine, among those with `on`.  (Per bit: a mask of the bit, a ballot, and the lanes that agree with it.)
@@ -66,7 +66,7 @@ __device__ __forceinline__ uint64_t same_digit(uint32_t digit, int bits, bool on
     const uint64_t all = __ballot(on);
     uint32_t lo = (uint32_t)all, hi = (uint32_t)(all >> 32);
 #pragma unroll
-    for (int b = 0; b < kMultiDigit; b++) {
+    for (int b = 0; b < kOnlyDigit; b++) {
         if (b < bits) {         // (uniform)
             const uint32_t mine = (uint32_t)((int32_t)(digit << (31 - b)) >> 31);
             const uint64_t set = __ballot(mine != 0u);
@@ -191,7 +191,7 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_one(const I *__restrict__
 template <typename I>
 __global__ __launch_bounds__(kSortThreads) void k_sort_hist(const I *__restrict__ idx, const uint32_t *__restrict__ keys_in, int64_t n, int64_t per, int64_t V, int64_t padding,
                                                             int shift, int nb, uint32_t *__restrict__ hist, uint32_t *__restrict__ long_rows) {
-    __shared__ uint32_t h[1 << kMultiDigit];
+    __shared__ uint32_t h[1 << kOnlyDigit];
     const int tid = threadIdx.x, bins = 1 << nb;
     if (tid == 0 && blockIdx.x == 0) long_rows[0] = 0;
     for (int d = tid; d < bins; d += kSortThreads) h[d] = 0;
@@ -221,15 +221,21 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(const I *__restri
     __syncthreads();
     {
         const int half = bins / 2, d = tid % half, share = kSortThreads / half;
-#pragma unroll 4
+        uint2 all = make_uint2(0, 0), mine = all;
+#pragma unroll 8
         for (int b = tid / half; b < (int)gridDim.x; b += share) {
             const uint2 c = reinterpret_cast<const uint2 *>(hist + (size_t)b * bins)[d];
-            atomicAdd(&place[2 * d], c.x);              // (counts in LDS: their order does not matter)
-            atomicAdd(&place[2 * d + 1], c.y);
-            if (b < (int)blockIdx.x) {
-                atomicAdd(&before[2 * d], c.x);
-                atomicAdd(&before[2 * d + 1], c.y);
-            }
+            const bool earlier = b < (int)blockIdx.x;
+            all.x += c.x;
+            all.y += c.y;
+            mine.x += earlier ? c.x : 0u;
+            mine.y += earlier ? c.y : 0u;
+        }
+        if (tid / half < (int)gridDim.x) {
+            atomicAdd(&place[2 * d], all.x);            // (counts in LDS: their order does not matter)
+            atomicAdd(&place[2 * d + 1], all.y);
+            atomicAdd(&before[2 * d], mine.x);
+            atomicAdd(&before[2 * d + 1], mine.y);
         }
     }
     __syncthreads();
@@ -238,7 +244,7 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(const I *__restri
     __syncthreads();
     const int64_t begin = blockIdx.x * per, end = begin + per < n ? begin + per : n;
     for (int64_t t0 = begin; t0 < end; t0 += kTile) {
-        for (int i = tid; i < kSortWaves * bins; i += kSortThreads) cnt[i] = 0;
+        for (int i = tid; i < kSortWaves * bins / 2; i += kSortThreads) reinterpret_cast<uint32_t *>(cnt)[i] = 0;
         uint32_t key[R], at[R], digit[R], rank[R];
         bool on[R];
 #pragma unroll
@@ -448,7 +454,7 @@ BwdPlan plan_bwd(int64_t n, int64_t V, int64_t D) {
     BwdPlan p = {};
     while (p.bits < 32 && ((uint64_t)V >> p.bits) != 0) p.bits++;        // keys 0 .. V
     const bool one = n <= kOneMax;
-    const int digit = one ? kOneDigit : kMultiDigit;
+    const int digit = one ? kOneDigit : p.bits <= kOnlyDigit ? kOnlyDigit : kMultiDigit;
     p.passes = (p.bits + digit - 1) / digit;
     p.nb_max = (p.bits + p.passes - 1) / p.passes;
     p.tile = kSortThreads * (n <= kMaxBlocks * 1024 ? 1 : n <= kMaxBlocks * 2048 ? 2 : 4);
@@ -483,7 +489,7 @@ void launch_scatter(const I *idx, const uint32_t *k_in, const uint32_t *p_in, in
                     uint32_t *keys, uint32_t *pos, hipStream_t s) {
     auto lds = [](int bins) { return 4 * (3 * bins + kSortWaves + 2 * R * kSortThreads) + 2 * kSortWaves * bins; };
     static hsLdsAttrOnce attr;
-    attr.set((const void *)k_sort_scatter<I, R>, lds(1 << kMultiDigit));
+    attr.set((const void *)k_sort_scatter<I, R>, lds(1 << kOnlyDigit));
     k_sort_scatter<I, R><<<(unsigned)p.blocks, kSortThreads, lds(1 << nb), s>>>(idx, k_in, p_in, n, p.per, V, padding, shift, nb, hist, keys, pos);
 }
 
