@@ -8,9 +8,10 @@
 //   sort    N <= 4 096: one workgroup, the pairs in registers, one pass per <= 8 bits of the index through LDS (one launch);
 //           longer: passes of <= 9 bits, two launches each (block histograms; ranks, every workgroup adding up the histograms itself).
 //   chunks  sorted positions in chunks of 32: a chunk that lies inside one run is summed to fp32 partials (a run of one index may be the whole batch).
-//   bounds  of every row's run, by bisection in the sorted indices, and a list of the long runs, in the same launch.
-//   rows    a wave per row of the table for the short runs (<= 8, most of them empty); a workgroup per long run and block of columns, its head and tail from g and its
-//           whole chunks from the partials, joined through LDS in a fixed order.
+//   runs    the run of every row, by bisection in the sorted indices, in the same launch: lists of the long and of the short ones, a flag for the others.
+//   rows    first the long runs (> 8 entries; a workgroup per run and block of columns: its head and tail from g and its whole chunks from the partials, joined
+//           through LDS in a fixed order), then the short ones (a wave each), then the zeros of the rows without one: the reads are over before the stores
+//           of the zeros, most of the bytes, fill the memory's queues.
 // fp32 sums: 32 terms per chunk, then the partials; the last operation rounds to the table's type.
 #include "holoscene_hip.h"
 #include "launch_util.h"
@@ -137,13 +138,13 @@ __device__ __forceinline__ void scan_exclusive(uint32_t *v, int n, uint32_t *wav
 // All of it in one workgroup: R = pairs per thread (N <= 1024 R), `passes` passes of <= 8 bits, the pairs through LDS between passes.
 template <typename I, int R>
 __global__ __launch_bounds__(kSortThreads) void k_sort_one(const I *__restrict__ idx, int n, int64_t V, int64_t padding, int bits, int passes, uint32_t *__restrict__ keys,
-                                                           uint32_t *__restrict__ pos, uint32_t *__restrict__ long_rows) {
+                                                           uint32_t *__restrict__ pos, uint32_t *__restrict__ list_n) {
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
     uint32_t *total = lds, *wave_sums = lds + 256;
     uint16_t *cnt = reinterpret_cast<uint16_t *>(lds + 256 + kSortWaves);
     uint32_t *lk = lds + 256 + kSortWaves + kSortWaves * 256 / 2, *lp = lk + 1024 * R;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    if (tid == 0) long_rows[0] = 0;            // (the next launch appends)
+    if (tid < 2) list_n[tid] = 0;              // (the next launch appends)
     uint32_t key[R], at[R], digit[R], rank[R];
     bool on[R];
 #pragma unroll
@@ -190,10 +191,10 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_one(const I *__restrict__
 // Multi-block, first launch of a pass: hist[block][digit] over the block's `per` pairs.  keys_in == NULL: the first pass, from the indices.
 template <typename I>
 __global__ __launch_bounds__(kSortThreads) void k_sort_hist(const I *__restrict__ idx, const uint32_t *__restrict__ keys_in, int64_t n, int64_t per, int64_t V, int64_t padding,
-                                                            int shift, int nb, uint32_t *__restrict__ hist, uint32_t *__restrict__ long_rows) {
+                                                            int shift, int nb, uint32_t *__restrict__ hist, uint32_t *__restrict__ list_n) {
     __shared__ uint32_t h[1 << kOnlyDigit];
     const int tid = threadIdx.x, bins = 1 << nb;
-    if (tid == 0 && blockIdx.x == 0) long_rows[0] = 0;
+    if (tid < 2 && blockIdx.x == 0) list_n[tid] = 0;
     for (int d = tid; d < bins; d += kSortThreads) h[d] = 0;
     __syncthreads();
     const int64_t begin = blockIdx.x * per, end = begin + per < n ? begin + per : n;
@@ -285,7 +286,10 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(const I *__restri
 constexpr int kChunk = 32;
 constexpr int kShort = 8, kWide = 4;        // runs up to kShort entries are summed by one group of lanes, kWide * VEC columns a lane at a time
 constexpr int64_t kMaxGrid = 0xffffff;     // workgroups of 256 a launch takes: a grid has less than 2^32 threads
-constexpr int kLongGroups = 256;            // workgroups (per block of columns) that share the long runs
+constexpr int kLongGroups = 256, kShortGroups = 8192;            // workgroups (per block of columns; in all) that share the long and the short runs
+
+struct Run { uint32_t row, first, end, pos; };              // pos: of its first entry, a load less in front of the gradient
+struct RunLists { Run *of_long, *of_short; uint32_t *n; uint8_t *used; };        // n: their lengths; used [V]: whether the row has a run
 
 // acc += the entries first, first + step, .. < end, in that order.  row(j): where entry j's element `col` lies.  BATCH entries are requested together, the missing
 // ones of the last batch at the first entry's address and not added (a branch between the requests would wait for each of them).
@@ -326,18 +330,32 @@ __device__ __forceinline__ int64_t lower_bound(const uint32_t *__restrict__ keys
 // chain of ~log2 n dependent loads: as part of the rows' kernel it was most of its time), the others sum the chunks that lie inside one run.
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void k_embed_chunks(const uint32_t *__restrict__ keys, const uint32_t *__restrict__ pos, const T *__restrict__ grad, int64_t ldg,
-                                                      int64_t n, uint32_t V, int D, int lanes, float *__restrict__ partial, uint2 *__restrict__ bounds, uint32_t *__restrict__ long_rows, unsigned bound_blocks) {
+                                                      int64_t n, uint32_t V, int D, int lanes, float *__restrict__ partial, RunLists lists, unsigned bound_blocks) {
     __shared__ float join[256 * VEC];
     const int tid = threadIdx.x;
     if (blockIdx.x < bound_blocks) {
         if (blockIdx.y != 0) return;
-        // one bound more than rows per workgroup: the end of its last row's run
-        __shared__ uint32_t first_of[257];
-        const int64_t v0 = (int64_t)blockIdx.x * 256;
+        __shared__ uint32_t first_of[257], part[2][4], base[2];        // one bound more than rows: the end of the last row's run
+        const int lane = tid & 63, wave = tid >> 6;
+        const int64_t v0 = (int64_t)blockIdx.x * 256, v = v0 + tid;
         for (int i = tid; i < 257; i += 256) first_of[i] = v0 + i <= V ? (uint32_t)lower_bound(keys, n, (uint32_t)(v0 + i)) : 0;
         __syncthreads();
-        if (v0 + tid <= V) bounds[v0 + tid] = make_uint2(first_of[tid], first_of[tid] < n ? pos[first_of[tid]] : 0u);        // .y: the first entry's position, a load less in the rows' chain
-        if (v0 + tid < V && first_of[tid + 1] - first_of[tid] > (uint32_t)kShort) long_rows[1 + atomicAdd(&long_rows[0], 1u)] = (uint32_t)(v0 + tid);      // (any order: each is a sum of its own)
+        const uint32_t first = first_of[tid], end = v < V ? first_of[tid + 1] : first, len = end - first;
+        const bool is_long = len > (uint32_t)kShort, is_short = len > 0 && !is_long;
+        const uint64_t longs = __ballot(is_long), shorts = __ballot(is_short), below = (1ull << lane) - 1;
+        if (lane == 0) {
+            part[0][wave] = __popcll(longs);
+            part[1][wave] = __popcll(shorts);
+        }
+        __syncthreads();
+        if (tid < 2) base[tid] = atomicAdd(&lists.n[tid], part[tid][0] + part[tid][1] + part[tid][2] + part[tid][3]);        // (any order: each run is a sum of its own)
+        __syncthreads();
+        if (v < V) lists.used[v] = len > 0;
+        if (len > 0) {
+            uint32_t at = base[is_short] + __popcll((is_short ? shorts : longs) & below);
+            for (int w = 0; w < wave; w++) at += part[is_short][w];
+            (is_short ? lists.of_short : lists.of_long)[at] = Run{(uint32_t)v, first, end, pos[first]};
+        }
         return;
     }
     const int64_t c = blockIdx.x - bound_blocks, c0 = c * kChunk;
@@ -361,12 +379,12 @@ __global__ __launch_bounds__(256) void k_embed_chunks(const uint32_t *__restrict
         if (col + e < D) out[e] = acc[e];
 }
 
-// The first long_groups * col_blocks workgroups: long runs, the others: a slot per row of the table -- the chain bounds -> position -> gradient is paid once per
-// row, not once per row and 1 KB of it, and with short runs there are few bytes to wait for otherwise.
+// The first long_groups * col_blocks workgroups: long runs; the next short_groups: short ones, a slot each; the others: a slot per row of the table, zeros where
+// it has no run.
 template <typename T, typename O, int VEC>
-__global__ __launch_bounds__(256) void k_embed_rows(const uint2 *__restrict__ bounds, const uint32_t *__restrict__ long_rows, const uint32_t *__restrict__ pos, const T *__restrict__ grad,
-                                                    int64_t ldg, int64_t V, int D, int lanes, const float *__restrict__ partial, float scale, O *__restrict__ gtable,
-                                                    unsigned long_groups, unsigned col_blocks) {
+__global__ __launch_bounds__(256) void k_embed_rows(const RunLists lists, const uint32_t *__restrict__ pos, const T *__restrict__ grad, int64_t ldg, int64_t V, int D, int lanes,
+                                                    const float *__restrict__ partial, float scale, O *__restrict__ gtable, unsigned long_groups, unsigned col_blocks,
+                                                    unsigned short_groups) {
     __shared__ float join[256 * VEC];
     const int tid = threadIdx.x, lane = tid & (lanes - 1), slot = tid / lanes, slots = 256 / lanes;
     auto write = [&](int64_t row, int col, const float *acc) {
@@ -381,10 +399,11 @@ __global__ __launch_bounds__(256) void k_embed_rows(const uint2 *__restrict__ bo
                 if (col + e < D) out[e] = o.v[e];
     };
     if (blockIdx.x < long_groups * col_blocks) {
-        const uint32_t n_long = long_rows[0];
+        const uint32_t n_long = lists.n[0];
         const int col = ((int)(blockIdx.x / long_groups) * lanes + lane) * VEC;
         for (uint32_t i = blockIdx.x % long_groups; i < n_long; i += long_groups) {
-            const int64_t v = long_rows[1 + i], rs = bounds[v].x, re = bounds[v + 1].x;
+            const Run run = lists.of_long[i];
+            const int64_t rs = run.first, re = run.end;
             const int64_t c_first = (rs + kChunk - 1) / kChunk, c_last = re / kChunk;      // whole chunks [c_first, c_last)
             const int64_t head = c_first < c_last ? c_first * kChunk : re, tail = c_first < c_last ? c_last * kChunk : re, skip = tail - head;
             float acc[VEC];
@@ -402,50 +421,66 @@ __global__ __launch_bounds__(256) void k_embed_rows(const uint2 *__restrict__ bo
                 for (int o = 1; o < slots; o++)
 #pragma unroll
                     for (int e = 0; e < VEC; e++) acc[e] += join[e * 256 + o * lanes + lane];
-                write(v, col, acc);
+                write(run.row, col, acc);
             }
             __syncthreads();
         }
         return;
     }
-    const int64_t v = (int64_t)(blockIdx.x - long_groups * col_blocks) * slots + slot;
-    if (v >= V) return;
-    const uint2 own = bounds[v];
-    const uint32_t s = own.x, e_ = bounds[v + 1].x;
-    if (e_ - s > (uint32_t)kShort) return;
-    for (int c0 = lane * VEC; c0 < D; c0 += kWide * lanes * VEC) {
-        float acc[kWide][VEC];
+    const unsigned group = blockIdx.x - long_groups * col_blocks;
+    if (group < short_groups) {
+        const uint32_t n_short = lists.n[1];
+        for (uint32_t i = group * slots + slot; i < n_short; i += short_groups * slots) {
+            const Run run = lists.of_short[i];
+            const int len = (int)(run.end - run.first);
+            uint32_t at[kShort];
+            at[0] = run.pos;
 #pragma unroll
-        for (int k = 0; k < kWide; k++)
+            for (int j = 1; j < kShort; j++) at[j] = pos[j < len ? run.first + j : run.first];
+            for (int c0 = lane * VEC; c0 < D; c0 += kWide * lanes * VEC) {
+                float acc[kWide][VEC];
 #pragma unroll
-            for (int e = 0; e < VEC; e++) acc[k][e] = 0.f;
-        for (uint32_t j = s; j < e_; j++) {
-            const T *row = grad + (int64_t)(j == s ? own.y : pos[j]) * ldg;
+                for (int k = 0; k < kWide; k++)
 #pragma unroll
-            for (int k = 0; k < kWide; k++) {
-                const int col = c0 + k * lanes * VEC;
-                if (col + VEC <= D) {
-                    const Loose<T, VEC> t = *reinterpret_cast<const Loose<T, VEC> *>(row + col);
+                    for (int e = 0; e < VEC; e++) acc[k][e] = 0.f;
 #pragma unroll
-                    for (int e = 0; e < VEC; e++) acc[k][e] += to_f32(t.v[e]);
-                } else {
+                for (int j = 0; j < kShort; j++) {
+                    if (j >= len) break;
+                    const T *row = grad + (int64_t)at[j] * ldg;
 #pragma unroll
-                    for (int e = 0; e < VEC; e++)
-                        if (col + e < D) acc[k][e] += to_f32(row[col + e]);
+                    for (int k = 0; k < kWide; k++) {
+                        const int col = c0 + k * lanes * VEC;
+                        if (col + VEC <= D) {
+                            const Loose<T, VEC> t = *reinterpret_cast<const Loose<T, VEC> *>(row + col);
+#pragma unroll
+                            for (int e = 0; e < VEC; e++) acc[k][e] += to_f32(t.v[e]);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < VEC; e++)
+                                if (col + e < D) acc[k][e] += to_f32(row[col + e]);
+                        }
+                    }
                 }
+#pragma unroll
+                for (int k = 0; k < kWide; k++)
+                    if (c0 + k * lanes * VEC < D) write(run.row, c0 + k * lanes * VEC, acc[k]);
             }
         }
-#pragma unroll
-        for (int k = 0; k < kWide; k++)
-            if (c0 + k * lanes * VEC < D) write(v, c0 + k * lanes * VEC, acc[k]);
+        return;
     }
+    const int64_t v = (int64_t)(group - short_groups) * slots + slot;
+    if (v >= V || lists.used[v]) return;
+    float zero[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; e++) zero[e] = 0.f;
+    for (int col = lane * VEC; col < D; col += lanes * VEC) write(v, col, zero);
 }
 
 // ------------------------------------------------------------------------------------------------ host
 struct BwdPlan {
     int bits, passes, nb_max, tile;
     int64_t blocks, per;            // multi-block sort
-    int64_t off_keys[2], off_pos[2], off_hist, off_partial, off_bounds, off_long, bytes;
+    int64_t off_keys[2], off_pos[2], off_hist, off_partial, off_used, off_long, off_short, off_n, bytes;
 };
 
 int64_t up256(int64_t b) { return (b + 255) / 256 * 256; }
@@ -470,18 +505,20 @@ BwdPlan plan_bwd(int64_t n, int64_t V, int64_t D) {
     }
     p.off_hist = one ? 0 : take(p.blocks * 4ll << p.nb_max);
     p.off_partial = take((n / kChunk) * D * 4);
-    p.off_bounds = take(8 * (V + 1));
-    p.off_long = take(4 * (1 + n / (kShort + 1)));
+    p.off_used = take(V);
+    p.off_long = take((int64_t)sizeof(Run) * (n / (kShort + 1)));
+    p.off_short = take((int64_t)sizeof(Run) * (n < V ? n : V));
+    p.off_n = take(8);
     p.bytes = at;
     return p;
 }
 
 template <typename I, int R>
-void launch_one(const I *idx, int n, int64_t V, int64_t padding, const BwdPlan &p, uint32_t *keys, uint32_t *pos, uint32_t *long_rows, hipStream_t s) {
+void launch_one(const I *idx, int n, int64_t V, int64_t padding, const BwdPlan &p, uint32_t *keys, uint32_t *pos, uint32_t *list_n, hipStream_t s) {
     const int lds = 4 * (256 + kSortWaves + kSortWaves * 256 / 2 + 2 * 1024 * R);
     static hsLdsAttrOnce attr;
     attr.set((const void *)k_sort_one<I, R>, lds);
-    k_sort_one<I, R><<<1, kSortThreads, lds, s>>>(idx, n, V, padding, p.bits, p.passes, keys, pos, long_rows);
+    k_sort_one<I, R><<<1, kSortThreads, lds, s>>>(idx, n, V, padding, p.bits, p.passes, keys, pos, list_n);
 }
 
 template <typename I, int R>
@@ -495,12 +532,12 @@ void launch_scatter(const I *idx, const uint32_t *k_in, const uint32_t *p_in, in
 
 template <typename I>
 void launch_sort(const I *idx, int64_t n, int64_t V, int64_t padding, const BwdPlan &p, char *ws, uint32_t *&keys, uint32_t *&pos, hipStream_t s) {
-    uint32_t *long_rows = (uint32_t *)(ws + p.off_long);
+    uint32_t *list_n = (uint32_t *)(ws + p.off_n);
     if (n <= kOneMax) {
         keys = (uint32_t *)(ws + p.off_keys[0]);
         pos = (uint32_t *)(ws + p.off_pos[0]);
-        if (n <= 1024) launch_one<I, 1>(idx, (int)n, V, padding, p, keys, pos, long_rows, s);
-        else launch_one<I, 4>(idx, (int)n, V, padding, p, keys, pos, long_rows, s);
+        if (n <= 1024) launch_one<I, 1>(idx, (int)n, V, padding, p, keys, pos, list_n, s);
+        else launch_one<I, 4>(idx, (int)n, V, padding, p, keys, pos, list_n, s);
         return;
     }
     uint32_t *hist = (uint32_t *)(ws + p.off_hist), *k_in = nullptr, *p_in = nullptr;
@@ -509,7 +546,7 @@ void launch_sort(const I *idx, int64_t n, int64_t V, int64_t padding, const BwdP
         const int nb = (p.bits - shift + p.passes - pass - 1) / (p.passes - pass);
         keys = (uint32_t *)(ws + p.off_keys[pass & 1]);
         pos = (uint32_t *)(ws + p.off_pos[pass & 1]);
-        k_sort_hist<I><<<(unsigned)p.blocks, kSortThreads, 0, s>>>(idx, k_in, n, p.per, V, padding, shift, nb, hist, long_rows);
+        k_sort_hist<I><<<(unsigned)p.blocks, kSortThreads, 0, s>>>(idx, k_in, n, p.per, V, padding, shift, nb, hist, list_n);
         if (p.tile == 1024) launch_scatter<I, 1>(idx, k_in, p_in, n, V, padding, p, shift, nb, hist, keys, pos, s);
         else if (p.tile == 2048) launch_scatter<I, 2>(idx, k_in, p_in, n, V, padding, p, shift, nb, hist, keys, pos, s);
         else launch_scatter<I, 4>(idx, k_in, p_in, n, V, padding, p, shift, nb, hist, keys, pos, s);
@@ -581,10 +618,11 @@ int hs_embed_bwd(const void *indices, int32_t index_bytes, const void *grad, int
     const unsigned col_blocks = (unsigned)((D + (int64_t)lanes * VEC - 1) / ((int64_t)lanes * VEC));
     const int64_t row_blocks = (V + 256 / lanes - 1) / (256 / lanes);
     const unsigned bound_blocks = (unsigned)(V / 256 + 1);
-    uint2 *bounds = (uint2 *)((char *)ws + p.off_bounds);
-    uint32_t *long_rows = (uint32_t *)((char *)ws + p.off_long);
+    const RunLists lists = {(Run *)((char *)ws + p.off_long), (Run *)((char *)ws + p.off_short), (uint32_t *)((char *)ws + p.off_n), (uint8_t *)ws + p.off_used};
     const int64_t most_long = n / (kShort + 1);
     const unsigned long_groups = (unsigned)(most_long < kLongGroups ? most_long : kLongGroups);
+    const int64_t most_short = ((n < V ? n : V) + 256 / lanes - 1) / (256 / lanes);
+    const unsigned short_groups = (unsigned)(most_short < kShortGroups ? most_short : kShortGroups);
     const int64_t chunks = n / kChunk, row_bytes = D * elem_bytes(table_dtype);
     HS_BY_DTYPE(grad_dtype, {
         using G = T;
@@ -594,16 +632,19 @@ int hs_embed_bwd(const void *indices, int32_t index_bytes, const void *grad, int
         for (int64_t c0 = 0; c0 == 0 || c0 < chunks;) {
             const int64_t take = chunks - c0 < kMaxGrid - first ? chunks - c0 : kMaxGrid - first;
             k_embed_chunks<G, W><<<dim3(first + (unsigned)take, col_blocks), 256, 0, s>>>(keys + c0 * kChunk, pos + c0 * kChunk, (const G *)grad, ldg, n, (uint32_t)V, (int)D, lanes,
-                                                                                       partial + c0 * D, bounds, long_rows, first);
+                                                                                       partial + c0 * D, lists, first);
             first = 0;
             if (take == chunks - c0) break;
             c0 += take;
         }
-        unsigned lead = long_groups * col_blocks;
+        unsigned lead = long_groups * col_blocks + short_groups;
         for (int64_t b0 = 0; b0 < row_blocks;) {
             const int64_t take = row_blocks - b0 < kMaxGrid - lead ? row_blocks - b0 : kMaxGrid - lead, v0 = b0 * (256 / lanes);
-            HS_BY_DTYPE(table_dtype, (k_embed_rows<G, T, W><<<lead + (unsigned)take, 256, 0, s>>>(bounds + v0, long_rows, pos, (const G *)grad, ldg, V - v0, (int)D, lanes, partial, scale,
-                                                                                               (T *)((char *)grad_table + v0 * row_bytes), lead ? long_groups : 0u, col_blocks)));
+            RunLists from = lists;
+            from.used += v0;
+            HS_BY_DTYPE(table_dtype, (k_embed_rows<G, T, W><<<lead + (unsigned)take, 256, 0, s>>>(from, pos, (const G *)grad, ldg, V - v0, (int)D, lanes, partial, scale,
+                                                                                               (T *)((char *)grad_table + v0 * row_bytes), lead ? long_groups : 0u, col_blocks,
+                                                                                               lead ? short_groups : 0u)));
             lead = 0;
             b0 += take;
         }
