@@ -155,7 +155,8 @@ _ROW_BYTES = ("hs_embed_bwd_ws_bytes", "hs_gated_mlp_saved_bytes", "hs_gated_mlp
 _p, _i, _l, _f = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
 # (declared once: a call then takes plain integers -- the smallest calls are bound by the host)
 _ROW_ARGTYPES = {"hs_embed_fwd": (_p, _i, _p, _l, _p, _l, _l, _l, _f, _i, _i, _p), "hs_embed_bwd_ws_bytes": (_l, _l, _l),
-                 "hs_embed_bwd": (_p, _i, _p, _l, _p, _l, _l, _l, _f, _l, _i, _i, _p, _l, _p), "hs_dropout_rows": (_p, _p, _p, _l, _i, _i, _p, _p)}
+                 "hs_embed_bwd": (_p, _i, _p, _l, _p, _l, _l, _l, _f, _l, _i, _i, _p, _l, _p), "hs_dropout_rows": (_p, _p, _p, _l, _i, _i, _p, _p),
+                 "hs_gated_mlp_saved_bytes": (_p,), "hs_gated_mlp_fwd_ws_bytes": (_p,), "hs_gated_mlp_bwd_ws_bytes": (_p,), "hs_gated_mlp_fwd": (_p, _p), "hs_gated_mlp_bwd": (_p, _p)}
 ROW_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}        # HS_F32 / HS_BF16 / HS_F16: section 10 (row operators)
 ROW_ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "sigmoid": 3, "relu": 4}       # HS_ACT_*
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}  # HS_F32 / HS_BF16
@@ -1636,18 +1637,20 @@ class _HipBackend:
         _check(load_library().hs_dropout_rows(x.data_ptr(), None if residual is None else residual.data_ptr(), y.data_ptr(), x.numel(), ROW_DTYPES[x.dtype], drop,
                                               rng.data_ptr(), _row_stream(x)), "hs_dropout_rows")
 
-    @classmethod
-    def _gated_args(cls, x, w_gate, w_up, w_down, activation):
-        return hsGatedMlp(x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), cls._ld(x), cls._ld(w_gate), cls._ld(w_up), cls._ld(w_down), x.shape[0],
-                          x.shape[1], w_gate.shape[0], ROW_DTYPES[x.dtype], ROW_ACTIVATIONS[activation])
+    @staticmethod
+    def _gated_args(x, w_gate, w_up, w_down, activation):
+        rows, dim = x.shape
+        hidden = w_gate.shape[0]
+        return hsGatedMlp(x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), x.stride(0) if rows > 1 else dim, w_gate.stride(0) if hidden > 1 else dim,
+                          w_up.stride(0) if hidden > 1 else dim, w_down.stride(0) if dim > 1 else hidden, rows, dim, hidden, ROW_DTYPES[x.dtype], ROW_ACTIVATIONS[activation])
 
     @staticmethod
-    def _gated_call(a, fn, nbytes, x):
+    def _gated_call(a, call, nbytes, x, fn):
         _check(min(nbytes, 0), fn)
         if nbytes:
             ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
             a.ws, a.ws_bytes = ws.data_ptr(), nbytes
-        _check(getattr(load_library(), fn)(ctypes.byref(a), ctypes.c_void_p(_row_stream(x))), fn)
+        _check(call(ctypes.byref(a), _row_stream(x)), fn)
 
     @classmethod
     def gated_mlp_fwd(cls, x, w_gate, w_up, w_down, activation, y, save):
@@ -1661,7 +1664,7 @@ class _HipBackend:
             saved = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
             a.saved = saved.data_ptr()
         a.y = y.data_ptr()
-        cls._gated_call(a, "hs_gated_mlp_fwd", lib.hs_gated_mlp_fwd_ws_bytes(ctypes.byref(a)), x)
+        cls._gated_call(a, lib.hs_gated_mlp_fwd, lib.hs_gated_mlp_fwd_ws_bytes(ctypes.byref(a)), x, "hs_gated_mlp_fwd")
         return saved
 
     @classmethod
@@ -1671,7 +1674,7 @@ class _HipBackend:
         a = cls._gated_args(x, w_gate, w_up, w_down, activation)
         a.grad, a.ld_grad, a.saved = grad.data_ptr(), cls._ld(grad), saved.data_ptr()
         a.gx, a.gw_gate, a.gw_up, a.gw_down = (None if t is None else t.data_ptr() for t in (gx, gw_gate, gw_up, gw_down))
-        cls._gated_call(a, "hs_gated_mlp_bwd", lib.hs_gated_mlp_bwd_ws_bytes(ctypes.byref(a)), x)
+        cls._gated_call(a, lib.hs_gated_mlp_bwd, lib.hs_gated_mlp_bwd_ws_bytes(ctypes.byref(a)), x, "hs_gated_mlp_bwd")
 
 
 class hsAdamState(ctypes.Structure):

@@ -61,6 +61,8 @@ def _as_rows(t):
     """[..., n] -> 2-D with consecutive elements in a row: the tensor itself (any row distance >= n), else a copy."""
     if t.dim() != 2:
         t = t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
+    if t.is_contiguous():
+        return t
     if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
         t = t.contiguous()
     return t
@@ -155,12 +157,13 @@ def gated_mlp_rows(x, w_gate, w_up, w_down, activation="silu"):
     _check_tensor(x, "x")
     if x.dim() < 1:
         raise RuntimeError("x must be [..., dim]")
+    device, dtype = x.device, x.dtype
     for t, name in ((w_gate, "w_gate"), (w_up, "w_up"), (w_down, "w_down")):
-        _check_tensor(t, name, device=x.device, dtype=x.dtype)
+        _check_tensor(t, name, device, dtype)
         if t.dim() != 2:
             raise RuntimeError(f"{name} must be a matrix, got {tuple(t.shape)}")
     hidden, dim = w_gate.shape
-    if x.shape[-1] != dim or w_up.shape != (hidden, dim) or w_down.shape != (dim, hidden):
+    if x.shape[-1] != dim or w_up.shape != w_gate.shape or w_down.shape != (dim, hidden):
         raise RuntimeError(f"x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, w_up {tuple(w_up.shape)}, w_down {tuple(w_down.shape)}: expected [..., dim], "
                            "[hidden, dim], [hidden, dim], [dim, hidden]")
     if max(hidden, dim) > 1 << 21:
@@ -171,7 +174,8 @@ def gated_mlp_rows(x, w_gate, w_up, w_down, activation="silu"):
         return _gated_mlp_rows.apply(x, w_gate, w_up, w_down, activation)
     if x.numel() == 0 or hidden == 0:
         return torch.zeros_like(x)
-    return _gated(_as_rows(x), _as_rows(w_gate), _as_rows(w_up), _as_rows(w_down), activation, False)[0].view(x.shape)
+    y = _gated(_as_rows(x), _as_rows(w_gate), _as_rows(w_up), _as_rows(w_down), activation, False)[0]
+    return y if x.dim() == 2 else y.view(x.shape)
 
 
 def _dropout(x, residual, drop, rng):
