@@ -105,17 +105,18 @@ __global__ __launch_bounds__(256) void k_rows_reduce(const ReduceJobs jobs) {
 struct Plan { int tile, slices; };
 struct TileCost { int rows, cols, fit; float first, more; };
 constexpr TileCost kTiles16[4] = {{256, 256, 1, 1.9f, 0.f}, {128, 128, 2, 0.8f, 0.38f}, {64, 64, 5, 0.5f, 0.15f}, {128, 128, 1, 0.66f, 0.f}};
-constexpr TileCost kTiles32[3] = {{256, 256, 1, 11.4f, 0.f}, {128, 64, 1, 2.1f, 0.f}, {64, 64, 1, 1.15f, 0.f}};
+constexpr TileCost kTiles32[3] = {{256, 256, 1, 11.4f, 0.f}, {128, 64, 1, 1.75f, 0.f}, {64, 64, 1, 1.f, 0.f}};
+constexpr int kSlices[] = {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 28, 32, 40, 48, 56, 64};
 template <typename U> Plan plan_product(int64_t I, int64_t cols, int64_t steps, int problems, bool sliceable) {
     const TileCost *kinds = sizeof(U) == 4 ? kTiles32 : kTiles16;
     Plan best = {0, 1};
     float least = 0.f;
-    for (int k = 0; k < (sizeof(U) == 4 ? 3 : 4); k++)
-        for (int slices = 1; slices <= (sliceable ? 64 : 1); slices *= 2) {
-            if (slices > 1 && steps / slices < 4) break;
-            const TileCost &t = kinds[k];
-            const int64_t groups = ((I + t.rows - 1) / t.rows) * ((cols + t.cols - 1) / t.cols) * problems * slices;
-            const int64_t each = (groups + 255) / 256, together = each < t.fit ? each : t.fit, rounds = (groups + 256 * together - 1) / (256 * together);
+    for (int k = 0; k < (sizeof(U) == 4 ? 3 : 4); k++) {
+        const TileCost &t = kinds[k];
+        const int64_t whole = ((I + t.rows - 1) / t.rows) * ((cols + t.cols - 1) / t.cols) * problems;
+        for (int slices : kSlices) {
+            if (slices > 1 && (!sliceable || steps < 4 * slices || whole > 1024)) break;
+            const int64_t each = (whole * slices + 255) / 256, together = each < t.fit ? each : t.fit, rounds = (each + together - 1) / together;
             float us = (float)rounds * ((float)((steps + slices - 1) / slices) * (t.first + t.more * (float)(together - 1)) + 3.f);
             if (slices > 1) us += 4.f + (float)(I * cols * problems) * (float)slices * 2e-6f;        // partial results written and read at 4 TB/s, one launch more
             if (least == 0.f || us < least) {
@@ -123,22 +124,24 @@ template <typename U> Plan plan_product(int64_t I, int64_t cols, int64_t steps, 
                 best = Plan{k, slices};
             }
         }
+    }
     return best;
 }
 
 template <typename T, typename U, bool AKS, bool BKS, int EPI> int launch_product(Args &p, int tile, int problems, hipStream_t s) {
     constexpr int P = planes<U>();
     if (tile == 0) return launch_tile<T, U, 1, 2, 256, 256, 2, 4, AKS, BKS, EPI>(p, problems, s);
-    if (tile == 1) return launch_tile<T, U, P, 2, 128, P == 3 ? 64 : 128, 2, 2, AKS, BKS, EPI>(p, problems, s);
+    // fp32, one workgroup a CU: eight waves, so that a wave's LDS reads pass beside another's products (128 x 64: 37 -> 30 us for G and U of 4 096 x 256 x 683)
+    if (tile == 1) return launch_tile<T, U, P, 2, 128, P == 3 ? 64 : 128, P == 3 ? 4 : 2, 2, AKS, BKS, EPI>(p, problems, s);
     if constexpr (P == 1) {
         if (tile == 3) return launch_tile<T, U, P, 4, 128, 128, 2, 4, AKS, BKS, EPI>(p, problems, s);
     }
-    return launch_tile<T, U, P, 2, 64, 64, 2, 2, AKS, BKS, EPI>(p, problems, s);
+    return launch_tile<T, U, P, P == 3 ? 3 : 2, 64, 64, P == 3 ? 4 : 2, 2, AKS, BKS, EPI>(p, problems, s);
 }
 
-// Up to this D the backward pass computes G and U again: 4 D operations an element against 16 bytes.  (At D = 256, 131 072 x 1 024: forward and this part of the
-// backward 660 us against 780 with G and U kept.)
-constexpr int64_t kAgainDim = 768;
+// Up to this D the backward pass computes G and U again: 4 D operations an element (fp32: six times that) against 16 bytes.  (At D = 256: 131 072 x 1 024 in
+// bf16, forward and this part of the backward 660 us against 780 with G and U kept; 4 096 x 683 in fp32 77 us against 66.)
+template <typename U> constexpr int64_t again_dim() { return sizeof(U) == 4 ? 128 : 768; }
 
 // Up to this many rows the forward products read the weights in place (rows_small.h).  4 096 x 12 288 bf16: 105 us at 33 rows, 145 at 64, where the tiles take
 // 104 at 65; fp32, whose tiles need copies in planes: 392 at 64 against 738 at 65.
@@ -190,7 +193,7 @@ template <typename T, typename U> struct Block {
     }
 
     // whether the backward pass computes G and U again instead of reading them
-    bool again() const { return D <= kAgainDim; }
+    bool again() const { return D <= again_dim<U>(); }
 
     struct Saved { float *g, *u; Operand h; int64_t bytes; };
     Saved saved_in(char *base) const {

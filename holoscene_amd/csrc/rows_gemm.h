@@ -145,6 +145,11 @@ __device__ __forceinline__ F8 load8(const float *p) {
     const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
     return F8{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
 }
+// the same of eight elements in LDS, rounded already
+template <typename U> __device__ __forceinline__ void store_staged(void *base, int64_t plane, int64_t at, const U *s) {
+    if constexpr (sizeof(U) == 4) store_operand8<U>(base, plane, at, load8(s).v);
+    else *reinterpret_cast<Pack<U, 8> *>((U *)base + at) = *reinterpret_cast<const Pack<U, 8> *>(s);
+}
 __device__ __forceinline__ void store8(float *p, const F8 &f) {
     reinterpret_cast<float4 *>(p)[0] = make_float4(f.v[0], f.v[1], f.v[2], f.v[3]);
     reinterpret_cast<float4 *>(p)[1] = make_float4(f.v[4], f.v[5], f.v[6], f.v[7]);
@@ -257,16 +262,22 @@ __device__ __forceinline__ TilePlace tile_place(int tiles_i, int tiles_j) {
     return TilePlace{group * 8 + in % rows, in / rows};
 }
 
-// Accumulators through LDS as a tile of fp32 rows: MP of each wave's MT row groups at a time, COLS columns of fp32 a row, items of 8 of the TJ result columns.
-template <int COLS, int MT, int MP_, int WI, int WAVES, int TJ> struct Staging {
-    static constexpr int MP = MP_, kPasses = MT / MP, kLines = WI * MP * 16, kPitch = COLS + 4, kItems = kLines * (TJ / 8), kIter = kItems / (64 * WAVES);
-    static constexpr int kBytes = kLines * kPitch * 4;
-    static_assert(kItems % (64 * WAVES) == 0 && kIter >= 1, "items must fill the workgroup");
-    static __device__ __forceinline__ int line(int tid, int k) { return (tid + k * 64 * WAVES) / (TJ / 8); }
-    static __device__ __forceinline__ int col(int tid, int k) { return (tid + k * 64 * WAVES) % (TJ / 8) * 8; }
-    static __device__ __forceinline__ int row(int tid, int pass, int k) {
-        const int r = line(tid, k);
-        return r / (MP * 16) * (MT * 16) + pass * MP * 16 + r % (MP * 16);
+// Results of the gate kernels through LDS: MP of each wave's MT row groups at a time (as many as MOST and the workgroup's LDS admit), COLS columns of U a row, items of
+// 8 of the TJ result columns.
+template <typename U, int COLS, int TJ, int MT, int WI, int WAVES, int MOST, int LDS> struct Staging {
+    static constexpr int kPitch = COLS + 16 / (int)sizeof(U);
+    static constexpr int bytes(int mp) { return WI * mp * 16 * kPitch * (int)sizeof(U); }
+    static constexpr int most(int mp) { return mp > 1 && (mp > MOST || bytes(mp) > LDS) ? most(mp / 2) : mp; }
+    static constexpr int MP = most(MT), kPasses = MT / MP, kLines = WI * MP * 16, kItems = kLines * (TJ / 8);
+    static_assert(bytes(MP) <= LDS && MT % MP == 0, "the epilogue's tile must fit");
+    // f(row of the tile (of pass 0), line of the stage, column) for this thread's items
+    template <typename F> static __device__ __forceinline__ void copy_out(int tid, F f) {
+#pragma unroll
+        for (int k = 0; k < (kItems + 64 * WAVES - 1) / (64 * WAVES); k++) {
+            const int item = tid + k * 64 * WAVES, line = item / (TJ / 8);
+            if (kItems % (64 * WAVES) != 0 && item >= kItems) break;
+            f(line / (MP * 16) * (MT * 16) + line % (MP * 16), line, item % (TJ / 8) * 8);
+        }
     }
 };
 
@@ -416,70 +427,70 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_rows_gemm(const Args p) {
             }
         }
     } else {
-        // Through LDS, MP row groups of every wave at a time, so that the elementwise part is a short loop over 8 consecutive columns a thread (full lines of
-        // global memory, one copy of the activation's code: unrolled over the accumulators it did not fit the instruction cache and took longer than
-        // the products).  Columns up to ldh are written: behind J nothing was read, so the padding of G, U, H, gg and gu is zero.
-        using St = Staging<BN, MT, EPI == EPI_GATE_BWD ? 1 : 2, WI, WAVES, TJ>;     // (G and U of a whole pass are in registers: 16 a thread and item)
-        F8 gq[St::kIter], uq[St::kIter];
-        auto fetch = [&](int pass, int k) {                 // (clamped: nothing branches between the requests)
-            int64_t i = i0 + St::row(tid, pass, k), j = j0 + St::col(tid, k);
+        // A lane has both projections (EPI_GATE) of the same elements, or fetches G and U of its own: the elementwise part is done where the products are, rounded,
+        // and only its results pass through LDS, so that full lines of global memory are written.  Columns up to ldh are written: behind J nothing was
+        // read, so the padding of G, U, H, gg and gu is zero.
+        constexpr int COLS = EPI == EPI_GATE ? TJ : 2 * TJ, N = DUAL ? NT / 2 : NT;
+        using St = Staging<U, COLS, TJ, MT, WI, WAVES, EPI == EPI_GATE ? MT : 1, BUFS * P * (BM + BN) * BK * 2>;
+        f32x4 gq[N], uq[N];
+        auto place = [&](int m, int n) {                    // (clamped: nothing branches between the requests)
+            int64_t i = i0 + (wi * MT + m) * 16 + li, j = j0 + (wj * N + n) * 16 + lq * 4;
             i = i < p.I ? i : p.I - 1;
-            j = j < p.ldh ? j : p.ldh - 8;
-            gq[k] = load8(p.g + i * p.ldh + j);
-            uq[k] = load8(p.u + i * p.ldh + j);
+            j = j < p.ldh ? j : p.ldh - 4;
+            return i * p.ldh + j;
         };
-        if constexpr (EPI == EPI_GATE_BWD) {
+        auto fetch = [&](int m) {
 #pragma unroll
-            for (int k = 0; k < St::kIter; k++) fetch(0, k);
-        }
-        float *stage = reinterpret_cast<float *>(lds);
+            for (int n = 0; n < N; n++) {
+                gq[n] = *reinterpret_cast<const f32x4 *>(p.g + place(m, n));
+                uq[n] = *reinterpret_cast<const f32x4 *>(p.u + place(m, n));
+            }
+        };
+        if constexpr (EPI == EPI_GATE_BWD) fetch(0);
+        U *stage = reinterpret_cast<U *>(lds);
         with_activation(p.act, [&](auto act) {
             constexpr int ACT = decltype(act)::value;
 #pragma unroll
             for (int pass = 0; pass < St::kPasses; pass++) {
                 meet();
 #pragma unroll
-                for (int m = 0; m < St::MP; m++)
+                for (int mp = 0; mp < St::MP; mp++) {
+                    const int m = pass * St::MP + mp;
 #pragma unroll
-                    for (int n = 0; n < NT; n++) {
-                        const int col = DUAL ? (n < NT / 2 ? (wj * (NT / 2) + n) * 16 : BN / 2 + (wj * (NT / 2) + n - NT / 2) * 16) : (wj * NT + n) * 16;
-                        *reinterpret_cast<f32x4 *>(stage + ((wi * St::MP + m) * 16 + li) * St::kPitch + col + lq * 4) = acc[pass * St::MP + m][n];
-                    }
-                meet();
+                    for (int n = 0; n < N; n++) {
+                        U *at = stage + ((wi * St::MP + mp) * 16 + li) * St::kPitch + (wj * N + n) * 16 + lq * 4;
+                        Pack<U, 4> o, o1;
+                        float d;
+                        if constexpr (EPI == EPI_GATE) {
+                            const f32x4 g = acc[m][n], u = acc[m][n + N];
 #pragma unroll
-                for (int k = 0; k < St::kIter; k++) {
-                    const int64_t i = i0 + St::row(tid, pass, k), at = i * p.ldh + j0 + St::col(tid, k);
-                    const bool in = i < p.I && j0 + St::col(tid, k) < p.ldh;
-                    const float *s = stage + St::line(tid, k) * St::kPitch + St::col(tid, k);
-                    const F8 a = load8(s);
-                    float unused;
-                    if constexpr (EPI == EPI_GATE) {
-                        const F8 u = load8(s + BN / 2);
-                        F8 h;
-#pragma unroll
-                        for (int e = 0; e < 8; e++) h.v[e] = activation<ACT, false>(a.v[e], unused) * u.v[e];
-                        if (in) {
-                            if (p.g) {
-                                store8(p.g + at, a);
-                                store8(p.u + at, u);
+                            for (int r = 0; r < 4; r++) o.v[r] = from_f32<U>(activation<ACT, false>(g[r], d) * u[r]);
+                            if (p.g && i0 + (wi * MT + m) * 16 + li < p.I && j0 + (wj * N + n) * 16 + lq * 4 < p.ldh) {
+                                *reinterpret_cast<f32x4 *>(p.g + place(m, n)) = g;
+                                *reinterpret_cast<f32x4 *>(p.u + place(m, n)) = u;
                             }
-                            store_operand8<U>(p.h, p.plane, at, h.v);
-                        }
-                    } else {
-                        F8 gg, gu;
+                        } else {
 #pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            float d;
-                            gu.v[e] = a.v[e] * activation<ACT, true>(gq[k].v[e], d);
-                            gg.v[e] = a.v[e] * uq[k].v[e] * d;
+                            for (int r = 0; r < 4; r++) {
+                                o1.v[r] = from_f32<U>(acc[m][n][r] * activation<ACT, true>(gq[n][r], d));
+                                o.v[r] = from_f32<U>(acc[m][n][r] * uq[n][r] * d);
+                            }
+                            *reinterpret_cast<Pack<U, 4> *>(at + TJ) = o1;
                         }
-                        if (pass + 1 < St::kPasses) fetch(pass + 1, k);
-                        if (in) {
-                            store_operand8<U>(p.gg, p.plane, at, gg.v);
-                            store_operand8<U>(p.gu, p.plane, at, gu.v);
-                        }
+                        *reinterpret_cast<Pack<U, 4> *>(at) = o;
                     }
                 }
+                if constexpr (EPI == EPI_GATE_BWD) {
+                    if (pass + 1 < St::kPasses) fetch(pass + 1);
+                }
+                meet();
+                St::copy_out(tid, [&](int row, int line, int col) {
+                    const int64_t i = i0 + row + pass * St::MP * 16, at = i * p.ldh + j0 + col;
+                    if (i >= p.I || j0 + col >= p.ldh) return;
+                    const U *s = stage + line * St::kPitch + col;
+                    store_staged(EPI == EPI_GATE ? p.h : p.gg, p.plane, at, s);
+                    if constexpr (EPI == EPI_GATE_BWD) store_staged(p.gu, p.plane, at, s + TJ);
+                });
             }
         });
     }
@@ -510,7 +521,6 @@ inline int launch_tile(Args p, int problems, hipStream_t s) {
     p.tiles_j = (int)tj;
     if constexpr (planes<U>() != P) as_segments(p);
     constexpr int lds = BUFS * P * (BM + BN) * BK * 2;
-    static_assert(Staging<BN, BM / WI / 16, 2, WI, WI * WJ, TJ>::kBytes <= lds, "the epilogue's tile must fit");
     static hsLdsAttrOnce attr;
     const void *fn = (const void *)k_rows_gemm<T, U, P, BUFS, BM, BN, WI, WJ, AKS, BKS, EPI>;
     attr.set(fn, lds);
@@ -600,54 +610,52 @@ __global__ __launch_bounds__(256) void k_gate_bwd(const Args p) {
                                        [&]() { if (s + 1 < steps) request2(buf ^ 1); }, acc2);
         buf ^= 1;
     }
-    using St = Staging<3 * TJ, MT, 2, WI, WAVES, TJ>;
-    static_assert(St::kBytes <= 2 * kBuf, "the epilogue's tile must fit");
+    // A lane has G, U and gH of the same elements: gg and gu are computed where they are, rounded, and only then pass through LDS, so that full lines of global
+    // memory are written (131 072 x 256 x 1 024: 369 us; G, U and gH in fp32 through LDS: 381)
+    using St = Staging<U, 2 * TJ, TJ, MT, WI, WAVES, MT, 2 * (int)kBuf>;
     const int li = lane & 15, lq = lane >> 4;
-    float *stage = reinterpret_cast<float *>(lds);
+    U *stage = reinterpret_cast<U *>(lds);
     with_activation(p.act, [&](auto act) {
         constexpr int ACT = decltype(act)::value;
 #pragma unroll
         for (int pass = 0; pass < St::kPasses; pass++) {
             meet();
 #pragma unroll
-            for (int m = 0; m < St::MP; m++) {
-                float *row = stage + ((wi * St::MP + m) * 16 + li) * St::kPitch + wj * N2 * 16 + lq * 4;
+            for (int m = 0; m < St::MP; m++)
 #pragma unroll
                 for (int n = 0; n < N2; n++) {
-                    *reinterpret_cast<f32x4 *>(row + n * 16) = acc[pass * St::MP + m][n];
-                    *reinterpret_cast<f32x4 *>(row + TJ + n * 16) = acc[pass * St::MP + m][n + N2];
-                    *reinterpret_cast<f32x4 *>(row + 2 * TJ + n * 16) = acc2[pass * St::MP + m][n];
+                    Pack<U, 4> gg, gu;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const float gh = acc2[pass * St::MP + m][n][r];
+                        float d;
+                        gu.v[r] = from_f32<U>(gh * activation<ACT, true>(acc[pass * St::MP + m][n][r], d));
+                        gg.v[r] = from_f32<U>(gh * acc[pass * St::MP + m][n + N2][r] * d);
+                    }
+                    U *at = stage + ((wi * St::MP + m) * 16 + li) * St::kPitch + (wj * N2 + n) * 16 + lq * 4;
+                    *reinterpret_cast<Pack<U, 4> *>(at) = gg;
+                    *reinterpret_cast<Pack<U, 4> *>(at + TJ) = gu;
                 }
-            }
             meet();
-#pragma unroll
-            for (int k = 0; k < St::kIter; k++) {
-                const int64_t i = i0 + St::row(tid, pass, k), at = i * p.ldh + j0 + St::col(tid, k);
-                const float *s = stage + St::line(tid, k) * St::kPitch + St::col(tid, k);
-                const F8 g = load8(s), u = load8(s + TJ), gh = load8(s + 2 * TJ);
-                F8 gg, gu;
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    float d;
-                    gu.v[e] = gh.v[e] * activation<ACT, true>(g.v[e], d);
-                    gg.v[e] = gh.v[e] * u.v[e] * d;
-                }
-                if (i < p.I && j0 + St::col(tid, k) < p.ldh) {
-                    store_operand8<U>(p.gg, p.plane, at, gg.v);
-                    store_operand8<U>(p.gu, p.plane, at, gu.v);
-                }
-            }
+            St::copy_out(tid, [&](int row, int line, int col) {
+                const int64_t i = i0 + row + pass * St::MP * 16, at = i * p.ldh + j0 + col;
+                if (i >= p.I || j0 + col >= p.ldh) return;
+                const U *s = stage + line * St::kPitch + col;
+                store_staged(p.gg, p.plane, at, s);
+                store_staged(p.gu, p.plane, at, s + TJ);
+            });
         }
     });
 }
 
 template <typename T, typename U> inline int launch_gate_bwd(Args p, hipStream_t s) {
+    constexpr int BM = kAgainM;
     if constexpr (planes<U>() == 3) as_segments(p);
-    const int64_t ti = (p.I + kAgainM - 1) / kAgainM, tj = (p.ldh + kAgainJ - 1) / kAgainJ;
+    const int64_t ti = (p.I + BM - 1) / BM, tj = (p.ldh + kAgainJ - 1) / kAgainJ;
     if (ti * tj > kMaxGrid / 256) return HS_ERR_ARG;
     p.tiles_i = (int)ti;
     p.tiles_j = (int)tj;
-    constexpr int lds = 2 * (kAgainM + 2 * kAgainJ) * BK * 2;
+    constexpr int lds = 2 * (BM + 2 * kAgainJ) * BK * 2;
     static hsLdsAttrOnce attr;
     attr.set((const void *)k_gate_bwd<T, U>, lds);
     k_gate_bwd<T, U><<<dim3((unsigned)(ti * tj)), 256, lds, s>>>(p);
