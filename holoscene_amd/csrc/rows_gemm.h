@@ -52,7 +52,7 @@ struct Args {
     int64_t plane_a, plane_b;                     // bytes between planes
     int64_t I;
     int32_t J, K;
-    int32_t tiles_i, tiles_j, slices;
+    int32_t tiles_i, tiles_j, problems, slices;
     // EPI_STORE
     void *out[2];                                 // per problem
     int64_t ldo;
@@ -252,14 +252,17 @@ template <int R, bool KS, int WAVES, int OWN> struct Side {
     }
 };
 
-// Which tile a workgroup takes: eight contiguous ranges of tiles, one per XCD (workgroups go round the XCDs), each walked in groups of 8 row tiles so that the
-// tiles in flight on an XCD share operands in its L2.
-struct TilePlace { int i, j; };
-__device__ __forceinline__ TilePlace tile_place(int tiles_i, int tiles_j) {
-    const int n = tiles_i * tiles_j, per_xcd = n / 8, rest = n % 8, xcd = blockIdx.x % 8;
+// Which tile of which problem and slice a workgroup takes: eight contiguous ranges, one per XCD (workgroups go round the XCDs), the tiles of a slice next to each
+// other, walked in groups of 8 row tiles, so that the tiles in flight on an XCD share operands in its L2.  (Slices spread over the XCDs, each of which then reads
+// the whole of the smaller operand: gWd of 131 072 x 256 x 1 024 128 us against 99, gWg and gWu of 4 096 x 256 x 683 in fp32 29 against 23.)  Problems that are
+// not sliced follow one another (blockIdx.y).
+struct TilePlace { int i, j, problem, slice; };
+__device__ __forceinline__ TilePlace tile_place(int tiles_i, int tiles_j, int problems, int slices) {      // problems: side by side in a slice
+    const int tiles = tiles_i * tiles_j, n = tiles * problems * slices, per_xcd = n / 8, rest = n % 8, xcd = blockIdx.x % 8;
     const int t = xcd * per_xcd + (xcd < rest ? xcd : rest) + blockIdx.x / 8;
-    const int group = t / (8 * tiles_j), in = t - group * 8 * tiles_j, rows = tiles_i - group * 8 < 8 ? tiles_i - group * 8 : 8;
-    return TilePlace{group * 8 + in % rows, in / rows};
+    const int which = t / tiles, at = t - which * tiles;
+    const int group = at / (8 * tiles_j), in = at - group * 8 * tiles_j, rows = tiles_i - group * 8 < 8 ? tiles_i - group * 8 : 8;
+    return TilePlace{group * 8 + in % rows, in / rows, which % problems + (int)blockIdx.y, which / problems};
 }
 
 // Results of the gate kernels through LDS: MP of each wave's MT row groups at a time (as many as MOST and the workgroup's LDS admit), COLS columns of U a row, items of
@@ -336,10 +339,10 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_rows_gemm(const Args p) {
     using SB = Side<BN, BKS, WAVES, NT>;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wi = wave / WJ, wj = wave % WJ;
-    const TilePlace t = tile_place(p.tiles_i, p.tiles_j);
+    const TilePlace t = tile_place(p.tiles_i, p.tiles_j, p.problems, p.slices);
     const int64_t i0 = (int64_t)t.i * BM;
     const int j0 = t.j * TJ;
-    const Seg *segs = p.seg[blockIdx.z];
+    const Seg *segs = p.seg[t.problem];
 
     SA sa;
     SB sb;
@@ -350,7 +353,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_rows_gemm(const Args p) {
     constexpr uint32_t kBuf = P * (SA::kBytes + SB::kBytes);
     const uint32_t lds0 = lds_addr(lds);
     const int steps_k = (p.K + BK - 1) / BK, steps = steps_k * p.n_seg;
-    const int s_begin = (int)((int64_t)steps * blockIdx.y / p.slices), s_end = (int)((int64_t)steps * (blockIdx.y + 1) / p.slices);
+    const int s_begin = (int)((int64_t)steps * t.slice / p.slices), s_end = (int)((int64_t)steps * (t.slice + 1) / p.slices);
     const int64_t a_step = AKS ? BK * p.lda * 2 : BK * 2, b_step = BKS ? BK * p.ldb * 2 : BK * 2;
     const int64_t a_tile = AKS ? i0 * 2 : i0 * p.lda * 2, b_tile = BKS ? (int64_t)j0 * 2 : (int64_t)j0 * p.ldb * 2;
     int sg = s_begin / (steps_k ? steps_k : 1), kk = s_begin - sg * steps_k;       // the next request's segment and step, and its operands' addresses
@@ -411,8 +414,8 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_rows_gemm(const Args p) {
             const int64_t i = i0 + (wi * MT + m) * 16 + li;
             if (i >= p.I) continue;
             using O = typename std::conditional<EPI == EPI_PARTIAL, float, U>::type;
-            O *row = (O *)p.out[blockIdx.z] + (EPI == EPI_PARTIAL ? (int64_t)blockIdx.y * p.slice_stride : 0) + i * p.ldo;
-            const bool wide = p.ldo % 4 == 0 && (uintptr_t)p.out[blockIdx.z] % (4 * sizeof(O)) == 0;
+            O *row = (O *)p.out[t.problem] + (EPI == EPI_PARTIAL ? (int64_t)t.slice * p.slice_stride : 0) + i * p.ldo;
+            const bool wide = p.ldo % 4 == 0 && (uintptr_t)p.out[t.problem] % (4 * sizeof(O)) == 0;
 #pragma unroll
             for (int n = 0; n < NT; n++) {
                 const int j = j0 + (wj * NT + n) * 16 + lq * 4;
@@ -516,7 +519,8 @@ inline int launch_tile(Args p, int problems, hipStream_t s) {
     // the gate epilogues also write the padding columns up to ldh (< J + 8)
     const int64_t cols = EPI == EPI_GATE || EPI == EPI_GATE_BWD ? p.ldh : p.J;
     const int64_t ti = (p.I + BM - 1) / BM, tj = (cols + TJ - 1) / TJ;
-    if (ti * tj > kMaxGrid / (64 * WI * WJ) || p.slices > 65535) return HS_ERR_ARG;
+    if (ti * tj > kMaxGrid / (64 * WI * WJ) / problems / p.slices) return HS_ERR_ARG;
+    p.problems = p.slices > 1 ? problems : 1;
     p.tiles_i = (int)ti;
     p.tiles_j = (int)tj;
     if constexpr (planes<U>() != P) as_segments(p);
@@ -524,7 +528,7 @@ inline int launch_tile(Args p, int problems, hipStream_t s) {
     static hsLdsAttrOnce attr;
     const void *fn = (const void *)k_rows_gemm<T, U, P, BUFS, BM, BN, WI, WJ, AKS, BKS, EPI>;
     attr.set(fn, lds);
-    k_rows_gemm<T, U, P, BUFS, BM, BN, WI, WJ, AKS, BKS, EPI><<<dim3((unsigned)(ti * tj), (unsigned)p.slices, (unsigned)problems), 64 * WI * WJ, lds, s>>>(p);
+    k_rows_gemm<T, U, P, BUFS, BM, BN, WI, WJ, AKS, BKS, EPI><<<dim3((unsigned)(ti * tj * p.problems * p.slices), (unsigned)(problems / p.problems)), 64 * WI * WJ, lds, s>>>(p);
     return hipGetLastError() == hipSuccess ? HS_OK : HS_ERR_LAUNCH;
 }
 
@@ -545,7 +549,7 @@ __global__ __launch_bounds__(256) void k_gate_bwd(const Args p) {
     constexpr uint32_t kBuf = SA::kBytes + S1::kBytes;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wi = wave / WJ, wj = wave % WJ;
-    const TilePlace t = tile_place(p.tiles_i, p.tiles_j);
+    const TilePlace t = tile_place(p.tiles_i, p.tiles_j, 1, 1);
     const int64_t i0 = (int64_t)t.i * BM;
     const int j0 = t.j * TJ;
     SA sx, sg;
