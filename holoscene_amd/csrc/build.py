@@ -1,4 +1,5 @@
-"""Build libholoscene_hip.so for gfx950 in-tree (hipcc cross-compiles without a GPU).
+"""Build libholoscene_hip.so for gfx950 in-tree (hipcc cross-compiles without a GPU), and _row_autograd.so, the autograd nodes of the row operators
+(host code against PyTorch's C++ interface).
 
     python -m holoscene_amd.csrc.build [--force]
 
@@ -9,10 +10,12 @@ import glob
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(os.path.dirname(HERE))
 LIB = os.path.join(HERE, "libholoscene_hip.so")
+NODES = os.path.join(HERE, "_row_autograd.so")
 ARCH = "gfx950"
 # -ffp-contract=off: the encoder must round exactly like the CPU oracle (no fused multiply-adds).
 # -packed-fp32-ops: no packed fp32 instructions (v_pk_add / mul / fma_f32), some forms of which have given wrong results on this hardware;
@@ -26,11 +29,20 @@ def sources():
     return sorted(glob.glob(os.path.join(HERE, "*.hip")))
 
 
+def _nodes_command():
+    import torch
+    base = os.path.dirname(torch.__file__)
+    include = [os.path.join(base, "include"), os.path.join(base, "include", "torch", "csrc", "api", "include"), "/opt/rocm/include", sysconfig.get_paths()["include"]]
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-DUSE_ROCM=1", "-D__HIP_PLATFORM_AMD__=1", "-DTORCH_API_INCLUDE_EXTENSION_H",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", os.path.join(ROOT, "include"), *[f for p in include for f in ("-isystem", p)],
+            os.path.join(HERE, "row_autograd.cpp"), "-o", NODES, "-L", os.path.join(base, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+
+
 def _stale():
-    if not os.path.exists(LIB):
+    if not os.path.exists(LIB) or not os.path.exists(NODES):
         return True
-    t = os.path.getmtime(LIB)
-    deps = sources() + glob.glob(os.path.join(HERE, "*.h")) + glob.glob(os.path.join(ROOT, "include", "*.h")) + [__file__]
+    t = min(os.path.getmtime(LIB), os.path.getmtime(NODES))
+    deps = sources() + [os.path.join(HERE, "row_autograd.cpp")] + glob.glob(os.path.join(HERE, "*.h")) + glob.glob(os.path.join(ROOT, "include", "*.h")) + [__file__]
     return any(os.path.getmtime(p) > t for p in deps)
 
 
@@ -45,6 +57,11 @@ def build(force=False, verbose=False, variant=None, extra_flags=()):
     lib = LIB if variant is None else os.path.join(HERE, f"libholoscene_hip_{variant}.so")
     objdir = HERE if variant is None else os.path.join(HERE, f"obj_{variant}")
     os.makedirs(objdir, exist_ok=True)
+    if variant is None:
+        cmd = _nodes_command()
+        if verbose:
+            print(" ".join(cmd))
+        procs.append(("row_autograd.cpp", subprocess.Popen(cmd)))
     for src in sources():
         obj = os.path.join(objdir, os.path.basename(src)[:-4] + ".o")
         objs.append(obj)
@@ -54,7 +71,7 @@ def build(force=False, verbose=False, variant=None, extra_flags=()):
         procs.append((src, subprocess.Popen(cmd)))
     for src, p in procs:
         if p.wait() != 0:
-            raise RuntimeError(f"hipcc failed on {src}")
+            raise RuntimeError(f"compiler failed on {src}")
     cmd = [hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", lib, *objs]
     subprocess.run(cmd, check=True)
     return lib

@@ -9,6 +9,8 @@ missing library, a CPU tensor or a non-fp32 tensor raises ``RuntimeError`` (the 
 raises the same type from TORCH_CHECK, hashencoder.cu:16-19).
 """
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 
 import torch
@@ -99,12 +101,6 @@ class hsDrawSched(ctypes.Structure):
                 ("counter_base", ctypes.c_uint64), ("n_sched", ctypes.c_int32), ("n_frames", ctypes.c_int32)]
 
 
-class hsGatedMlp(ctypes.Structure):
-    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "w_gate", "w_up", "w_down")] + [(n, ctypes.c_int64) for n in ("ldx", "ld_gate", "ld_up", "ld_down", "rows", "dim", "hidden")]
-                + [("dtype", ctypes.c_int32), ("activation", ctypes.c_int32), ("y", ctypes.c_void_p), ("saved", ctypes.c_void_p), ("grad", ctypes.c_void_p),
-                   ("ld_grad", ctypes.c_int64)] + [(n, ctypes.c_void_p) for n in ("gx", "gw_gate", "gw_up", "gw_down", "ws")] + [("ws_bytes", ctypes.c_int64)])
-
-
 ABI_VERSION = 10
 
 # Small zero-initialised accumulators (bias-gradient sums the backward kernels add to by atomics): slices of a pool the optimiser zeroes
@@ -151,13 +147,9 @@ def _gate(gate):
 
 
 _lib = None
+_ROW_ENTRIES = ("hs_embed_fwd", "hs_embed_bwd_ws_bytes", "hs_embed_bwd", "hs_dropout_rows", "hs_gated_mlp_saved_bytes", "hs_gated_mlp_fwd_ws_bytes", "hs_gated_mlp_bwd_ws_bytes",
+                "hs_gated_mlp_fwd", "hs_gated_mlp_bwd")
 _ROW_BYTES = ("hs_embed_bwd_ws_bytes", "hs_gated_mlp_saved_bytes", "hs_gated_mlp_fwd_ws_bytes", "hs_gated_mlp_bwd_ws_bytes")      # sizes, or a negative error
-_p, _i, _l, _f = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
-# (declared once: a call then takes plain integers -- the smallest calls are bound by the host)
-_ROW_ARGTYPES = {"hs_embed_fwd": (_p, _i, _p, _l, _p, _l, _l, _l, _f, _i, _i, _p), "hs_embed_bwd_ws_bytes": (_l, _l, _l),
-                 "hs_embed_bwd": (_p, _i, _p, _l, _p, _l, _l, _l, _f, _l, _i, _i, _p, _l, _p), "hs_dropout_rows": (_p, _p, _p, _l, _i, _i, _p, _p),
-                 "hs_gated_mlp_saved_bytes": (_p,), "hs_gated_mlp_fwd_ws_bytes": (_p,), "hs_gated_mlp_bwd_ws_bytes": (_p,), "hs_gated_mlp_fwd": (_p, _p), "hs_gated_mlp_bwd": (_p, _p)}
-ROW_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}        # HS_F32 / HS_BF16 / HS_F16: section 10 (row operators)
 ROW_ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "sigmoid": 3, "relu": 4}       # HS_ACT_*
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}  # HS_F32 / HS_BF16
 
@@ -174,8 +166,6 @@ def load_library():
         for name in dir_symbols():
             if name != "hs_target_arch":
                 getattr(_lib, name).restype = ctypes.c_int64 if name in _ROW_BYTES else ctypes.c_int
-        for name, types in _ROW_ARGTYPES.items():
-            getattr(_lib, name).argtypes = types
         if _lib.hs_abi_version() != ABI_VERSION:
             raise RuntimeError(f"{LIB_PATH}: ABI version {_lib.hs_abi_version()}, this package needs {ABI_VERSION} -- rebuild "
                                "(python -m holoscene_amd.csrc.build)")
@@ -219,13 +209,23 @@ def _stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-def _row_stream(t):
-    """The current stream of t's device, as an integer (the row operators' calls).  torch.cuda.current_stream builds a Stream object: 2 us on the calling
-    thread and 8 on autograd's, of 10 us that such a call takes in all."""
-    return _RAW_STREAM(t.device.index) if _RAW_STREAM is not None else torch.cuda.current_stream(t.device).cuda_stream
+_row_autograd = None
 
 
-_RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+def row_autograd():
+    """The row operators' autograd nodes (csrc/row_autograd.cpp), bound to the loaded library."""
+    global _row_autograd
+    if _row_autograd is None:
+        lib = load_library()
+        path = os.path.join(_CSRC, "_row_autograd.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"{path} is missing: run `python -m holoscene_amd.csrc.build`. There is no other path for the row operators.")
+        loader = importlib.machinery.ExtensionFileLoader("_row_autograd", path)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_row_autograd", loader))
+        loader.exec_module(module)
+        module.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _ROW_ENTRIES})
+        _row_autograd = module
+    return _row_autograd
 
 
 SCHEDULE = int(os.environ.get("HOLOSCENE_HASH_SCHEDULE", "1"))
@@ -1606,75 +1606,6 @@ class _HipBackend:
         lib = load_library()
         _check(lib.hs_loss_eikonal(_dev(g1, "g1"), _dev(g2, "g2"), ctypes.c_int64(g1.shape[0]), ctypes.c_float(w_eik), ctypes.c_float(w_smooth),
                                    _dev(acc2, "acc2"), _dev(d_g1, "d_g1"), _dev(d_g2, "d_g2"), _stream()), "hs_loss_eikonal")
-
-
-    # ---- row operators (include/holoscene_hip.h section 10).  Callers (model/row_ops.py) have checked shapes, types and devices and made the
-    # tensors' device current; rows may be strided, elements of a row are consecutive.
-    @staticmethod
-    def _ld(t):
-        """Row distance of a 2-D tensor; a matrix of one row (or none) may carry any stride."""
-        return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-    @classmethod
-    def embed_fwd(cls, indices, table, out, scale):
-        lib = load_library()
-        V, D = table.shape
-        _check(lib.hs_embed_fwd(indices.data_ptr(), indices.element_size(), table.data_ptr(), cls._ld(table), out.data_ptr(), indices.numel(), V, D, scale,
-                                ROW_DTYPES[table.dtype], ROW_DTYPES[out.dtype], _row_stream(out)), "hs_embed_fwd")
-
-    @classmethod
-    def embed_bwd(cls, indices, grad, grad_table, scale, padding):
-        lib = load_library()
-        n, (V, D) = indices.numel(), grad_table.shape
-        nbytes = lib.hs_embed_bwd_ws_bytes(n, V, D)
-        _check(min(nbytes, 0), "hs_embed_bwd")
-        ws = torch.empty(nbytes, device=grad.device, dtype=torch.uint8)
-        _check(lib.hs_embed_bwd(indices.data_ptr(), indices.element_size(), grad.data_ptr(), cls._ld(grad), grad_table.data_ptr(), n, V, D, scale, padding,
-                                ROW_DTYPES[grad.dtype], ROW_DTYPES[grad_table.dtype], ws.data_ptr(), nbytes, _row_stream(grad)), "hs_embed_bwd")
-
-    @staticmethod
-    def dropout_rows(x, residual, y, drop, rng):
-        _check(load_library().hs_dropout_rows(x.data_ptr(), None if residual is None else residual.data_ptr(), y.data_ptr(), x.numel(), ROW_DTYPES[x.dtype], drop,
-                                              rng.data_ptr(), _row_stream(x)), "hs_dropout_rows")
-
-    @staticmethod
-    def _gated_args(x, w_gate, w_up, w_down, activation):
-        rows, dim = x.shape
-        hidden = w_gate.shape[0]
-        return hsGatedMlp(x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), x.stride(0) if rows > 1 else dim, w_gate.stride(0) if hidden > 1 else dim,
-                          w_up.stride(0) if hidden > 1 else dim, w_down.stride(0) if dim > 1 else hidden, rows, dim, hidden, ROW_DTYPES[x.dtype], ROW_ACTIVATIONS[activation])
-
-    @staticmethod
-    def _gated_call(a, call, nbytes, x, fn):
-        _check(min(nbytes, 0), fn)
-        if nbytes:
-            ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
-            a.ws, a.ws_bytes = ws.data_ptr(), nbytes
-        _check(call(ctypes.byref(a), _row_stream(x)), fn)
-
-    @classmethod
-    def gated_mlp_fwd(cls, x, w_gate, w_up, w_down, activation, y, save):
-        """save: also returns the buffer that gated_mlp_bwd reads."""
-        lib = load_library()
-        a = cls._gated_args(x, w_gate, w_up, w_down, activation)
-        saved = None
-        if save:
-            nbytes = lib.hs_gated_mlp_saved_bytes(ctypes.byref(a))
-            _check(min(nbytes, 0), "hs_gated_mlp_fwd")
-            saved = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
-            a.saved = saved.data_ptr()
-        a.y = y.data_ptr()
-        cls._gated_call(a, lib.hs_gated_mlp_fwd, lib.hs_gated_mlp_fwd_ws_bytes(ctypes.byref(a)), x, "hs_gated_mlp_fwd")
-        return saved
-
-    @classmethod
-    def gated_mlp_bwd(cls, grad, x, w_gate, w_up, w_down, activation, saved, gx, gw_gate, gw_up, gw_down):
-        """gx, gw_*: written, None = not wanted."""
-        lib = load_library()
-        a = cls._gated_args(x, w_gate, w_up, w_down, activation)
-        a.grad, a.ld_grad, a.saved = grad.data_ptr(), cls._ld(grad), saved.data_ptr()
-        a.gx, a.gw_gate, a.gw_up, a.gw_down = (None if t is None else t.data_ptr() for t in (gx, gw_gate, gw_up, gw_down))
-        cls._gated_call(a, lib.hs_gated_mlp_bwd, lib.hs_gated_mlp_bwd_ws_bytes(ctypes.byref(a)), x, "hs_gated_mlp_bwd")
 
 
 class hsAdamState(ctypes.Structure):

@@ -917,6 +917,7 @@ int hs_dropout_rows(const void *x, const void *residual, void *y, int64_t n, int
 #define HS_ACT_GELU_TANH 2
 #define HS_ACT_SIGMOID 3
 #define HS_ACT_RELU 4
+#define HS_GATED_MLP_MAX (1 << 21)      /* the largest dim and hidden */
 typedef struct hsGatedMlp {
     const void *x, *w_gate, *w_up, *w_down;
     int64_t ldx, ld_gate, ld_up, ld_down;       /* in elements */

@@ -54,8 +54,14 @@ def test_dropout_refusals():
     assert call(x=None) == -3 and call(y=None) == -3 and call(rng=None) == -3
 
 
+class hsGatedMlp(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "w_gate", "w_up", "w_down")] + [(n, ctypes.c_int64) for n in ("ldx", "ld_gate", "ld_up", "ld_down", "rows", "dim", "hidden")]
+                + [("dtype", ctypes.c_int32), ("activation", ctypes.c_int32), ("y", ctypes.c_void_p), ("saved", ctypes.c_void_p), ("grad", ctypes.c_void_p),
+                   ("ld_grad", ctypes.c_int64)] + [(n, ctypes.c_void_p) for n in ("gx", "gw_gate", "gw_up", "gw_down", "ws")] + [("ws_bytes", ctypes.c_int64)])
+
+
 def gated(**kw):
-    a = backend.hsGatedMlp(x=256, w_gate=256, w_up=256, w_down=256, ldx=16, ld_gate=16, ld_up=16, ld_down=32, rows=4, dim=16, hidden=32, dtype=1, activation=0, y=256,
+    a = hsGatedMlp(x=256, w_gate=256, w_up=256, w_down=256, ldx=16, ld_gate=16, ld_up=16, ld_down=32, rows=4, dim=16, hidden=32, dtype=1, activation=0, y=256,
                            saved=256, grad=256, ld_grad=16, ws=256, ws_bytes=1 << 40)
     for k, v in kw.items():
         setattr(a, k, v)

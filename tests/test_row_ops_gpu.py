@@ -446,6 +446,38 @@ def test_gated_refusals():
         g.sum().backward()
 
 
+@pytest.mark.parametrize("lead", [(6,), (2, 3)])
+def test_saved_operands_are_guarded(lead):
+    """A second backward pass, or one after an operand has been written, is refused as for torch's own operators."""
+    x, wg, wu, wd, _ = gated_inputs(6, 8, 16, torch.float32)
+    x, leaf = x.view(*lead, 8), wg.clone().requires_grad_()
+    y = ops().gated_mlp_rows(x, leaf, wu, wd)
+    y.sum().backward()
+    with pytest.raises(RuntimeError, match="second time"):
+        y.sum().backward()
+    for t in (x, wu):
+        y = ops().gated_mlp_rows(x, leaf, wu, wd)
+        t.mul_(2)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+    idx, table = torch.arange(4, device=DEV), torch.randn(5, 8, device=DEV, requires_grad=True)
+    out = ops().embedding_rows(idx, table)
+    idx += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+
+
+def test_second_derivatives_are_refused():
+    x, wg, wu, wd, gy = gated_inputs(6, 8, 16, torch.float32)
+    rng, idx = torch.tensor([3, 4], device=DEV), torch.arange(6, device=DEV)
+    for f, leaf in ((lambda t: ops().gated_mlp_rows(t, wg, wu, wd), x), (lambda t: ops().dropout_rows(t, 0.5, rng), x), (lambda t: ops().dropout_rows(x, 0.5, rng, residual=t), x),
+                    (lambda t: ops().embedding_rows(idx, t), x)):
+        leaf, g = leaf.clone().requires_grad_(), gy.clone().requires_grad_()
+        first, = torch.autograd.grad(f(leaf), leaf, g, create_graph=True)
+        with pytest.raises(RuntimeError, match="cannot be differentiated again"):
+            first.sum().backward()
+
+
 # ------------------------------------------------------------------------------------------------ together
 def _chain(idx, table, ws, rng, gy):
     """Codes -> dropout -> gated block -> dropout + residual, and all gradients."""
@@ -478,7 +510,7 @@ def test_chain_matches_its_definition(dtype):
     # every tensor between two operators is rounded to the type (5 of them forward, 5 backward), each rounding relative to its own size; sums over 72 or 200
     # such terms of either sign grow like their norm.  Norms: 10 roundings of half(t) each, and the fp32 arithmetic (2^-18 covers sums of 200 terms)
     for g, w, what in zip(got, want, ("y", "table", "w_gate", "w_up", "w_down")):
-        rel = float((g.double() - w).norm() / w.norm())
+        rel = float((g.detach().double() - w).norm() / w.norm())
         assert rel < 10 * half(dtype) + 2.0 ** -18, (what, rel)
 
 
