@@ -13,6 +13,10 @@
 //           through LDS in a fixed order), then the short ones (a wave each), then the zeros of the rows without one: the reads are over before the stores
 //           of the zeros, most of the bytes, fill the memory's queues.
 // fp32 sums: 32 terms per chunk, then the partials; the last operation rounds to the table's type.
+//
+// Measured: 16 384 zipf-distributed rows of 2 048 bf16, table of 50 021: lookup 23.5 us (134 MB, 5.7 TB/s); gradient: sort 2 x (2.8 + 7.9), chunks and runs 12.6,
+// rows 61 (205 MB of table written, 67 MB of gradient read: 54 us at the rate of a large copy).  131 072 rows of 32 fp32, 8 indices among 1 024: lookup 7.2, sort
+// 4.8 + 19.0 (one pass), chunks 10.7, rows 4.3.  The lookup and the rows are bound by memory, the sort by its chains of dependent LDS operations and launches.
 #include "holoscene_hip.h"
 #include "launch_util.h"
 #include "row_types.h"
@@ -59,7 +63,7 @@ template <typename I> __device__ __forceinline__ uint32_t sort_key(const I *__re
 
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
 constexpr int kOneMax = 4096, kOneDigit = 8;        // the one-workgroup sort (16 384 pairs in it: 37 us, bound by one CU's vector instructions; over 16 CUs 24)
-constexpr int kMultiDigit = 9, kOnlyDigit = 11;    // the multi-block sort: tiles of 1, 2 or 4 pairs per thread; up to 11 bits in a single pass
+constexpr int kMultiDigit = 9, kOnlyDigit = 11;    // the multi-block sort: tiles of 1, 2 or 4 pairs per thread; up to 11 bits in a single pass (131 072 pairs: 23.8 us, in two of 9 bits 24.4 and two launches more)
 constexpr int kMaxBlocks = 64;                      // workgroups of the multi-block sort (each adds up all their histograms)
 
 // Lanes of this wave whose digit equals mine, among those with `on`.  (Per bit: a mask of the bit, a ballot, and the lanes that agree with it.)

@@ -31,7 +31,8 @@ struct Arena {
 inline int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
 
 // Operands that are not in that form, copied into it: src [rows, cols] -> dst [planes][rows][8 chunks], zeros behind cols.  All of a pass in one launch (fp32
-// has every operand in it; a launch each cost more than the copies).
+// has every operand in it; a launch each cost more than the copies).  Bound by memory and its launch: 1 021 x 1 000 x 2 730 f16 4.7 us, the fp32 operands of a pass of
+// 4 096 x 256 x 683 6.0 and 7.0 us.
 constexpr int kMaxPack = 6;
 struct PackJob { const void *src; void *dst; int64_t ld, rows, cols, chunks, plane; unsigned first; };      // first: the job's first workgroup
 struct PackJobs { PackJob j[kMaxPack]; int n; unsigned blocks; };
@@ -69,7 +70,7 @@ __global__ __launch_bounds__(256) void k_rows_pack(const PackJobs jobs) {
 }
 
 // out = sum of the slices' partial results, in the order of the slices: all results of a pass that were cut into slices, in one launch at its end (a launch
-// each behind its product: 1 021 x 1 000 x 2 730 step, host 15 us more).
+// each behind its product: 1 021 x 1 000 x 2 730 step, host 15 us more).  Bound by memory: 21 us for 32 slices of 2 x 1 024 x 256 and 32 of 256 x 1 024.
 constexpr int kMaxReduce = 4;
 struct ReduceJob { const float *parts; void *out; int64_t n, stride; int slices; unsigned first; };
 struct ReduceJobs { ReduceJob j[kMaxReduce]; int n; unsigned blocks; };
@@ -99,8 +100,8 @@ __global__ __launch_bounds__(256) void k_rows_reduce(const ReduceJobs jobs) {
 // a lone workgroup on a CU waits for its requests (`first`), every further one of the `fit` that LDS admits adds its own work (`more`).  The 256 x 256
 // tile reads the least per product and has the highest rate (1.2 PFLOP/s against 0.93 and 0.6); with few tiles of the result the smaller ones, or
 // slices whose fp32 partial results are added up by another launch, fill the device.  E.g. 1 021 x 1 000 over K = 5 460: 52 us in 64 x 64 tiles,
-// 72 in 128 x 128, 29 in 128 x 128 and four slices, 22 with the requests three steps ahead (eight waves, four buffers, so one workgroup a CU: with
-// many tiles two workgroups of two buffers are faster, 228 us against 343 for G and U of 131 072 x 256 x 1 024).  fp32 (six plane products): the large tile in
+// 72 in 128 x 128, 29 in 128 x 128 and four slices, 21 with the requests three steps ahead (eight waves, four buffers, so one workgroup a CU: with
+// many tiles two workgroups of two buffers are faster, 231 us against 337 for G and U of 131 072 x 256 x 1 024, and 256 x 256 tiles 217).  fp32 (six plane products): the large tile in
 // six passes, 200 TFLOP/s; small tiles with the planes in LDS, one workgroup a CU.
 struct Plan { int tile, slices; };
 struct TileCost { int rows, cols, fit; float first, more; };

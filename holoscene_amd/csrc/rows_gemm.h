@@ -16,6 +16,11 @@
 // ds_read_b64_tr_b16.  What lies outside an operand is requested at an address beyond the buffer descriptor, which reads as zero.
 //
 // The tile's orientation in the matrix instruction is C^T (its rows = J): a lane then holds four consecutive columns of one row of C.
+//
+// Measured, 8 192 x 4 096 x 12 288 bf16 (256 x 256 tiles): gate and up 1.40 ms (1.18 PFLOP/s, with act(G) U and G, U written), down 0.67 (1.23), gx 1.30 (1.27), gWg and
+// gWu 1.35 (1.22), gWd 0.68 (1.21); the library's product of 8 192^3 reaches 1.40.  The matrix cores are busy 54 to 63 % of the cycles, the LDS 23 %, and the
+// waves wait 30 % of theirs: what is left is the meeting of the waves at every step of 64.  At 131 072 x 256 x 1 024 a tile has four steps, and its beginning and end
+// are half of it: gate 217 us (0.63 PFLOP/s), down 82, gx 160, gWg and gWu 138, gWd 99.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -535,9 +540,9 @@ inline int launch_tile(Args p, int problems, hipStream_t s) {
 // ------------------------------------------------------------------------------------------------ gg and gu without G and U
 // gH = gy Wd, G = x Wg^T, U = x Wu^T over the same K = D in one workgroup: 4 D operations an element of H more than reading G and U back, 16 bytes less written
 // and read (fp32: 16-bit G and U would add two roundings to every gradient).  Tile 128 x 64 of each of the three, four waves, two workgroups a CU
-// (fp32: plane products as segments).  Larger tiles read less and were slower: with K this short half the time is the beginnings and the ends of tiles, and a second
-// workgroup is what fills them (131 072 x 256 x 1 024: 383 us; 128 x 128 435, 256 x 64 435, 256 x 128 413; 24 % of the cycles in the matrix cores, 37 % in
-// the vector units).
+// (fp32: plane products as segments).  131 072 x 256 x 1 024: 370 us (0.56 PFLOP/s; matrix cores 25 % of the cycles, vector units 43 %, LDS 24 %; without the
+// stores 321).  Larger tiles read less and were slower: with K this short half the time is the beginnings and the ends of tiles, and a second workgroup
+// is what fills them (128 x 128 435, 256 x 64 435, 256 x 128 413, 64 x 64 423; eight waves 366, no gain for twice the LDS reads).
 constexpr int kAgainM = 128, kAgainJ = 64;
 
 template <typename T, typename U>
