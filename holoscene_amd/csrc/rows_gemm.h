@@ -96,7 +96,8 @@ template <int ACT, bool D> __device__ __forceinline__ float activation(float g, 
         return g * c;
     } else {                                            // HS_ACT_GELU_TANH: 2 sqrt(2 / pi) (g + 0.044715 g^3)
         const float s = logistic(1.5957691216057308f * (g + 0.044715f * g * g * g));
-        if constexpr (D) d = s + g * s * (1.f - s) * 1.5957691216057308f * (1.f + 0.134145f * g * g);
+        const float t = s * (1.f - s);
+        if constexpr (D) d = s + (t > 0.f ? g * t * 1.5957691216057308f * (1.f + 0.134145f * g * g) : 0.f);        // (t = 0: g^2 may be infinite)
         return g * s;
     }
 }

@@ -39,7 +39,8 @@ def gated_mlp_rows(x, w_gate, w_up, w_down, activation="silu"):
     dim and hidden are at most 2^21.  activation: "silu", "gelu" (g Phi(g)), "gelu_tanh" (its tanh form), "sigmoid", "relu".  float32 operands are
     multiplied as three bf16 planes each (24 bits, as linear_rows under HOLOSCENE_FP32_GEMM=split3; an infinity among them gives NaN).  Rows may be
     strided; 16-bit operands whose rows are not 16-byte aligned are copied once per call.  The forward keeps the gated product for the backward pass, and both
-    projections in fp32 where reading them back costs less than computing them again (dim > 768, in float32 > 128)."""
+    projections in fp32 where reading them back costs less than computing them again (dim > 768, in float32 > 128).  The gated product and its two
+    gradients are rounded to x's type between the products: in float16 they are infinite beyond 65 504."""
     for t, name in ((x, "x"), (w_gate, "w_gate"), (w_up, "w_up"), (w_down, "w_down")):
         _check_tensor(t, name)
     if activation not in _be.ROW_ACTIVATIONS:

@@ -431,6 +431,76 @@ def test_gated_not_finite_stays_in_its_row():
         assert torch.equal(y[rows], clean[rows]) and bool(torch.isnan(y[7]).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("act", ACTS)
+def test_gated_far_preactivations(act, dtype):
+    """Preactivations whose square passes the largest float: the functions and their slopes have reached their limits."""
+    for rows, D in ((3, 8), (70, 8), (70, 1000)):           # few rows; slopes from G computed again, and from G kept
+        x = torch.zeros(rows, D, device=DEV, dtype=dtype)
+        x[:, 0] = 1
+        wg, wu, wd = (torch.zeros(s, device=DEV, dtype=dtype) for s in ((16, D), (16, D), (D, 16)))
+        wg[:, 0] = torch.tensor([1e20, -1e20, 1.0, -1.0]).repeat(4).to(dtype).to(DEV)
+        wu[:, 0] = 0.5
+        wd[0, :] = 2.0 ** -60
+        leaves = [t.requires_grad_() for t in (x, wg, wu, wd)]
+        y = ops().gated_mlp_rows(*leaves, activation=act)
+        grads = torch.autograd.grad(y, leaves, torch.ones_like(y))
+        assert all(bool(torch.isfinite(t).all()) for t in (y, *grads)), (rows, D)
+        slope = {"sigmoid": [0.0, 0.0], "relu": [1.0, 0.0]}.get(act, [1.0, 0.0])
+        want = torch.tensor(slope, dtype=torch.float64) * 0.5 * 2.0 ** -60 * rows
+        within(grads[1][:2, 0].cpu(), want, want * (rows + 8) * half(dtype), "slope")
+
+
+def test_embedding_gradient_ignores_what_takes_none():
+    """Not a number in the gradient of padded and outside positions."""
+    for n in (100, 5000, 40000):
+        idx = torch.arange(n, device=DEV) % 7 - 1
+        table, g = torch.randn(5, 40, device=DEV).requires_grad_(), torch.ones(n, 40, device=DEV)
+        g[(idx < 0) | (idx > 4) | (idx == 2)] = float("nan")
+        gt, = torch.autograd.grad(ops().embedding_rows(idx, table, padding_idx=2), table, g)
+        want = torch.bincount(idx[(idx >= 0) & (idx < 5) & (idx != 2)], minlength=5).float()[:, None].expand(5, 40)
+        assert torch.equal(gt, want)
+
+
+@pytest.mark.parametrize("tied", [(1, 2), (0, 0)])
+def test_gated_shared_operands(tied):
+    """One tensor as both projections; x as its own residual in dropout."""
+    x, wg, wu, wd, gy = gated_inputs(70, 64, 96, torch.float32)
+    if tied == (1, 2):
+        w = wg.clone().requires_grad_()
+        g, = torch.autograd.grad(ops().gated_mlp_rows(x, w, w, wd), w, gy)
+        a, b = wg.clone().requires_grad_(), wg.clone().requires_grad_()
+        ga, gb = torch.autograd.grad(ops().gated_mlp_rows(x, a, b, wd), (a, b), gy)
+        assert torch.equal(g, ga + gb)
+    else:
+        t, rng = x.clone().requires_grad_(), torch.tensor([1, 2], device=DEV)
+        g, = torch.autograd.grad(ops().dropout_rows(t, 0.4, rng, residual=t), t, gy)
+        assert torch.equal(g, ops().dropout_rows(gy, 0.4, rng) + gy)
+
+
+def test_calls_from_two_threads():
+    """Two host threads, a stream each: nothing is shared between calls."""
+    import threading
+    inputs = [_chain_inputs(torch.bfloat16, n=200 + 37 * k, seed=k) for k in range(2)]
+    want = [_chain(*i) for i in inputs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = _chain(*inputs[k])
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[k])):
+                    bad.append(k)
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
 def test_gated_refusals():
     x, wg, wu, wd, _ = gated_inputs(4, 8, 16, torch.float32)
     f = ops().gated_mlp_rows
