@@ -317,12 +317,19 @@ __device__ __forceinline__ void add_entries(int64_t first, int64_t end, int step
     }
 }
 
-// first place in keys[0, n) that is >= v
+// First place in keys[0, n) that is >= v, by eights: seven loads that do not depend on each other a step, so the chain has a third of a bisection's loads.
 __device__ __forceinline__ int64_t lower_bound(const uint32_t *__restrict__ keys, int64_t n, uint32_t v) {
-    int64_t lo = 0, hi = n;
-    while (lo < hi) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (keys[mid] < v) lo = mid + 1; else hi = mid;
+    int64_t lo = 0, len = n;                    // the answer lies in [lo, lo + len]
+    while (len > 0) {
+        const int64_t step = len >= 8 ? len / 8 : 1;
+        int smaller = 0;
+#pragma unroll
+        for (int j = 1; j < 8; j++) {
+            const int64_t at = j * step <= len ? lo + j * step - 1 : lo + len - 1;
+            smaller += keys[at] < v && j * step <= len;
+        }
+        lo += smaller * step;
+        len = smaller == 7 ? len - 7 * step : step - 1;
     }
     return lo;
 }
