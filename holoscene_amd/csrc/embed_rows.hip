@@ -15,8 +15,8 @@
 // fp32 sums: 32 terms per chunk, then the partials; the last operation rounds to the table's type.
 //
 // Measured: 16 384 zipf-distributed rows of 2 048 bf16, table of 50 021: lookup 23.5 us (134 MB, 5.7 TB/s); gradient: sort 2 x (2.8 + 7.9), chunks and runs 12.6,
-// rows 61 (205 MB of table written, 67 MB of gradient read: 54 us at the rate of a large copy).  131 072 rows of 32 fp32, 8 indices among 1 024: lookup 7.2, sort
-// 4.8 + 19.0 (one pass), chunks 10.7, rows 4.3.  The lookup and the rows are bound by memory, the sort by its chains of dependent LDS operations and launches.
+// rows 59 (205 MB of table written, 67 MB of gradient read: 54 us at the rate of a large copy).  131 072 rows of 32 fp32, 8 indices among 1 024: lookup 7.2, sort
+// 4.8 + 19.0 (one pass), chunks 9.9, rows 4.5.  The lookup and the rows are bound by memory, the sort by its chains of dependent LDS operations and launches.
 #include "holoscene_hip.h"
 #include "launch_util.h"
 #include "row_types.h"
@@ -288,7 +288,7 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(const I *__restri
 
 // ------------------------------------------------------------------------------------------------ sums
 constexpr int kChunk = 32;
-constexpr int kShort = 8, kWide = 4;        // runs up to kShort entries are summed by one group of lanes, kWide * VEC columns a lane at a time
+constexpr int kShort = 8, kWide = 2;        // runs up to kShort entries are summed by one group of lanes, kWide * VEC columns a lane at a time
 constexpr int64_t kMaxGrid = 0xffffff;     // workgroups of 256 a launch takes: a grid has less than 2^32 threads
 constexpr int kLongGroups = 256, kShortGroups = 8192;            // workgroups (per block of columns; in all) that share the long and the short runs
 
@@ -423,7 +423,7 @@ __global__ __launch_bounds__(256) void k_embed_rows(const RunLists lists, const 
             if (col < D) {
                 // head and tail as one sequence, then the chunks
                 add_entries<4, T, VEC>(rs + slot, re - skip, slots, D - col, [&](int64_t j) { return grad + (int64_t)pos[j < head ? j : j + skip] * ldg + col; }, acc);
-                add_entries<8, float, VEC>(c_first + slot, c_last, slots, D - col, [&](int64_t c) { return partial + c * D + col; }, acc);
+                add_entries<4, float, VEC>(c_first + slot, c_last, slots, D - col, [&](int64_t c) { return partial + c * D + col; }, acc);
             }
 #pragma unroll
             for (int e = 0; e < VEC; e++) join[e * 256 + tid] = acc[e];
