@@ -2,7 +2,7 @@
 //     G = x Wg^T, U = x Wu^T, H = act(G) U (one launch), y = H Wd^T;
 //     gH = gy Wd, gg = gH U act'(G), gu = gH act(G) (one launch), gx = gg Wg + gu Wu, gWg = gg^T x, gWu = gu^T x (one launch), gWd = gy^T H.
 // Roundings besides the results' own: H, gg and gu to the operand type, because the matrix cores multiply 16-bit operands (fp32: as three bf16 planes,
-// 24 bits).  G and U are never rounded: the forward keeps them in fp32 for the backward pass, or the backward pass computes them again (k_gate_bwd) where that
+// 24 bits; few results: two planes, fine()).  G and U are never rounded: the forward keeps them in fp32 for the backward pass, or the backward pass computes them again (k_gate_bwd) where that
 // moves fewer bytes than it costs products.
 #pragma once
 #include "rows_gemm.h"
@@ -161,6 +161,15 @@ template <typename T, typename U> struct Block {
 
     void check(int r) { if (rc == HS_OK) rc = r; }
 
+    // H, gg and gu of the 16-bit types in two planes where a result has few elements: rounded once they bring as much error into a result as its own rounding, 1.4 times
+    // in all over many elements, but over few of them anything up to twice; in two planes nothing that shows.  The steps of the products that read them
+    // double, which so small ones do not feel (a step of 1 x 32 x 2 976 bf16 is bound by the host); 1 x 4 096 x 12 288, where reading the weights is all there is,
+    // would: down projection 25.1 -> 28.4 us.
+    static constexpr int64_t kFineResults = 2048;
+    bool fine() const { return sizeof(U) == 2 && (M < F ? M : F) * D <= kFineResults; }
+    int inner_planes() const { return fine() ? 2 : planes<U>(); }
+    template <typename O> static const void *plane1(const O &o) { return (const char *)o.p + o.plane * 2; }        // (of an operand in two planes of 16 bits)
+
     // The operand itself, or the copy of it that the next pack() makes.
     PackJobs jobs = {};
     Operand operand(const void *p, int64_t ld, int64_t rows, int64_t cols, bool force = false) {
@@ -203,7 +212,7 @@ template <typename T, typename U> struct Block {
         v.g = gu ? (float *)base : nullptr;
         v.u = gu ? (float *)(base + gu) : nullptr;
         v.h = Operand{base + 2 * gu, ldh, n};
-        v.bytes = 2 * gu + n * 2 * planes<U>();
+        v.bytes = 2 * gu + n * 2 * inner_planes();
         return v;
     }
 
@@ -211,17 +220,24 @@ template <typename T, typename U> struct Block {
         Saved sv = saved_in((char *)a.saved);
         if (!a.saved) {
             sv.g = sv.u = nullptr;
-            sv.h = Operand{ws.take(M * ldh * 2 * planes<U>()), ldh, M * ldh};
+            sv.h = Operand{ws.take(M * ldh * 2 * inner_planes()), ldh, M * ldh};
         }
         if (!run || rc != HS_OK) return;
         SmallArgs p = {};
         p.x = a.x; p.w = a.w_gate; p.w1 = a.w_up; p.ldx = a.ldx; p.ldw = a.ld_gate; p.ldw1 = a.ld_up; p.M = (int)M; p.N = (int)F; p.K = (int)D; p.act = a.activation;
         p.g = sv.g; p.u = sv.u; p.h = (void *)sv.h.p; p.ldh = ldh; p.plane = sv.h.plane;
-        check(launch_small<T, U, EPI_GATE>(p, s));
+        if constexpr (sizeof(U) == 2) {
+            if (fine()) check(launch_small<T, U, EPI_GATE, true>(p, s));
+            else check(launch_small<T, U, EPI_GATE, false>(p, s));
+        } else check(launch_small<T, U, EPI_GATE, false>(p, s));
         SmallArgs q = {};
         q.x = sv.h.p; q.w = q.w1 = a.w_down; q.ldx = ldh; q.ldw = q.ldw1 = a.ld_down; q.M = (int)M; q.N = (int)D; q.K = (int)F; q.plane = sv.h.plane;
         q.y = a.y; q.ldy = D;
-        if (rc == HS_OK) check(launch_small<T, U, EPI_STORE>(q, s));
+        if (rc != HS_OK) return;
+        if constexpr (sizeof(U) == 2) {
+            if (fine()) return check(launch_small<T, U, EPI_STORE, true>(q, s));
+        }
+        check(launch_small<T, U, EPI_STORE, false>(q, s));
     }
 
     void fwd() {
@@ -233,14 +249,22 @@ template <typename T, typename U> struct Block {
         Saved sv = saved_in((char *)a.saved);
         if (!a.saved) {
             sv.g = sv.u = nullptr;
-            sv.h = Operand{ws.take(M * ldh * 2 * planes<U>()), ldh, M * ldh};
+            sv.h = Operand{ws.take(M * ldh * 2 * inner_planes()), ldh, M * ldh};
         }
         pack();
         Args p = product(x, wg, M, F, D);
         p.seg[0][0].b1 = wu.p;
         p.g = sv.g; p.u = sv.u; p.h = (void *)sv.h.p; p.ldh = ldh; p.plane = sv.h.plane; p.act = a.activation;
-        if (run && rc == HS_OK) check(launch_product<T, U, false, false, EPI_GATE>(p, plan_product<U>(M, 2 * ldh, steps(D), 1, false).tile, 1, s));
+        if (run && rc == HS_OK) {
+            if (!fine()) check(launch_product<T, U, false, false, EPI_GATE>(p, plan_product<U>(M, 2 * ldh, steps(D), 1, false).tile, 1, s));
+            else if constexpr (sizeof(U) == 2) check(launch_tile<T, U, 1, 2, 64, 64, 2, 2, false, false, EPI_GATE_FINE>(p, 1, s));
+        }
         Args q = product(sv.h, wd, M, D, F);
+        if (fine()) {
+            q.seg[0][1] = q.seg[0][0];
+            q.seg[0][0].a = plane1(sv.h);        // (the smaller plane's product first)
+            q.n_seg = 2;
+        }
         result<false, false>(q, &a.y, 1);
         reduce();
     }
@@ -286,10 +310,18 @@ template <typename T, typename U> struct Block {
         check(hipGetLastError() == hipSuccess ? HS_OK : HS_ERR_LAUNCH);
     }
 
-    // C_z [I, J] = A_z^T B over the rows
-    void weight_gradient(const Operand *av, const Operand &b, void *const *out, int problems, int64_t I, int64_t J) {
+    // C_z [I, J] = A_z^T B over the rows; in_a: the two planes of fine() are A's, not B's
+    void weight_gradient(const Operand *av, const Operand &b, void *const *out, int problems, int64_t I, int64_t J, bool in_a) {
         Args p = product(av[0], b, I, J, M);
         if (problems == 2) p.seg[1][0] = Seg{av[1].p, b.p, nullptr};
+        if (fine()) {
+            for (int z = 0; z < problems; z++) {
+                p.seg[z][1] = p.seg[z][0];
+                if (in_a) p.seg[z][0].a = plane1(av[z]);
+                else p.seg[z][0].b = plane1(b);
+            }
+            p.n_seg = 2;
+        }
         result<true, true>(p, out, problems);
     }
 
@@ -304,7 +336,7 @@ template <typename T, typename U> struct Block {
         pack();
         if (inner) {
             const int64_t n = M * ldh;
-            const Operand gg{ws.take(n * 2 * planes<U>()), ldh, n}, gu{ws.take(n * 2 * planes<U>()), ldh, n};
+            const Operand gg{ws.take(n * 2 * inner_planes()), ldh, n}, gu{ws.take(n * 2 * inner_planes()), ldh, n};
             if (run && rc == HS_OK) {
                 Args p = again() ? product(x, wg, M, F, D) : product(gy, wd, M, F, D);
                 p.g = sv.g; p.u = sv.u; p.gg = (void *)gg.p; p.gu = (void *)gu.p; p.ldh = ldh; p.plane = n; p.act = a.activation;
@@ -312,24 +344,33 @@ template <typename T, typename U> struct Block {
                     p.seg[0][0].b1 = wu.p;
                     p.seg[1][0] = Seg{gy.p, wd.p, nullptr};
                     p.lda2 = gy.ld; p.ldb2 = wd.ld; p.plane_a2 = gy.plane * 2; p.plane_b2 = wd.plane * 2;
-                    check(launch_gate_bwd<T, U>(p, s));
-                } else {
+                    if (!fine()) check(launch_gate_bwd<T, U, false>(p, s));
+                    else if constexpr (sizeof(U) == 2) check(launch_gate_bwd<T, U, true>(p, s));
+                } else if (!fine()) {
                     check(launch_product<T, U, false, true, EPI_GATE_BWD>(p, plan_product<U>(M, ldh, steps(D), 1, false).tile, 1, s));
+                } else if constexpr (sizeof(U) == 2) {
+                    check(launch_tile<T, U, 1, 2, 64, 64, 2, 2, false, true, EPI_GATE_BWD_FINE>(p, 1, s));
                 }
             }
             if (a.gx) {
                 Args p = product(gg, wg, M, D, F);
                 p.seg[0][1] = Seg{gu.p, wu.p, nullptr};
                 p.n_seg = 2;
+                if (fine()) {
+                    for (int k = 0; k < 2; k++) p.seg[0][2 + k] = p.seg[0][k];
+                    p.seg[0][0].a = plane1(gg);
+                    p.seg[0][1].a = plane1(gu);
+                    p.n_seg = 4;
+                }
                 result<false, true>(p, &a.gx, 1);
             }
             if (xw) {
                 const Operand av[2] = {a.gw_gate ? gg : gu, gu};
                 void *const out[2] = {a.gw_gate ? a.gw_gate : a.gw_up, a.gw_up};
-                weight_gradient(av, x, out, a.gw_gate && a.gw_up ? 2 : 1, F, D);
+                weight_gradient(av, x, out, a.gw_gate && a.gw_up ? 2 : 1, F, D, true);
             }
         }
-        if (a.gw_down) weight_gradient(&gy, sv.h, &a.gw_down, 1, D, F);
+        if (a.gw_down) weight_gradient(&gy, sv.h, &a.gw_down, 1, D, F, false);
         reduce();
     }
 };

@@ -71,7 +71,10 @@ struct Args {
     int64_t lda2, ldb2, plane_a2, plane_b2;
 };
 
-enum { EPI_STORE = 0, EPI_PARTIAL = 1, EPI_GATE = 2, EPI_GATE_BWD = 3 };       // result; fp32 partial result; H (G, U); gg, gu from G, U
+// result; fp32 partial result; H (G, U); gg, gu from G, U; the last two with their results in two planes (16-bit types: fine() in gated_mlp.h)
+enum { EPI_STORE = 0, EPI_PARTIAL = 1, EPI_GATE = 2, EPI_GATE_BWD = 3, EPI_GATE_FINE = 4, EPI_GATE_BWD_FINE = 5 };
+constexpr bool gate_forward(int epi) { return epi == EPI_GATE || epi == EPI_GATE_FINE; }
+constexpr bool gate_backward(int epi) { return epi == EPI_GATE_BWD || epi == EPI_GATE_BWD_FINE; }
 
 // ------------------------------------------------------------------------------------------------ activations (fp32)
 // act(g) and, with D, act'(g).  The logistic function is v_exp_f32 and v_rcp_f32 (one step each): its error is |g| 2^-24 relative to s (1 - s), below the
@@ -150,6 +153,22 @@ struct F8 { float v[8]; };
 __device__ __forceinline__ F8 load8(const float *p) {
     const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
     return F8{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+}
+// four elements of an operand of a 16-bit type in two planes, v = p0 + p1 up to the square of the type's rounding; an infinity or NaN stays in plane 0 alone
+template <typename U> __device__ __forceinline__ void split2(float v, U (&p)[2]) {
+    p[0] = from_f32<U>(v);
+    p[1] = __builtin_isfinite(to_f32(p[0])) ? from_f32<U>(v - to_f32(p[0])) : (U)0.f;
+}
+template <typename U> __device__ __forceinline__ void store_fine4(void *base, int64_t plane, int64_t at, const float (&v)[4]) {
+    Pack<U, 4> o[2];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        U p[2];
+        split2(v[e], p);
+        o[0].v[e] = p[0]; o[1].v[e] = p[1];
+    }
+#pragma unroll
+    for (int q = 0; q < 2; q++) *reinterpret_cast<Pack<U, 4> *>((U *)base + q * plane + at) = o[q];
 }
 // the same of eight elements in LDS, rounded already
 template <typename U> __device__ __forceinline__ void store_staged(void *base, int64_t plane, int64_t at, const U *s) {
@@ -339,7 +358,7 @@ __device__ __forceinline__ void multiply_step(A a, B b, R request, f32x4 (&acc)[
 template <typename T, typename U, int P, int BUFS, int BM, int BN, int WI, int WJ, bool AKS, bool BKS, int EPI>
 __global__ __launch_bounds__(64 * WI * WJ) void k_rows_gemm(const Args p) {
     constexpr int WAVES = WI * WJ, MT = BM / WI / 16, NT = BN / WJ / 16;
-    constexpr bool DUAL = EPI == EPI_GATE;
+    constexpr bool DUAL = gate_forward(EPI);
     constexpr int TJ = DUAL ? BN / 2 : BN;                   // columns of C per tile
     using SA = Side<BM, AKS, WAVES, MT>;
     using SB = Side<BN, BKS, WAVES, NT>;
@@ -439,8 +458,9 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_rows_gemm(const Args p) {
         // A lane has both projections (EPI_GATE) of the same elements, or fetches G and U of its own: the elementwise part is done where the products are, rounded,
         // and only its results pass through LDS, so that full lines of global memory are written.  Columns up to ldh are written: behind J nothing was
         // read, so the padding of G, U, H, gg and gu is zero.
-        constexpr int COLS = EPI == EPI_GATE ? TJ : 2 * TJ, N = DUAL ? NT / 2 : NT;
-        using St = Staging<U, COLS, TJ, MT, WI, WAVES, EPI == EPI_GATE ? MT : 1, BUFS * P * (BM + BN) * BK * 2>;
+        // (EPI_GATE_FINE and its like, few results: written from where they are, in two planes.)
+        constexpr int COLS = DUAL ? TJ : 2 * TJ, N = DUAL ? NT / 2 : NT;
+        using St = Staging<U, COLS, TJ, MT, WI, WAVES, DUAL ? MT : 1, BUFS * P * (BM + BN) * BK * 2>;
         f32x4 gq[N], uq[N];
         auto place = [&](int m, int n) {                    // (clamped: nothing branches between the requests)
             int64_t i = i0 + (wi * MT + m) * 16 + li, j = j0 + (wj * N + n) * 16 + lq * 4;
@@ -455,6 +475,40 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_rows_gemm(const Args p) {
                 uq[n] = *reinterpret_cast<const f32x4 *>(p.u + place(m, n));
             }
         };
+        if constexpr (EPI == EPI_GATE_FINE || EPI == EPI_GATE_BWD_FINE) {
+            with_activation(p.act, [&](auto act) {
+                constexpr int ACT = decltype(act)::value;
+#pragma unroll
+                for (int m = 0; m < MT; m++) {
+                    if constexpr (!DUAL) fetch(m);
+#pragma unroll
+                    for (int n = 0; n < N; n++) {
+                        if (i0 + (wi * MT + m) * 16 + li >= p.I || j0 + (wj * N + n) * 16 + lq * 4 >= p.ldh) continue;
+                        const int64_t at = place(m, n);
+                        float o[4], o1[4], d;
+                        if constexpr (DUAL) {
+                            const f32x4 g = acc[m][n], u = acc[m][n + N];
+#pragma unroll
+                            for (int r = 0; r < 4; r++) o[r] = activation<ACT, false>(g[r], d) * u[r];
+                            if (p.g) {
+                                *reinterpret_cast<f32x4 *>(p.g + at) = g;
+                                *reinterpret_cast<f32x4 *>(p.u + at) = u;
+                            }
+                            store_fine4<U>(p.h, p.plane, at, o);
+                        } else {
+#pragma unroll
+                            for (int r = 0; r < 4; r++) {
+                                o1[r] = acc[m][n][r] * activation<ACT, true>(gq[n][r], d);
+                                o[r] = acc[m][n][r] * uq[n][r] * d;
+                            }
+                            store_fine4<U>(p.gg, p.plane, at, o);
+                            store_fine4<U>(p.gu, p.plane, at, o1);
+                        }
+                    }
+                }
+            });
+            return;
+        }
         if constexpr (EPI == EPI_GATE_BWD) fetch(0);
         U *stage = reinterpret_cast<U *>(lds);
         with_activation(p.act, [&](auto act) {
@@ -521,9 +575,9 @@ inline void as_segments(Args &p) {
 
 template <typename T, typename U, int P, int BUFS, int BM, int BN, int WI, int WJ, bool AKS, bool BKS, int EPI>
 inline int launch_tile(Args p, int problems, hipStream_t s) {
-    constexpr int TJ = EPI == EPI_GATE ? BN / 2 : BN;
+    constexpr int TJ = gate_forward(EPI) ? BN / 2 : BN;
     // the gate epilogues also write the padding columns up to ldh (< J + 8)
-    const int64_t cols = EPI == EPI_GATE || EPI == EPI_GATE_BWD ? p.ldh : p.J;
+    const int64_t cols = gate_forward(EPI) || gate_backward(EPI) ? p.ldh : p.J;
     const int64_t ti = (p.I + BM - 1) / BM, tj = (cols + TJ - 1) / TJ;
     if (ti * tj > kMaxGrid / (64 * WI * WJ) / problems / p.slices) return HS_ERR_ARG;
     p.problems = p.slices > 1 ? problems : 1;
@@ -546,7 +600,7 @@ inline int launch_tile(Args p, int problems, hipStream_t s) {
 // is what fills them (128 x 128 435, 256 x 64 435, 256 x 128 413, 64 x 64 423; eight waves 366, no gain for twice the LDS reads).
 constexpr int kAgainM = 128, kAgainJ = 64;
 
-template <typename T, typename U>
+template <typename T, typename U, bool FINE>
 __global__ __launch_bounds__(256) void k_gate_bwd(const Args p) {
     constexpr int BM = kAgainM, TJ = kAgainJ, WAVES = 4, WI = 2, WJ = 2, MT = BM / WI / 16, N2 = TJ / WJ / 16, N1 = 2 * N2;
     using SA = Side<BM, false, WAVES, MT>;
@@ -624,6 +678,26 @@ __global__ __launch_bounds__(256) void k_gate_bwd(const Args p) {
     // memory are written (131 072 x 256 x 1 024: 369 us; G, U and gH in fp32 through LDS: 381)
     using St = Staging<U, 2 * TJ, TJ, MT, WI, WAVES, MT, 2 * (int)kBuf>;
     const int li = lane & 15, lq = lane >> 4;
+    if constexpr (FINE) {
+        with_activation(p.act, [&](auto act) {
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int n = 0; n < N2; n++) {
+                    const int64_t i = i0 + (wi * MT + m) * 16 + li, j = j0 + (wj * N2 + n) * 16 + lq * 4;
+                    if (i >= p.I || j >= p.ldh) continue;
+                    float gg[4], gu[4], d;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        gu[r] = acc2[m][n][r] * activation<decltype(act)::value, true>(acc[m][n][r], d);
+                        gg[r] = acc2[m][n][r] * acc[m][n + N2][r] * d;
+                    }
+                    store_fine4<U>(p.gg, p.plane, i * p.ldh + j, gg);
+                    store_fine4<U>(p.gu, p.plane, i * p.ldh + j, gu);
+                }
+        });
+        return;
+    }
     U *stage = reinterpret_cast<U *>(lds);
     with_activation(p.act, [&](auto act) {
         constexpr int ACT = decltype(act)::value;
@@ -658,7 +732,7 @@ __global__ __launch_bounds__(256) void k_gate_bwd(const Args p) {
     });
 }
 
-template <typename T, typename U> inline int launch_gate_bwd(Args p, hipStream_t s) {
+template <typename T, typename U, bool FINE> inline int launch_gate_bwd(Args p, hipStream_t s) {
     constexpr int BM = kAgainM;
     if constexpr (planes<U>() == 3) as_segments(p);
     const int64_t ti = (p.I + BM - 1) / BM, tj = (p.ldh + kAgainJ - 1) / kAgainJ;
@@ -667,8 +741,8 @@ template <typename T, typename U> inline int launch_gate_bwd(Args p, hipStream_t
     p.tiles_j = (int)tj;
     constexpr int lds = 2 * (BM + 2 * kAgainJ) * BK * 2;
     static hsLdsAttrOnce attr;
-    attr.set((const void *)k_gate_bwd<T, U>, lds);
-    k_gate_bwd<T, U><<<dim3((unsigned)(ti * tj)), 256, lds, s>>>(p);
+    attr.set((const void *)k_gate_bwd<T, U, FINE>, lds);
+    k_gate_bwd<T, U, FINE><<<dim3((unsigned)(ti * tj)), 256, lds, s>>>(p);
     return hipGetLastError() == hipSuccess ? HS_OK : HS_ERR_LAUNCH;
 }
 

@@ -48,7 +48,9 @@ template <typename T, typename U, int P> __device__ __forceinline__ void small_f
     }
 }
 
-template <typename T, int P> __device__ __forceinline__ f32x4 small_product(const i16x8 (&w)[P], const i16x8 (&x)[P], f32x4 c) {
+template <typename T, int P, int PX> __device__ __forceinline__ f32x4 small_product(const i16x8 (&w)[P], const i16x8 (&x)[PX], f32x4 c) {
+    if constexpr (P == 1 && PX == 2) return mfma<T>(w[0], x[0], mfma<T>(w[0], x[1], c));
+    else
 #pragma unroll
     for (int t = 0; t < (P == 3 ? 6 : 1); t++) c = plane_product<T, P>(t, w, x, c);
     return c;
@@ -61,10 +63,11 @@ template <typename U, int P> __device__ __forceinline__ void small_planes(const 
     for (int q = 0; q < P; q++) f[q] = *reinterpret_cast<const i16x8 *>((const E *)h + q * plane + at);
 }
 
-template <typename T, typename U, int TOK, int WAVES, int EPI>
+// FINE: H in two planes of a 16-bit type
+template <typename T, typename U, int TOK, int WAVES, int EPI, bool FINE>
 __global__ __launch_bounds__(64 * WAVES) void k_rows_small(const SmallArgs p) {
     constexpr bool GATE = EPI == EPI_GATE;
-    constexpr int P = sizeof(U) == 4 ? 3 : 1, NW = GATE ? 2 : 1;
+    constexpr int P = sizeof(U) == 4 ? 3 : 1, PX = FINE && !GATE ? 2 : P, NW = GATE ? 2 : 1;
     __shared__ f32x4 join[WAVES][NW * TOK][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, q = lane >> 4;
     const int n0 = blockIdx.x * 16, n = n0 + r < p.N ? n0 + r : p.N - 1;         // (rows behind the last read it again; their results are not stored)
@@ -72,9 +75,9 @@ __global__ __launch_bounds__(64 * WAVES) void k_rows_small(const SmallArgs p) {
     int64_t xrow[TOK];
 #pragma unroll
     for (int t = 0; t < TOK; t++) xrow[t] = (int64_t)(t * 16 + r < p.M ? t * 16 + r : p.M - 1) * p.ldx;
-    auto load_x = [&](int t, int k, int K, i16x8 (&f)[P]) {
+    auto load_x = [&](int t, int k, int K, i16x8 (&f)[PX]) {
         if constexpr (GATE) small_fragment<T, U, P>((const U *)p.x + xrow[t], k, K, f);
-        else small_planes<U, P>(p.x, p.plane, xrow[t] + k, f);
+        else small_planes<U, PX>(p.x, p.plane, xrow[t] + k, f);
     };
     f32x4 acc[NW][TOK];
 #pragma unroll
@@ -92,10 +95,10 @@ __global__ __launch_bounds__(64 * WAVES) void k_rows_small(const SmallArgs p) {
             for (int s = 0; s < 4; s++)
 #pragma unroll
                 for (int t = 0; t < TOK; t++) {
-                    i16x8 fx[P];
+                    i16x8 fx[PX];
                     load_x(t, k0 + 32 * s + 8 * q, 0x7fffffff, fx);
 #pragma unroll
-                    for (int w = 0; w < NW; w++) acc[w][t] = small_product<T, P>(fw[w][s], fx, acc[w][t]);
+                    for (int w = 0; w < NW; w++) acc[w][t] = small_product<T, P, PX>(fw[w][s], fx, acc[w][t]);
                 }
         } else {
             for (int s = 0; s < 4 && k0 + 32 * s < p.K; s++) {
@@ -104,13 +107,13 @@ __global__ __launch_bounds__(64 * WAVES) void k_rows_small(const SmallArgs p) {
                 for (int w = 0; w < NW; w++) small_fragment<T, U, P>(wrow[w], k0 + 32 * s + 8 * q, p.K, fw[w]);
 #pragma unroll
                 for (int t = 0; t < TOK; t++) {
-                    i16x8 fx[P];
+                    i16x8 fx[PX];
                     if (k0 + 32 * s + 8 * q < p.K) load_x(t, k0 + 32 * s + 8 * q, p.K, fx);
                     else
 #pragma unroll
-                        for (int c = 0; c < P; c++) fx[c] = i16x8{0, 0, 0, 0, 0, 0, 0, 0};
+                        for (int c = 0; c < PX; c++) fx[c] = i16x8{0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-                    for (int w = 0; w < NW; w++) acc[w][t] = small_product<T, P>(fw[w], fx, acc[w][t]);
+                    for (int w = 0; w < NW; w++) acc[w][t] = small_product<T, P, PX>(fw[w], fx, acc[w][t]);
                 }
             }
         }
@@ -148,6 +151,11 @@ __global__ __launch_bounds__(64 * WAVES) void k_rows_small(const SmallArgs p) {
                         split3(h, o);
 #pragma unroll
                         for (int c = 0; c < 3; c++) ((bf16_t *)p.h)[c * p.plane + at] = o[c];
+                    } else if constexpr (FINE) {
+                        U o[2];
+                        split2(h, o);
+                        ((U *)p.h)[at] = o[0];
+                        ((U *)p.h)[p.plane + at] = o[1];
                     } else {
                         ((U *)p.h)[at] = from_f32<U>(h);
                     }
@@ -162,13 +170,13 @@ __global__ __launch_bounds__(64 * WAVES) void k_rows_small(const SmallArgs p) {
     }
 }
 
-template <typename T, typename U, int EPI> inline int launch_small(const SmallArgs &p, hipStream_t s) {
+template <typename T, typename U, int EPI, bool FINE> inline int launch_small(const SmallArgs &p, hipStream_t s) {
     constexpr int WAVES = EPI == EPI_GATE ? 4 : 8;
     const int64_t cols = EPI == EPI_GATE ? p.ldh : p.N;
     const unsigned blocks = (unsigned)((cols + 15) / 16);
-    if (p.M <= 16) k_rows_small<T, U, 1, WAVES, EPI><<<blocks, 64 * WAVES, 0, s>>>(p);
-    else if (p.M <= 32) k_rows_small<T, U, 2, WAVES, EPI><<<blocks, 64 * WAVES, 0, s>>>(p);
-    else if constexpr (sizeof(U) == 4) k_rows_small<T, U, 4, WAVES, EPI><<<blocks, 64 * WAVES, 0, s>>>(p);
+    if (p.M <= 16) k_rows_small<T, U, 1, WAVES, EPI, FINE><<<blocks, 64 * WAVES, 0, s>>>(p);
+    else if (p.M <= 32) k_rows_small<T, U, 2, WAVES, EPI, FINE><<<blocks, 64 * WAVES, 0, s>>>(p);
+    else if constexpr (sizeof(U) == 4) k_rows_small<T, U, 4, WAVES, EPI, FINE><<<blocks, 64 * WAVES, 0, s>>>(p);
     else return HS_ERR_ARG;
     return hipGetLastError() == hipSuccess ? HS_OK : HS_ERR_LAUNCH;
 }
