@@ -320,9 +320,10 @@ template <typename T, int P> __device__ __forceinline__ f32x4 plane_product(int 
 // One step (64 of K) of a wave's products.  Fragments are requested PF groups of matrix instructions ahead of their use, and the order written here is pinned
 // (sched_group_barrier: 0x100 LDS reads, 0x8 matrix instructions): left to itself the compiler puts every read directly in front of its use, with a wait for
 // its whole latency between (8 192 x 4 096 x 12 288: 774 -> 699 us).  a(m, ks, plane), b(n, ks, plane): the fragments; RA, RB: LDS instructions of one.
-// request(): the next step's LDS-DMA, issued while the first fragments are on their way.
+// request(): the next step's LDS-DMA, issued while the first fragments are on their way.  P == 3: the five smaller plane products are summed in `low`, 2^-8 of acc at most,
+// so that acc is rounded once in 32 of K and not six times (error of y against 64 bits at 3 033 x 2 016 x 64: 1.1e-6 -> 4.2e-7; fp32 library products 6.0e-7).
 template <typename T, int MT, int NT, int P, int RA, int RB, typename A, typename B, typename R>
-__device__ __forceinline__ void multiply_step(A a, B b, R request, f32x4 (&acc)[MT][NT]) {
+__device__ __forceinline__ void multiply_step(A a, B b, R request, f32x4 (&acc)[MT][NT], f32x4 (&low)[P == 3 ? MT : 1][NT]) {
     constexpr int G = 2 * MT, PF = P == 3 ? 1 : MT >= 4 ? 3 : 2, TERMS = P == 3 ? 6 : 1;
     i16x8 fa[G][P], fb[2][NT][P];
 #pragma unroll
@@ -348,7 +349,10 @@ __device__ __forceinline__ void multiply_step(A a, B b, R request, f32x4 (&acc)[
 #pragma unroll
         for (int t = 0; t < TERMS; t++)
 #pragma unroll
-            for (int n = 0; n < NT; n++) acc[g % MT][n] = plane_product<T, P>(t, fb[g / MT][n], fa[g], acc[g % MT][n]);
+            for (int n = 0; n < NT; n++) {
+                f32x4 &to = P == 3 && t + 1 < TERMS ? low[P == 3 ? g % MT : 0][n] : acc[g % MT][n];
+                to = plane_product<T, P>(t, fb[g / MT][n], fa[g], to);
+            }
         if constexpr (reads > 0) __builtin_amdgcn_sched_group_barrier(0x100, reads, 0);
         __builtin_amdgcn_sched_group_barrier(0x8, NT * TERMS, 0);
     });
@@ -405,11 +409,14 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_rows_gemm(const Args p) {
             if (++sg < p.n_seg) point();
         }
     };
-    f32x4 acc[MT][NT];
+    f32x4 acc[MT][NT], low[P == 3 ? MT : 1][NT];
 #pragma unroll
     for (int m = 0; m < MT; m++)
 #pragma unroll
-        for (int n = 0; n < NT; n++) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int n = 0; n < NT; n++) {
+            acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (P == 3) low[P == 3 ? m : 0][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
     // BUFS buffers: a step's requests are made BUFS - 1 steps ahead, into the buffer that the step before the current one has just left
     if (s_begin < s_end) point();
 #pragma unroll
@@ -427,8 +434,14 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_rows_gemm(const Args p) {
             [&](int n, int ks, int q) {         // (EPI_GATE: the tile's upper half is the up projection's rows)
                 return DUAL && n >= NT / 2 ? sb.fragment(at_b + q * SB::kBytes, n - NT / 2, ks, BN / 2) : sb.fragment(at_b + q * SB::kBytes, n, ks);
             },
-            [&]() { if (s + BUFS - 1 < s_end) request(buf == 0 ? BUFS - 1 : buf - 1); }, acc);
+            [&]() { if (s + BUFS - 1 < s_end) request(buf == 0 ? BUFS - 1 : buf - 1); }, acc, low);
         buf = buf + 1 == BUFS ? 0 : buf + 1;
+    }
+    if constexpr (P == 3) {
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int n = 0; n < NT; n++) acc[m][n] += low[m][n];
     }
 
     // ---- epilogue: acc[m][n][r] is row i0 + 16 (wi MT + m) + (lane & 15), column 16 unit + 4 (lane >> 4) + r
@@ -642,7 +655,7 @@ __global__ __launch_bounds__(256) void k_gate_bwd(const Args p) {
         s2.request(wave, b, b, left, lds0 + buf * kBuf + SA::kBytes);
         advance();
     };
-    f32x4 acc[MT][N1], acc2[MT][N2];
+    f32x4 acc[MT][N1], acc2[MT][N2], none1[1][N1], none2[1][N2];
 #pragma unroll
     for (int m = 0; m < MT; m++) {
 #pragma unroll
@@ -664,14 +677,14 @@ __global__ __launch_bounds__(256) void k_gate_bwd(const Args p) {
                                                request2(buf ^ 1);
                                            }
                                        },
-                                       acc);
+                                       acc, none1);
         buf ^= 1;
     }
     for (int s = 0; s < steps; s++) {
         wait_and_meet<0>();
         const uint32_t at = lds0 + buf * kBuf;
         multiply_step<T, MT, N2, 1, 1, 2>([&](int m, int ks, int) { return sx.fragment(at, m, ks); }, [&](int n, int ks, int) { return s2.fragment(at + SA::kBytes, n, ks); },
-                                       [&]() { if (s + 1 < steps) request2(buf ^ 1); }, acc2);
+                                       [&]() { if (s + 1 < steps) request2(buf ^ 1); }, acc2, none2);
         buf ^= 1;
     }
     // A lane has G, U and gH of the same elements: gg and gu are computed where they are, rounded, and only then pass through LDS, so that full lines of global

@@ -48,12 +48,14 @@ template <typename T, typename U, int P> __device__ __forceinline__ void small_f
     }
 }
 
-template <typename T, int P, int PX> __device__ __forceinline__ f32x4 small_product(const i16x8 (&w)[P], const i16x8 (&x)[PX], f32x4 c) {
-    if constexpr (P == 1 && PX == 2) return mfma<T>(w[0], x[0], mfma<T>(w[0], x[1], c));
-    else
+// c += the product, of several planes the smaller ones' to `low` (which is 2^-8 of c at most: c is rounded once)
+template <typename T, int P, int PX> __device__ __forceinline__ void small_product(const i16x8 (&w)[P], const i16x8 (&x)[PX], f32x4 &c, f32x4 &low) {
+    if constexpr (P == 1 && PX == 2) low = mfma<T>(w[0], x[1], low);
+    if constexpr (P == 3) {
 #pragma unroll
-    for (int t = 0; t < (P == 3 ? 6 : 1); t++) c = plane_product<T, P>(t, w, x, c);
-    return c;
+        for (int t = 0; t < 5; t++) low = plane_product<T, P>(t, w, x, low);
+    }
+    c = mfma<T>(w[0], x[0], c);
 }
 
 // the same of H as EPI_GATE left it: planes of whole fragments
@@ -79,11 +81,11 @@ __global__ __launch_bounds__(64 * WAVES) void k_rows_small(const SmallArgs p) {
         if constexpr (GATE) small_fragment<T, U, P>((const U *)p.x + xrow[t], k, K, f);
         else small_planes<U, PX>(p.x, p.plane, xrow[t] + k, f);
     };
-    f32x4 acc[NW][TOK];
+    f32x4 acc[NW][TOK], low[NW][TOK];
 #pragma unroll
     for (int w = 0; w < NW; w++)
 #pragma unroll
-        for (int t = 0; t < TOK; t++) acc[w][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < TOK; t++) acc[w][t] = low[w][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int k0 = wave * kSmallTurn; k0 < p.K; k0 += WAVES * kSmallTurn) {
         if (k0 + kSmallTurn <= p.K) {
             i16x8 fw[NW][4][P];
@@ -98,7 +100,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_rows_small(const SmallArgs p) {
                     i16x8 fx[PX];
                     load_x(t, k0 + 32 * s + 8 * q, 0x7fffffff, fx);
 #pragma unroll
-                    for (int w = 0; w < NW; w++) acc[w][t] = small_product<T, P, PX>(fw[w][s], fx, acc[w][t]);
+                    for (int w = 0; w < NW; w++) small_product<T, P, PX>(fw[w][s], fx, acc[w][t], low[w][t]);
                 }
         } else {
             for (int s = 0; s < 4 && k0 + 32 * s < p.K; s++) {
@@ -113,7 +115,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_rows_small(const SmallArgs p) {
 #pragma unroll
                         for (int c = 0; c < PX; c++) fx[c] = i16x8{0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-                    for (int w = 0; w < NW; w++) acc[w][t] = small_product<T, P, PX>(fw[w], fx, acc[w][t]);
+                    for (int w = 0; w < NW; w++) small_product<T, P, PX>(fw[w], fx, acc[w][t], low[w][t]);
                 }
             }
         }
@@ -121,7 +123,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_rows_small(const SmallArgs p) {
 #pragma unroll
     for (int w = 0; w < NW; w++)
 #pragma unroll
-        for (int t = 0; t < TOK; t++) join[wave][w * TOK + t][lane] = acc[w][t];
+        for (int t = 0; t < TOK; t++) join[wave][w * TOK + t][lane] = PX > 1 ? acc[w][t] + low[w][t] : acc[w][t];
     __syncthreads();
     // a wave per 16 rows of x: row t 16 + r, results n0 + 4 q ..
     for (int t = wave; t < TOK; t += WAVES) {
