@@ -79,6 +79,15 @@ def test_embedding_one_index_takes_everything(n):
     check_embed(torch.full((n,), 49, dtype=torch.int32, device=DEV), table, padding=49)         # nothing is left
 
 
+@pytest.mark.parametrize("n", [5000, 70000])
+@pytest.mark.parametrize("V", [1, 2, 511, 512, 2046, 2047, 2048, 2049, 300000])
+def test_embedding_digits(n, V):
+    """Tables at the edges of the sort's digits and passes, 32-bit indices, a padding row."""
+    gen = torch.Generator().manual_seed(n + V)
+    idx = torch.randint(-1, V + 1, (n,), generator=gen, dtype=torch.int32).to(DEV)
+    check_embed(idx, torch.randn(V, 12, generator=gen).to(torch.bfloat16).to(DEV), padding=V // 2)
+
+
 def test_embedding_long_runs_and_gaps():
     gen = torch.Generator().manual_seed(3)
     for V, frames in ((1024, [5, 5, 900, 1023, 0, 0, 5, 77]), (3_000_000, [2_999_999, 12, 0, 2_048_001])):
@@ -345,6 +354,12 @@ def test_gated_activations(act, dtype):
                                          (torch.bfloat16, 513, 1536, 2056)])
 def test_gated_large_tiles_and_slices(dtype, M, D, F):
     check_gated(*gated_inputs(M, D, F, dtype), act="silu")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,D,F", [(2500, 200, 90), (1500, 333, 777), (900, 2100, 130), (5000, 40, 500), (33, 700, 1300), (6000, 300, 17)])
+def test_gated_uneven_slices(M, D, F, dtype):
+    check_gated(*gated_inputs(M, D, F, dtype), "silu")
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -636,3 +651,47 @@ def test_modules_train_together():
     assert not bool(emb.weight.grad[0].any())
     drop.eval()
     assert torch.equal(drop(outs[0], residual=outs[1]), outs[0] + outs[1]) and int(drop.rng[1]) == 2
+
+
+def test_training_step_in_a_graph():
+    """The modules' forward and backward() captured as one graph, the leaves' gradients written by every replay, against the same steps run eagerly."""
+    r = ops()
+    torch.manual_seed(1)
+
+    def make():
+        torch.manual_seed(2)
+        return r.RowEmbedding(40, 64, std=1.0).to(DEV), r.GatedMLP(64, 96, "gelu").to(DEV), r.RowDropout(0.2, seed=5).to(DEV)
+
+    def step(mods, idx, gy):
+        emb, mlp, drop = mods
+        x = emb(idx)
+        y = drop(mlp(x), residual=x)
+        y.backward(gy)
+        return y.detach()
+    idx, gy = torch.arange(300, device=DEV) * 7 % 40, torch.randn(300, 64, device=DEV)
+    captured, eager = make(), make()
+    params = [[p for m in mods for p in m.parameters()] for mods in (captured, eager)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(captured, idx, gy)
+    torch.cuda.current_stream().wait_stream(side)
+    for p in params[0]:
+        p.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(captured, idx, gy)
+    eager[2].rng.copy_(captured[2].rng)
+    gen = torch.Generator().manual_seed(3)
+    for k in range(4):
+        idx.copy_(torch.randint(0, 40, (300,), generator=gen))
+        gy.copy_(torch.randn(300, 64, generator=gen))
+        graph.replay()
+        for p in params[1]:
+            p.grad = None
+        want = step(eager, idx, gy)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), k
+        assert all(torch.equal(a.grad, b.grad) for a, b in zip(*params)), k
+    assert torch.equal(captured[2].rng, eager[2].rng)
