@@ -145,8 +145,9 @@ template <typename T, typename U, bool AKS, bool BKS, int EPI> int launch_produc
 template <typename U> constexpr int64_t again_dim() { return sizeof(U) == 4 ? 128 : 768; }
 
 // Up to this many rows the forward products read the weights in place (rows_small.h).  4 096 x 12 288 bf16: 105 us at 33 rows, 145 at 64, where the tiles take
-// 104 at 65; fp32, whose tiles need copies in planes: 392 at 64 against 738 at 65.
-template <typename U> constexpr int64_t small_rows() { return sizeof(U) == 4 ? 64 : 32; }
+// 104 at 65.  fp32, whose tiles need copies in planes: 4 096 x 12 288 368 us at 33 rows and 417 at 64 against 545 in tiles, but 1 000 x 2 730 52 and 60 against
+// 45, and 239 and 36 at 32 rows: to 64 rows for large weights, to 32 for the others.
+template <typename U> int64_t small_rows(int64_t D, int64_t F) { return sizeof(U) == 4 && D * F >= (1 << 23) ? 64 : 32; }
 
 template <typename T, typename U> struct Block {
     const hsGatedMlp &a;
@@ -164,7 +165,7 @@ template <typename T, typename U> struct Block {
     // H, gg and gu of the 16-bit types in two planes where a result has few elements: rounded once they bring as much error into a result as its own rounding, 1.4 times
     // in all over many elements, but over few of them anything up to twice; in two planes nothing that shows.  The steps of the products that read them
     // double, which so small ones do not feel (a step of 1 x 32 x 2 976 bf16 is bound by the host); 1 x 4 096 x 12 288, where reading the weights is all there is,
-    // would: down projection 25.1 -> 28.4 us.
+    // would: down projection 25.1 -> 28.4 us (eight waves a workgroup).
     static constexpr int64_t kFineResults = 2048;
     bool fine() const { return sizeof(U) == 2 && (M < F ? M : F) * D <= kFineResults; }
     int inner_planes() const { return fine() ? 2 : planes<U>(); }
@@ -241,7 +242,7 @@ template <typename T, typename U> struct Block {
     }
 
     void fwd() {
-        if (M <= small_rows<U>()) return fwd_small();
+        if (M <= small_rows<U>(D, F)) return fwd_small();
         const Operand x = operand(a.x, a.ldx, M, D);
         Operand wg, wu;
         projections(wg, wu);

@@ -1,12 +1,11 @@
-// rows_small.h -- the forward products of the gated feed-forward block for few rows (serving; small_rows() in gated_mlp.h: 32, fp32 64), where reading the weights once is all there is.
+// rows_small.h -- the forward products of the gated feed-forward block for few rows (serving; small_rows() in gated_mlp.h), where reading the weights once is all there is.
 //
 // A workgroup takes 16 rows of the weights (with EPI_GATE of both projections) and every row of x; its waves share K in turns of 128 elements, so that the
 // workgroup streams whole stretches of each weight row, straight from global memory into the registers of the matrix instructions (a lane's fragment is 16
 // consecutive bytes).  The weights are the instruction's A: a lane ends with four consecutive results of one row of x.  The waves' partial sums meet in
 // LDS in the order of the waves.  Any row distance and alignment is read in place -- a copy of an unaligned weight would cost more than the product.
 // fp32: each operand is split into its three planes in registers.
-// Bound by reading the weights: 1 x 4 096 x 12 288 bf16 37.4 us (gate and up, 201 MB, 5.4 TB/s) and 25.1 us (down, 101 MB, 4.0 TB/s: 256 workgroups, one round of
-// the device, so its beginning and end show); 13 x 1 000 x 2 730 f16 6.0 and 5.8 us (16 MB: latency).
+// Bound by reading the weights: 1 x 4 096 x 12 288 bf16 37.4 us (gate and up, 201 MB, 5.4 TB/s) and 20.5 us (down, 101 MB, 4.9 TB/s); 13 x 1 000 x 2 730 f16 6.0 and 5.8 us (16 MB: latency).
 #pragma once
 #include "rows_gemm.h"
 
@@ -88,20 +87,25 @@ __global__ __launch_bounds__(64 * WAVES) void k_rows_small(const SmallArgs p) {
         for (int t = 0; t < TOK; t++) acc[w][t] = low[w][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int k0 = wave * kSmallTurn; k0 < p.K; k0 += WAVES * kSmallTurn) {
         if (k0 + kSmallTurn <= p.K) {
-            i16x8 fw[NW][4][P];
+            // (four groups of rows: half a turn's fragments at a time, or the registers leave one wave a SIMD: 50 x 4 096 x 12 288 fp32 463 -> 393 us)
+            constexpr int HALF = TOK == 4 ? 2 : 4;
 #pragma unroll
-            for (int s = 0; s < 4; s++)
+            for (int s0 = 0; s0 < 4; s0 += HALF) {
+                i16x8 fw[NW][HALF][P];
 #pragma unroll
-                for (int w = 0; w < NW; w++) small_fragment<T, U, P>(wrow[w], k0 + 32 * s + 8 * q, 0x7fffffff, fw[w][s]);
+                for (int s = 0; s < HALF; s++)
 #pragma unroll
-            for (int s = 0; s < 4; s++)
+                    for (int w = 0; w < NW; w++) small_fragment<T, U, P>(wrow[w], k0 + 32 * (s0 + s) + 8 * q, 0x7fffffff, fw[w][s]);
 #pragma unroll
-                for (int t = 0; t < TOK; t++) {
-                    i16x8 fx[PX];
-                    load_x(t, k0 + 32 * s + 8 * q, 0x7fffffff, fx);
+                for (int s = 0; s < HALF; s++)
 #pragma unroll
-                    for (int w = 0; w < NW; w++) small_product<T, P, PX>(fw[w][s], fx, acc[w][t], low[w][t]);
-                }
+                    for (int t = 0; t < TOK; t++) {
+                        i16x8 fx[PX];
+                        load_x(t, k0 + 32 * (s0 + s) + 8 * q, 0x7fffffff, fx);
+#pragma unroll
+                        for (int w = 0; w < NW; w++) small_product<T, P, PX>(fw[w][s], fx, acc[w][t], low[w][t]);
+                    }
+            }
         } else {
             for (int s = 0; s < 4 && k0 + 32 * s < p.K; s++) {
                 i16x8 fw[NW][P];
@@ -173,7 +177,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_rows_small(const SmallArgs p) {
 }
 
 template <typename T, typename U, int EPI, bool FINE> inline int launch_small(const SmallArgs &p, hipStream_t s) {
-    constexpr int WAVES = EPI == EPI_GATE ? 4 : 8;
+    // (the down projection has few workgroups: 1 x 4 096 x 12 288 bf16 25.1 us with eight waves, 20.5 with 16; fp32 the same with either)
+    constexpr int WAVES = EPI == EPI_GATE ? 4 : sizeof(U) == 2 ? 16 : 8;
     const int64_t cols = EPI == EPI_GATE ? p.ldh : p.N;
     const unsigned blocks = (unsigned)((cols + 15) / 16);
     if (p.M <= 16) k_rows_small<T, U, 1, WAVES, EPI, FINE><<<blocks, 64 * WAVES, 0, s>>>(p);

@@ -350,7 +350,7 @@ def test_gated_activations(act, dtype):
     check_gated(x * 4, wg, wu, wd, gy, act)          # (gates of several units: both tails of the activation)
 
 
-@pytest.mark.parametrize("dtype,M,D,F", [(torch.bfloat16, 4096, 64, 1600), (torch.float16, 2000, 1000, 1210), (torch.bfloat16, 20000, 256, 128), (torch.float32, 3000, 72, 700),
+@pytest.mark.parametrize("dtype,M,D,F", [(torch.float32, 50, 1101, 7700), (torch.float32, 64, 4000, 2100), (torch.bfloat16, 1, 4096, 2200), (torch.float16, 20, 1501, 4099), (torch.bfloat16, 4096, 64, 1600), (torch.float16, 2000, 1000, 1210), (torch.bfloat16, 20000, 256, 128), (torch.float32, 3000, 72, 700),
                                          (torch.bfloat16, 513, 1536, 2056)])
 def test_gated_large_tiles_and_slices(dtype, M, D, F):
     check_gated(*gated_inputs(M, D, F, dtype), act="silu")
