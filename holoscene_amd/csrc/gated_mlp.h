@@ -112,7 +112,8 @@ template <typename U> Plan plan_product(int64_t I, int64_t cols, int64_t steps, 
     const TileCost *kinds = sizeof(U) == 4 ? kTiles32 : kTiles16;
     Plan best = {0, 1};
     float least = 0.f;
-    for (int k = 0; k < (sizeof(U) == 4 ? 3 : 4); k++) {
+    // (fp32, one step: the large tile takes six, one a plane product -- forward of 113 397 x 502 x 13 372 us, without it 358)
+    for (int k = sizeof(U) == 4 && steps == 1 ? 1 : 0; k < (sizeof(U) == 4 ? 3 : 4); k++) {
         const TileCost &t = kinds[k];
         const int64_t whole = ((I + t.rows - 1) / t.rows) * ((cols + t.cols - 1) / t.cols) * problems;
         for (int slices : kSlices) {
