@@ -93,10 +93,12 @@ void *stream_of(const Tensor &t) { return c10::hip::getCurrentHIPStream(t.device
 
 Tensor bytes_on(const Tensor &t, int64_t n) { return at::empty({n}, t.options().dtype(at::kByte)); }
 
-// Gradients that cannot be differentiated again: where the caller asks for a graph of them (create_graph), whoever follows it is told so.
-variable_list no_second_derivative(const variable_list &grads, variable_list out) {
+// Gradients that cannot be differentiated again: where the caller asks for a graph of them (create_graph), whoever follows it is told so.  A gradient leads
+// to the incoming one where that requires a gradient itself, and with `operands` to the operands whatever the incoming one is: in
+// grad(y, x, ones, create_graph=True), a gradient penalty, it is a constant.
+variable_list no_second_derivative(const variable_list &grads, variable_list out, bool operands = false) {
     if (!at::GradMode::is_enabled()) return out;
-    bool any = false;
+    bool any = operands;
     for (const Tensor &g : grads) any = any || (g.defined() && g.requires_grad());
     if (!any) return out;
     for (Tensor &t : out)
@@ -280,6 +282,8 @@ Tensor gated(const Tensor &x, const Tensor &wg, const Tensor &wu, const Tensor &
 struct GatedMlpRows : torch::autograd::Function<GatedMlpRows> {
     static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &wg, const Tensor &wu, const Tensor &wd, int64_t activation) {
         ctx->saved_data["shape"] = x.sizes().vec();
+        // (every gradient depends on x, Wg or Wu; where Wd alone takes one, it depends on nothing that does)
+        ctx->saved_data["again"] = x.requires_grad() || wg.requires_grad() || wu.requires_grad();
         if (x.numel() == 0 || wg.numel() == 0) {
             ctx->save_for_backward({x, wg, wu, wd});
             return at::zeros_like(x);
@@ -315,7 +319,7 @@ struct GatedMlpRows : torch::autograd::Function<GatedMlpRows> {
                 if (out[0].defined() && ctx->saved_data["shape"].toIntVector().size() != 2) out[0] = out[0].view(ctx->saved_data["shape"].toIntVector());
             }
         }
-        return no_second_derivative(grads, std::move(out));
+        return no_second_derivative(grads, std::move(out), ctx->saved_data["again"].toBool());
     }
 };
 

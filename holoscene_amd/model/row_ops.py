@@ -8,7 +8,10 @@ dropout, each with its backward pass, on the kernels of csrc/embed_rows.hip, csr
 float32, bfloat16 and float16 storage, fp32 arithmetic, one rounding per result.  As everywhere in this package there is no CPU path: a tensor
 that is not on the GPU, or a type or shape the kernels do not take, raises RuntimeError.  The work runs on the current stream of the tensors' device
 and can be captured into a HIP graph (with a backward pass: capture before an eager graph of the same leaves is built, or drop it first -- its
-gradient accumulators belong to the eager stream); results do not depend on the launch (no floating-point atomics).  Gradients of gradients are not provided.
+gradient accumulators belong to the eager stream); results do not depend on the launch (no floating-point atomics).
+
+Gradients of gradients are not provided: with create_graph=True the gradients come back, and a backward pass that reaches them raises RuntimeError.  Those of
+embedding_rows and dropout_rows, linear operators, depend on the incoming gradient only; where that is a constant, so are they.
 """
 import torch
 import torch.nn as nn

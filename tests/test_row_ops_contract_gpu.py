@@ -1,0 +1,49 @@
+"""GPU: what the row operators (model/row_ops.py) owe a caller beside their values: gradients that are asked to be differentiable, results that are written in
+place, operands that are not finite, lazily negated operands, transforms that would lose the operators without a word."""
+import pytest
+import torch
+
+from test_row_ops_gpu import DEV, TYPES, gated_inputs, ops
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------------------ gradients of gradients
+@pytest.mark.parametrize("which", [0, 1, 2, 3])
+@pytest.mark.parametrize("form", ["rows", "leading dims", "copied"])
+def test_gradient_penalty_is_refused(which, form):
+    """grad(y, t, ones, create_graph=True): the incoming gradient is a constant, the block's gradients still depend on its operands."""
+    x, wg, wu, wd, _ = gated_inputs(6, 8, 16, torch.float32)
+    if form == "leading dims":
+        x = x.view(2, 3, 8)
+    if form == "copied":
+        x, wg = x.t().contiguous().t(), wg.t().contiguous().t()
+    leaves = [t.clone().requires_grad_(i == which or (which == 3 and i == 0)) for i, t in enumerate((x, wg, wu, wd))]        # (Wd's gradient depends on the others only)
+    y = ops().gated_mlp_rows(*leaves)
+    first, = torch.autograd.grad(y, leaves[which], torch.ones_like(y), create_graph=True)
+    want, = torch.autograd.grad(ops().gated_mlp_rows(*leaves), leaves[which], torch.ones_like(y))
+    assert torch.equal(first, want) and first.requires_grad
+    with pytest.raises(RuntimeError, match="cannot be differentiated again"):
+        (y.mean() + (first.norm() - 1) ** 2).backward()
+
+
+def test_gradients_that_depend_on_nothing_are_constants():
+    """Lookup, dropout, and Wd's gradient where nothing else takes one: linear, so with a constant incoming gradient there is nothing to differentiate."""
+    x, wg, wu, wd, _ = gated_inputs(6, 8, 16, torch.float32)
+    rng, idx = torch.tensor([3, 4], device=DEV), torch.arange(6, device=DEV)
+    for f, leaf in ((lambda t: ops().embedding_rows(idx, t), x), (lambda t: ops().dropout_rows(t, 0.5, rng), x), (lambda t: ops().dropout_rows(x, 0.5, rng, residual=t), x),
+                    (lambda t: ops().gated_mlp_rows(x, wg, wu, t), wd)):
+        leaf = leaf.clone().requires_grad_()
+        y = f(leaf)
+        first, = torch.autograd.grad(y, leaf, torch.ones_like(y), create_graph=True)
+        (y.mean() + (first.norm() - 1) ** 2).backward()
+        alone, = torch.autograd.grad(f(leaf).mean(), leaf)
+        assert torch.equal(leaf.grad, alone)
+
+
+def test_backward_with_create_graph_keeps_its_values():
+    x, wg, wu, wd, gy = gated_inputs(40, 24, 32, torch.float32)
+    a, b = ([t.clone().requires_grad_() for t in (x, wg, wu, wd)] for _ in range(2))
+    ops().gated_mlp_rows(*a).backward(gy)
+    grads = torch.autograd.grad(ops().gated_mlp_rows(*b), b, gy, create_graph=True)
+    assert all(torch.equal(s.grad, t) for s, t in zip(a, grads))
