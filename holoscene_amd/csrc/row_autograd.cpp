@@ -63,7 +63,13 @@ int32_t row_type(at::ScalarType t, const char *name) {
     return HS_F16;
 }
 
+// What would lose the operator without an error: a tangent (the call past autograd computes the value alone).
+void check_plain(const Tensor &t, const char *name) {
+    TORCH_CHECK(!t._fw_grad(0).defined(), name, " has a tangent: the row operators do not take part in forward mode differentiation");
+}
+
 void check_dense(const Tensor &t, const char *name) {
+    check_plain(t, name);
     TORCH_CHECK(t.defined() && t.is_cuda(), name, " must be a CUDA tensor");
     TORCH_CHECK(t.layout() == at::kStrided, name, " must be a dense tensor");
 }

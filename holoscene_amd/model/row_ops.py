@@ -11,7 +11,8 @@ and can be captured into a HIP graph (with a backward pass: capture before an ea
 gradient accumulators belong to the eager stream); results do not depend on the launch (no floating-point atomics).
 
 Gradients of gradients are not provided: with create_graph=True the gradients come back, and a backward pass that reaches them raises RuntimeError.  Those of
-embedding_rows and dropout_rows, linear operators, depend on the incoming gradient only; where that is a constant, so are they.
+embedding_rows and dropout_rows, linear operators, depend on the incoming gradient only; where that is a constant, so are they.  A tensor with a
+tangent (forward mode) is refused.
 """
 import torch
 import torch.nn as nn

@@ -47,3 +47,16 @@ def test_backward_with_create_graph_keeps_its_values():
     ops().gated_mlp_rows(*a).backward(gy)
     grads = torch.autograd.grad(ops().gated_mlp_rows(*b), b, gy, create_graph=True)
     assert all(torch.equal(s.grad, t) for s, t in zip(a, grads))
+
+
+# ------------------------------------------------------------------------------------------------ transforms
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fwd
+    x, wg, wu, wd, gy = gated_inputs(6, 8, 16, torch.float32)
+    rng, idx = torch.tensor([3, 4], device=DEV), torch.arange(6, device=DEV)
+    with fwd.dual_level():
+        d = fwd.make_dual(x, gy)
+        for f in (lambda: ops().gated_mlp_rows(d, wg, wu, wd), lambda: ops().gated_mlp_rows(x, wg, wu, fwd.make_dual(wd, wd)), lambda: ops().embedding_rows(idx, d),
+                  lambda: ops().dropout_rows(d, 0.5, rng), lambda: ops().dropout_rows(x, 0.5, rng, residual=d)):
+            with pytest.raises(RuntimeError, match="has a tangent"):
+                f()
