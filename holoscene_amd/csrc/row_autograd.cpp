@@ -8,6 +8,7 @@
 // The library is the one that hashencoder/backend.py has loaded and checked; bind() receives its entry points.  Errors are raised as RuntimeError (TORCH_CHECK).
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -63,9 +64,11 @@ int32_t row_type(at::ScalarType t, const char *name) {
     return HS_F16;
 }
 
-// What would lose the operator without an error: a tangent (the call past autograd computes the value alone).
+// What would lose the operator without an error: a tangent (the call past autograd computes the value alone), a trace (it would record the result's allocation,
+// not the launch that fills it).
 void check_plain(const Tensor &t, const char *name) {
     TORCH_CHECK(!t._fw_grad(0).defined(), name, " has a tangent: the row operators do not take part in forward mode differentiation");
+    TORCH_CHECK(!torch::jit::tracer::isTracing(), "the row operators cannot be traced (torch.jit.trace)");
 }
 
 void check_dense(const Tensor &t, const char *name) {

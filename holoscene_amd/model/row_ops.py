@@ -12,7 +12,7 @@ gradient accumulators belong to the eager stream); results do not depend on the 
 
 Gradients of gradients are not provided: with create_graph=True the gradients come back, and a backward pass that reaches them raises RuntimeError.  Those of
 embedding_rows and dropout_rows, linear operators, depend on the incoming gradient only; where that is a constant, so are they.  A tensor with a
-tangent (forward mode) is refused.
+tangent (forward mode) and a call under torch.jit.trace are refused.
 """
 import torch
 import torch.nn as nn

@@ -60,3 +60,12 @@ def test_forward_mode_is_refused():
                   lambda: ops().dropout_rows(d, 0.5, rng), lambda: ops().dropout_rows(x, 0.5, rng, residual=d)):
             with pytest.raises(RuntimeError, match="has a tangent"):
                 f()
+
+
+@pytest.mark.filterwarnings("ignore::DeprecationWarning")
+def test_tracing_is_refused():
+    x, wg, wu, wd, _ = gated_inputs(6, 8, 16, torch.float32)
+    rng, idx = torch.tensor([3, 4], device=DEV), torch.arange(6, device=DEV)
+    for f in (lambda t: ops().gated_mlp_rows(t, wg, wu, wd), lambda t: ops().embedding_rows(idx, t), lambda t: ops().dropout_rows(t, 0.5, rng)):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(f, (x,))
