@@ -4,7 +4,7 @@
 namespace {
 
 bool sizes_ok(const hsGatedMlp &a) {
-    return a.rows >= 0 && a.dim >= 0 && a.hidden >= 0 && a.rows <= 0x7fffffff && a.dim <= HS_GATED_MLP_MAX && a.hidden <= HS_GATED_MLP_MAX && a.ldx >= a.dim && a.ld_gate >= a.dim &&
+    return a.rows > 0 && a.dim > 0 && a.hidden > 0 && a.rows <= 0x7fffffff && a.dim <= HS_GATED_MLP_MAX && a.hidden <= HS_GATED_MLP_MAX && a.ldx >= a.dim && a.ld_gate >= a.dim &&
            a.ld_up >= a.dim && a.ld_down >= a.hidden && a.activation >= 0 && a.activation <= HS_ACT_RELU && hs_row::known_dtype(a.dtype);
 }
 
@@ -24,7 +24,7 @@ int64_t hs_gated_mlp_bwd_ws_bytes(const hsGatedMlp *a) { return !a ? HS_ERR_NULL
 
 int hs_gated_mlp_fwd(const hsGatedMlp *a, void *stream) {
     if (!a) return HS_ERR_NULL;
-    if (!sizes_ok(*a) || a->rows == 0 || a->dim == 0 || a->hidden == 0) return HS_ERR_ARG;
+    if (!sizes_ok(*a)) return HS_ERR_ARG;
     if (!a->x || !a->w_gate || !a->w_up || !a->w_down || !a->y) return HS_ERR_NULL;
     const int64_t need = call(*a, 2, nullptr);
     if (need > 0 && !a->ws) return HS_ERR_NULL;
@@ -34,7 +34,7 @@ int hs_gated_mlp_fwd(const hsGatedMlp *a, void *stream) {
 
 int hs_gated_mlp_bwd(const hsGatedMlp *a, void *stream) {
     if (!a) return HS_ERR_NULL;
-    if (!sizes_ok(*a) || a->rows == 0 || a->dim == 0 || a->hidden == 0 || a->ld_grad < a->dim) return HS_ERR_ARG;
+    if (!sizes_ok(*a) || a->ld_grad < a->dim) return HS_ERR_ARG;
     if (!a->x || !a->w_gate || !a->w_up || !a->w_down || !a->grad || !a->saved) return HS_ERR_NULL;
     const int64_t need = call(*a, 3, nullptr);
     if (need > 0 && !a->ws) return HS_ERR_NULL;

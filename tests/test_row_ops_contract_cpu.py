@@ -4,6 +4,7 @@ import torch
 import torch.autograd.forward_ad as fwd
 
 from holoscene_amd.model import row_ops
+from test_row_ops_cpu import gated, lib
 
 
 def calls(t):
@@ -33,3 +34,13 @@ def test_tracing_is_refused():
     for k in range(3):
         with pytest.raises(RuntimeError, match="cannot be traced"):
             torch.jit.trace(lambda t: list(calls(t))[k](), (x,))
+
+
+# ------------------------------------------------------------------------------------------------ sizes, from C
+def test_work_space_queries_refuse_empty_blocks():
+    """Without rows, columns or hidden elements there is no product to plan (the plan divided by the number of its tiles: SIGFPE)."""
+    for dtype in (0, 1, 2):
+        for bad in (dict(rows=0), dict(dim=0), dict(hidden=0), dict(rows=100, dim=0), dict(rows=100, hidden=0), dict(rows=0, dim=0, hidden=0)):
+            args = gated(dtype=dtype, gx=256, gw_gate=256, gw_up=256, gw_down=256, **bad)
+            assert lib().hs_gated_mlp_fwd_ws_bytes(args) == -1 and lib().hs_gated_mlp_bwd_ws_bytes(args) == -1, (dtype, bad)
+            assert lib().hs_gated_mlp_saved_bytes(args) == -1, (dtype, bad)
