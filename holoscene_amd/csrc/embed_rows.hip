@@ -496,7 +496,7 @@ struct BwdPlan {
 
 int64_t up256(int64_t b) { return (b + 255) / 256 * 256; }
 
-BwdPlan plan_bwd(int64_t n, int64_t V, int64_t D) {
+BwdPlan plan_bwd(int64_t n, int64_t V, int64_t D) {        // (V > 0: at least one pass)
     BwdPlan p = {};
     while (p.bits < 32 && ((uint64_t)V >> p.bits) != 0) p.bits++;        // keys 0 .. V
     const bool one = n <= kOneMax;
@@ -607,7 +607,7 @@ int hs_embed_fwd(const void *indices, int32_t index_bytes, const void *table, in
     return HS_OK;
 }
 
-int64_t hs_embed_bwd_ws_bytes(int64_t n, int64_t V, int64_t D) { return sizes_ok(n, V, D) ? plan_bwd(n, V, D).bytes : HS_ERR_ARG; }
+int64_t hs_embed_bwd_ws_bytes(int64_t n, int64_t V, int64_t D) { return !sizes_ok(n, V, D) ? HS_ERR_ARG : V > 0 && D > 0 ? plan_bwd(n, V, D).bytes : 0; }
 
 int hs_embed_bwd(const void *indices, int32_t index_bytes, const void *grad, int64_t ldg, void *grad_table, int64_t n, int64_t V, int64_t D, float scale, int64_t padding,
                  int32_t grad_dtype, int32_t table_dtype, void *ws, int64_t ws_bytes, void *stream) {

@@ -4,7 +4,7 @@ import torch
 import torch.autograd.forward_ad as fwd
 
 from holoscene_amd.model import row_ops
-from test_row_ops_cpu import gated, lib
+from test_row_ops_cpu import I64, gated, lib
 
 
 def calls(t):
@@ -44,3 +44,11 @@ def test_work_space_queries_refuse_empty_blocks():
             args = gated(dtype=dtype, gx=256, gw_gate=256, gw_up=256, gw_down=256, **bad)
             assert lib().hs_gated_mlp_fwd_ws_bytes(args) == -1 and lib().hs_gated_mlp_bwd_ws_bytes(args) == -1, (dtype, bad)
             assert lib().hs_gated_mlp_saved_bytes(args) == -1, (dtype, bad)
+
+
+def test_lookup_work_space_of_an_empty_table():
+    """A table without rows takes no pass of the sort (which the plan divided by: SIGFPE); its gradient needs nothing."""
+    f = lib().hs_embed_bwd_ws_bytes
+    for n in (0, 1, 5000, 1 << 20):
+        assert f(I64(n), I64(0), I64(16)) == 0 and f(I64(n), I64(5), I64(0)) == 0
+    assert f(I64(0), I64(5), I64(16)) >= 8
