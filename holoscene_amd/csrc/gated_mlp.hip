@@ -4,7 +4,7 @@
 namespace {
 
 bool sizes_ok(const hsGatedMlp &a) {
-    return a.rows > 0 && a.dim > 0 && a.hidden > 0 && a.rows <= 0x7fffffff && a.dim <= HS_GATED_MLP_MAX && a.hidden <= HS_GATED_MLP_MAX && a.ldx >= a.dim && a.ld_gate >= a.dim &&
+    return a.rows > 0 && a.dim > 0 && a.hidden > 0 && a.rows <= HS_GATED_MLP_MAX_ROWS && a.dim <= HS_GATED_MLP_MAX && a.hidden <= HS_GATED_MLP_MAX && a.ldx >= a.dim && a.ld_gate >= a.dim &&
            a.ld_up >= a.dim && a.ld_down >= a.hidden && a.activation >= 0 && a.activation <= HS_ACT_RELU && hs_row::known_dtype(a.dtype);
 }
 

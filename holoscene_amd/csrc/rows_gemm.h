@@ -56,7 +56,7 @@ struct Args {
     int64_t lda, ldb;                             // in elements, multiples of 8
     int64_t plane_a, plane_b;                     // bytes between planes
     int64_t I;
-    int32_t J, K;
+    int32_t J, K;                                 // K < 2^31 - BK (HS_GATED_MLP_MAX_ROWS): rounded up to whole steps in 32 bits
     int32_t tiles_i, tiles_j, problems, slices;
     // EPI_STORE
     void *out[2];                                 // per problem

@@ -911,13 +911,14 @@ int hs_embed_bwd(const void *indices, int32_t index_bytes, const void *grad, int
 int hs_dropout_rows(const void *x, const void *residual, void *y, int64_t n, int32_t dtype, int32_t drop, const uint64_t *rng, void *stream);
 
 /* y = (act(x Wg^T) * (x Wu^T)) Wd^T and its gradient; x [rows, dim], Wg, Wu [hidden, dim], Wd [dim, hidden], every one with a row distance of its own; y and the
- * gradients contiguous.  All three sizes > 0, dim and hidden <= 2^21.  fp32: an infinite operand gives NaN (infinity times a plane that is zero). */
+ * gradients contiguous.  All three sizes > 0, dim and hidden <= 2^21, rows <= 2^31 - 128.  fp32: an infinite operand gives NaN (infinity times a plane that is zero). */
 #define HS_ACT_SILU 0
 #define HS_ACT_GELU 1           /* g Phi(g) */
 #define HS_ACT_GELU_TANH 2
 #define HS_ACT_SIGMOID 3
 #define HS_ACT_RELU 4
 #define HS_GATED_MLP_MAX (1 << 21)      /* the largest dim and hidden */
+#define HS_GATED_MLP_MAX_ROWS 0x7fffff80        /* 2^31 - 128: the steps along the rows are counted in 32 bits */
 typedef struct hsGatedMlp {
     const void *x, *w_gate, *w_up, *w_down;
     int64_t ldx, ld_gate, ld_up, ld_down;       /* in elements */

@@ -52,3 +52,14 @@ def test_lookup_work_space_of_an_empty_table():
     for n in (0, 1, 5000, 1 << 20):
         assert f(I64(n), I64(0), I64(16)) == 0 and f(I64(n), I64(5), I64(0)) == 0
     assert f(I64(0), I64(5), I64(16)) >= 8
+
+
+def test_most_rows_of_a_block():
+    """The weight gradients contract over the rows, in steps of 64 counted in 32 bits: the last step must end below 2^31."""
+    most = (1 << 31) - 128
+    for dtype in (0, 1, 2):
+        for f in (lib().hs_gated_mlp_saved_bytes, lib().hs_gated_mlp_fwd_ws_bytes, lib().hs_gated_mlp_bwd_ws_bytes):
+            assert f(gated(rows=most, dtype=dtype, gw_down=256)) >= 0
+            assert all(f(gated(rows=rows, dtype=dtype, gw_down=256)) == -1 for rows in (most + 1, (1 << 31) - 63, (1 << 31) - 1, 1 << 31))
+        for f in (lib().hs_gated_mlp_fwd, lib().hs_gated_mlp_bwd):
+            assert all(f(gated(rows=rows, dtype=dtype, gw_down=256, ws_bytes=1 << 62), None) == -1 for rows in (most + 1, (1 << 31) - 63, (1 << 31) - 1, 1 << 31))
