@@ -358,6 +358,19 @@ __device__ __forceinline__ void multiply_step(A a, B b, R request, f32x4 (&acc)[
     });
 }
 
+// Zeroes a wave's products of the columns from `left` on (counted from its unit 0): the padding columns of H, gg and gu, in the last tile of a row.  Their operand's
+// rows were read as zeros, but zero times an infinity of x or gy is NaN, which the product after the gate would carry into the row's every result.
+template <int MT, int NT> __device__ __forceinline__ void zero_columns(f32x4 (&acc)[MT][NT], int n0, int units, int left, int lq) {
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        if (n < n0 || n >= n0 + units) continue;
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) acc[m][n][r] = (n - n0) * 16 + lq * 4 + r < left ? acc[m][n][r] : 0.f;
+    }
+}
+
 // T: the matrix instruction's type; U: the user's type (float: T = bf16, planes); P: planes in LDS.
 template <typename T, typename U, int P, int BUFS, int BM, int BN, int WI, int WJ, bool AKS, bool BKS, int EPI>
 __global__ __launch_bounds__(64 * WI * WJ) void k_rows_gemm(const Args p) {
@@ -469,10 +482,13 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_rows_gemm(const Args p) {
         }
     } else {
         // A lane has both projections (EPI_GATE) of the same elements, or fetches G and U of its own: the elementwise part is done where the products are, rounded,
-        // and only its results pass through LDS, so that full lines of global memory are written.  Columns up to ldh are written: behind J nothing was
-        // read, so the padding of G, U, H, gg and gu is zero.
+        // and only its results pass through LDS, so that full lines of global memory are written.  Columns up to ldh are written, zeros behind J.
         // (EPI_GATE_FINE and its like, few results: written from where they are, in two planes.)
         constexpr int COLS = DUAL ? TJ : 2 * TJ, N = DUAL ? NT / 2 : NT;
+        if (j0 + TJ > p.J) {        // (uniform)
+            zero_columns(acc, 0, N, p.J - j0 - wj * N * 16, lq);
+            if constexpr (DUAL) zero_columns(acc, N, N, p.J - j0 - wj * N * 16, lq);
+        }
         using St = Staging<U, COLS, TJ, MT, WI, WAVES, DUAL ? MT : 1, BUFS * P * (BM + BN) * BK * 2>;
         f32x4 gq[N], uq[N];
         auto place = [&](int m, int n) {                    // (clamped: nothing branches between the requests)
@@ -695,6 +711,12 @@ __global__ __launch_bounds__(256) void k_gate_bwd(const Args p) {
     // memory are written (131 072 x 256 x 1 024: 369 us; G, U and gH in fp32 through LDS: 381)
     using St = Staging<U, 2 * TJ, TJ, MT, WI, WAVES, MT, 2 * (int)kBuf>;
     const int li = lane & 15, lq = lane >> 4;
+    if (j0 + TJ > p.J) {        // (uniform)
+        const int left = p.J - j0 - wj * N2 * 16;
+        zero_columns(acc, 0, N2, left, lq);
+        zero_columns(acc, N2, N2, left, lq);
+        zero_columns(acc2, 0, N2, left, lq);
+    }
     if constexpr (FINE) {
         with_activation(p.act, [&](auto act) {
 #pragma unroll

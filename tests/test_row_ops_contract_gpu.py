@@ -69,3 +69,29 @@ def test_tracing_is_refused():
     for f in (lambda t: ops().gated_mlp_rows(t, wg, wu, wd), lambda t: ops().embedding_rows(idx, t), lambda t: ops().dropout_rows(t, 0.5, rng)):
         with pytest.raises(RuntimeError, match="cannot be traced"):
             torch.jit.trace(f, (x,))
+
+
+# ------------------------------------------------------------------------------------------------ operands that are not finite
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,D,F", [(40, 64, 100), (40, 64, 104), (300, 264, 130), (300, 1000, 130), (65, 1024, 77), (2100, 33, 250)])
+def test_an_infinity_is_what_the_definition_makes_of_it(M, D, F, dtype):
+    """Positive operands, one infinite element of x and one of the incoming gradient: their rows' results are infinite, not NaN, whatever hidden % 8 is (the
+    columns that fill the last group of eight are multiplied by zeros)."""
+    x, wg, wu, wd, gy = (t.abs() + 2.0 ** -6 for t in gated_inputs(M, D, F, dtype))
+    for t in (x, wg, wu, wd, gy):
+        t[t > 4] = 4
+    scale = 2.0 ** -8
+    x, gy = x * scale, gy * scale              # (finite results stay below 65 504)
+    bad_x, bad_g = M // 2, M - 1
+    x[bad_x, D - 1] = float("inf")
+    gy[bad_g, 0] = float("inf")
+    leaves = [t.clone().requires_grad_() for t in (x, wg, wu, wd)]
+    y = ops().gated_mlp_rows(*leaves, activation="relu")
+    got = [y.detach(), *torch.autograd.grad(y, leaves, gy)]
+    ref = [t.double().clone().requires_grad_() for t in (x, wg, wu, wd)]
+    z = (torch.relu(ref[0] @ ref[1].t()) * (ref[0] @ ref[2].t())) @ ref[3].t()
+    want = [z.detach(), *torch.autograd.grad(z, ref, gy.double())]
+    for a, b, what in zip(got, want, ("y", "gx", "gw_gate", "gw_up", "gw_down")):
+        same = bool((torch.isinf(a) == torch.isinf(b)).all()) and bool((torch.isnan(a) == torch.isnan(b)).all())
+        assert same, what
+    assert bool(torch.isinf(y[bad_x]).all()) and bool(torch.isinf(got[1][bad_g]).all())
