@@ -274,11 +274,12 @@ template <typename F> void gated_call(hsGatedMlp &a, F call, int64_t bytes, cons
     checked(call(&a, stream_of(x)), what);
 }
 
-// y for 2-D rows; saved: receives what the backward pass reads
-Tensor gated(const Tensor &x, const Tensor &wg, const Tensor &wu, const Tensor &wd, int64_t activation, Tensor *saved) {
+// y, of the given shape (its own memory and no view of it: a caller may write a result in place, which autograd refuses for views that a node returns), from 2-D
+// rows; saved: receives what the backward pass reads
+Tensor gated(const Tensor &x, const Tensor &wg, const Tensor &wu, const Tensor &wd, int64_t activation, at::IntArrayRef shape, Tensor *saved) {
     const c10::DeviceGuard guard(x.device());
     hsGatedMlp a = gated_args(x, wg, wu, wd, activation);
-    Tensor y = at::empty({a.rows, a.dim}, x.options());
+    Tensor y = at::empty(shape, x.options());
     a.y = y.mutable_data_ptr();
     if (saved) {
         *saved = bytes_on(x, checked(lib.gated_saved_bytes(&a), "hs_gated_mlp_fwd"));
@@ -298,10 +299,10 @@ struct GatedMlpRows : torch::autograd::Function<GatedMlpRows> {
             return at::zeros_like(x);
         }
         const Tensor rows = as_rows(x), g = as_rows(wg), u = as_rows(wu), d = as_rows(wd);
-        Tensor saved, y = gated(rows, g, u, d, activation, &saved);
+        Tensor saved, y = gated(rows, g, u, d, activation, x.sizes(), &saved);
         ctx->save_for_backward({rows, g, u, d, saved});
         ctx->saved_data["activation"] = activation;
-        return x.dim() == 2 ? y : y.view(x.sizes());
+        return y;
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
         variable_list out(5);
@@ -345,8 +346,7 @@ Tensor gated_mlp_rows(const Tensor &x, const Tensor &wg, const Tensor &wu, const
     TORCH_CHECK(x.size(-1) == 0 || x.numel() / x.size(-1) <= HS_GATED_MLP_MAX_ROWS, "x ", x.sizes(), " has more than ", HS_GATED_MLP_MAX_ROWS, " rows");
     if (recorded({&x, &wg, &wu, &wd})) return GatedMlpRows::apply(x, wg, wu, wd, activation);
     if (x.numel() == 0 || wg.size(0) == 0) return at::zeros_like(x);
-    const Tensor y = gated(as_rows(x), as_rows(wg), as_rows(wu), as_rows(wd), activation, nullptr);
-    return x.dim() == 2 ? y : y.view(x.sizes());
+    return gated(as_rows(x), as_rows(wg), as_rows(wu), as_rows(wd), activation, x.sizes(), nullptr);
 }
 
 }  // namespace

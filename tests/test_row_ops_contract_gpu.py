@@ -95,3 +95,25 @@ def test_an_infinity_is_what_the_definition_makes_of_it(M, D, F, dtype):
         same = bool((torch.isinf(a) == torch.isinf(b)).all()) and bool((torch.isnan(a) == torch.isnan(b)).all())
         assert same, what
     assert bool(torch.isinf(y[bad_x]).all()) and bool(torch.isinf(got[1][bad_g]).all())
+
+
+# ------------------------------------------------------------------------------------------------ results written in place
+@pytest.mark.parametrize("lead", [(6,), (2, 3), (1, 6, 1), ()])
+def test_results_can_be_written_in_place(lead):
+    """The result belongs to the caller: writing it in place is as good as writing a copy, with any number of leading dims."""
+    rows = 1
+    for n in lead:
+        rows *= n
+    x, wg, wu, wd, gy = gated_inputs(rows, 8, 16, torch.float32)
+    table, idx, rng = torch.randn(9, 8, device=DEV), (torch.arange(rows, device=DEV) * 5 % 9).view(lead), torch.tensor([7, 1], device=DEV)
+    x, gy = x.view(*lead, 8), gy.view(*lead, 8)
+    calls = ((lambda t: ops().gated_mlp_rows(t, wg, wu, wd), x), (lambda t: ops().dropout_rows(t, 0.5, rng), x), (lambda t: ops().dropout_rows(t, 0.5, rng, residual=x), x),
+             (lambda t: ops().embedding_rows(idx, t), table))
+    for f, t in calls:
+        leaf = t.clone().requires_grad_()
+        want = f(leaf) * 3 + x
+        want_grad, = torch.autograd.grad(want, leaf, gy)
+        y = f(leaf)
+        y.mul_(3).add_(x)
+        grad, = torch.autograd.grad(y, leaf, gy)
+        assert torch.equal(y, want) and torch.equal(grad, want_grad)
