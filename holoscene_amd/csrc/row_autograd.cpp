@@ -83,13 +83,14 @@ void check_like(const Tensor &t, const char *name, const Tensor &other) {
     TORCH_CHECK(t.scalar_type() == other.scalar_type(), name, " must be a ", other.scalar_type(), " tensor, got ", t.scalar_type());
 }
 
-// [..., n] -> 2-D with consecutive elements in a row: the tensor itself (any row distance >= n), else a copy
+// [..., n] -> 2-D with consecutive elements in a row: the tensor itself (any row distance >= n), else a copy.  (Here and in dropout(): a view that is negated when
+// it is read, such as the imaginary part of a conjugate, is written out first.)
 Tensor as_rows(const Tensor &t) {
-    Tensor r = t;
+    Tensor r = t.resolve_neg();
     if (t.dim() != 2) {
         int64_t rows = 1;
         for (int64_t d = 0; d + 1 < t.dim(); d++) rows *= t.size(d);
-        r = t.reshape({rows, t.size(-1)});
+        r = r.reshape({rows, t.size(-1)});
     }
     if (r.is_contiguous() || ((r.size(1) <= 1 || r.stride(1) == 1) && (r.size(0) <= 1 || r.stride(0) >= r.size(1)))) return r;
     return r.contiguous();
@@ -177,18 +178,18 @@ Tensor embedding_rows(const Tensor &indices, const Tensor &table, double scale, 
     TORCH_CHECK(!padding || (*padding >= 0 && *padding < table.size(0)), "padding_idx ", *padding, " is outside the table's ", table.size(0), " rows");
     const at::ScalarType type = out_type.value_or(table.scalar_type());
     row_type(type, "out_dtype");
-    const Tensor idx = indices.contiguous();
+    const Tensor idx = indices.resolve_neg().contiguous();
     if (!recorded({&table})) return embed(idx, table, scale, type);
     return EmbeddingRows::apply(idx, table, scale, padding.value_or(-1), (int64_t)type);
 }
 
 // ------------------------------------------------------------------------------------------------ dropout
 Tensor dropout(const Tensor &x, const Tensor &residual, int64_t drop, const Tensor &rng) {
-    const Tensor in = x.contiguous();
+    const Tensor in = x.resolve_neg().contiguous();
     Tensor y = at::empty_like(in);
     if (y.numel() == 0) return y;
     const c10::DeviceGuard guard(in.device());
-    const Tensor r = residual.defined() ? residual.contiguous() : residual;
+    const Tensor r = residual.defined() ? residual.resolve_neg().contiguous() : residual;
     checked(lib.dropout_rows(in.const_data_ptr(), r.defined() ? r.const_data_ptr() : nullptr, y.mutable_data_ptr(), in.numel(), row_type(in.scalar_type(), "x"), (int32_t)drop,
                              (const uint64_t *)rng.const_data_ptr(), stream_of(in)), "hs_dropout_rows");
     return y;
@@ -234,7 +235,7 @@ Tensor dropout_rows(const Tensor &x, double p, const Tensor &rng, const std::opt
     row_type(x.scalar_type(), "x");
     check_dense(rng, "rng");
     TORCH_CHECK(rng.device() == x.device(), "rng is on ", rng.device(), ", expected ", x.device());
-    TORCH_CHECK(rng.scalar_type() == at::kLong && rng.dim() == 1 && rng.size(0) == 2 && rng.is_contiguous(), "rng must be two consecutive int64 (seed, number of the call)");
+    TORCH_CHECK(rng.scalar_type() == at::kLong && rng.dim() == 1 && rng.size(0) == 2 && rng.is_contiguous() && !rng.is_neg(), "rng must be two consecutive int64 (seed, number of the call)");
     if (residual) {
         check_like(*residual, "residual", x);
         TORCH_CHECK(residual->sizes() == x.sizes(), "residual ", residual->sizes(), " must have x's shape ", x.sizes());

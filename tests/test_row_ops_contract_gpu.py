@@ -117,3 +117,26 @@ def test_results_can_be_written_in_place(lead):
         y.mul_(3).add_(x)
         grad, = torch.autograd.grad(y, leaf, gy)
         assert torch.equal(y, want) and torch.equal(grad, want_grad)
+
+
+# ------------------------------------------------------------------------------------------------ lazily negated operands
+@pytest.mark.parametrize("lazy", [lambda t: torch.complex(torch.zeros_like(t), -t).conj().imag, lambda t: torch._neg_view(-t)], ids=["conjugate", "contiguous"])
+@pytest.mark.parametrize("D", [1, 8])
+def test_lazily_negated_operands(lazy, D):
+    """The imaginary part of a conjugate is a view whose elements are negated when they are read."""
+    x, wg, wu, wd, gy = gated_inputs(6, D, 7, torch.float32)
+    table, rng, idx = gated_inputs(6, D, 7, torch.float32, seed=1)[0], torch.tensor([2, 9], device=DEV), torch.tensor([0, 3, 3, 1, 2, 5], device=DEV)
+    assert lazy(x).is_neg() and torch.equal(lazy(x), x)
+    f, args = ops().gated_mlp_rows, [x, wg, wu, wd]
+    for i in range(4):
+        assert torch.equal(f(*[lazy(t) if k == i else t for k, t in enumerate(args)]), f(*args)), i
+    assert torch.equal(ops().dropout_rows(lazy(x), 0.25, rng, residual=lazy(gy)), ops().dropout_rows(x, 0.25, rng, residual=gy))
+    assert torch.equal(ops().embedding_rows(idx, lazy(table)), table[idx])
+    assert torch.equal(ops().embedding_rows(torch._neg_view(-idx), table), table[idx])
+    with pytest.raises(RuntimeError, match="rng"):
+        ops().dropout_rows(x, 0.25, torch._neg_view(-rng))
+    for g, leaf in ((lambda t: f(t, wg, wu, wd), x), (lambda t: ops().dropout_rows(t, 0.25, rng), x), (lambda t: ops().embedding_rows(idx, t), table)):
+        leaf = leaf.clone().requires_grad_()
+        want, = torch.autograd.grad(g(leaf), leaf, gy)
+        got, = torch.autograd.grad(g(leaf), leaf, lazy(gy))
+        assert torch.equal(got, want)
