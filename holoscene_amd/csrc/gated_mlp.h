@@ -266,6 +266,7 @@ template <typename T, typename U> struct Block {
             q.seg[0][1] = q.seg[0][0];
             q.seg[0][0].a = plane1(sv.h);        // (the smaller plane's product first)
             q.n_seg = 2;
+            q.low_seg = 1;
         }
         result<false, false>(q, &a.y, 1);
         reduce();
@@ -323,6 +324,7 @@ template <typename T, typename U> struct Block {
                 else p.seg[z][0].b = plane1(b);
             }
             p.n_seg = 2;
+            p.low_seg = 1;
         }
         result<true, true>(p, out, problems);
     }
@@ -363,6 +365,7 @@ template <typename T, typename U> struct Block {
                     p.seg[0][0].a = plane1(gg);
                     p.seg[0][1].a = plane1(gu);
                     p.n_seg = 4;
+                    p.low_seg = 2;
                 }
                 result<false, true>(p, &a.gx, 1);
             }

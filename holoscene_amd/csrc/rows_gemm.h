@@ -53,6 +53,7 @@ struct Seg { const void *a, *b, *b1; };          // b1: the up projection's weig
 struct Args {
     Seg seg[2][kMaxSeg];                          // [problem][segment]
     int32_t n_seg;
+    int32_t low_seg;                              // how many of them, the first ones, are products of an operand's lower plane (16-bit types, fine() in gated_mlp.h)
     int64_t lda, ldb;                             // in elements, multiples of 8
     int64_t plane_a, plane_b;                     // bytes between planes
     int64_t I;
@@ -371,6 +372,16 @@ template <int MT, int NT> __device__ __forceinline__ void zero_columns(f32x4 (&a
     }
 }
 
+__device__ __forceinline__ float finite_part(float v) { return __builtin_isfinite(v) ? v : 0.f; }
+template <int MT, int NT> __device__ __forceinline__ void finite_part(f32x4 (&acc)[MT][NT]) {
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) acc[m][n][r] = finite_part(acc[m][n][r]);
+}
+
 // T: the matrix instruction's type; U: the user's type (float: T = bf16, planes); P: planes in LDS.
 template <typename T, typename U, int P, int BUFS, int BM, int BN, int WI, int WJ, bool AKS, bool BKS, int EPI>
 __global__ __launch_bounds__(64 * WI * WJ) void k_rows_gemm(const Args p) {
@@ -438,7 +449,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_rows_gemm(const Args p) {
     constexpr int kAhead = (BUFS - 2) * P * (SA::kReq + SB::kReq);       // a wave's requests for the steps after this one
     static_assert(kAhead < 64, "the wait counts to 63");
     int buf = 0;
-    for (int s = s_begin; s < s_end; s++) {
+    auto step = [&](int s) {
         if (s + BUFS - 2 < s_end) wait_and_meet<kAhead>();
         else wait_and_meet<0>();
         const uint32_t at = lds0 + (uint32_t)buf * kBuf, at_b = at + P * SA::kBytes;
@@ -449,6 +460,20 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_rows_gemm(const Args p) {
             },
             [&]() { if (s + BUFS - 1 < s_end) request(buf == 0 ? BUFS - 1 : buf - 1); }, acc, low);
         buf = buf + 1 == BUFS ? 0 : buf + 1;
+    };
+    if constexpr ((EPI == EPI_STORE || EPI == EPI_PARTIAL) && sizeof(U) == 2) {
+        // lower planes first; an infinity among the other operand's elements makes any value of theirs, zero among them: what is not finite then is left to the
+        // upper planes, whose product says what it is
+        const int low_end = p.low_seg * steps_k < s_end ? p.low_seg * steps_k : s_end;
+        int s = s_begin;
+#pragma unroll 1
+        for (int part = low_end > s_begin ? 0 : 1; part < 2; part++) {
+            const int stop = part == 0 ? low_end : s_end;
+            for (; s < stop; s++) step(s);
+            if (part == 0) finite_part(acc);
+        }
+    } else {
+        for (int s = s_begin; s < s_end; s++) step(s);
     }
     if constexpr (P == 3) {
 #pragma unroll

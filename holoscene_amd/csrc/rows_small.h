@@ -127,7 +127,13 @@ __global__ __launch_bounds__(64 * WAVES) void k_rows_small(const SmallArgs p) {
 #pragma unroll
     for (int w = 0; w < NW; w++)
 #pragma unroll
-        for (int t = 0; t < TOK; t++) join[wave][w * TOK + t][lane] = PX > 1 ? acc[w][t] + low[w][t] : acc[w][t];
+        for (int t = 0; t < TOK; t++) {
+            if constexpr (P == 1 && PX == 2) {          // (an infinite weight times H's lower plane: any value, see rows_gemm.h)
+#pragma unroll
+                for (int e = 0; e < 4; e++) low[w][t][e] = finite_part(low[w][t][e]);
+            }
+            join[wave][w * TOK + t][lane] = PX > 1 ? acc[w][t] + low[w][t] : acc[w][t];
+        }
     __syncthreads();
     // a wave per 16 rows of x: row t 16 + r, results n0 + 4 q ..
     for (int t = wave; t < TOK; t += WAVES) {

@@ -97,6 +97,30 @@ def test_an_infinity_is_what_the_definition_makes_of_it(M, D, F, dtype):
     assert bool(torch.isinf(y[bad_x]).all()) and bool(torch.isinf(got[1][bad_g]).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("where", ["x and gradient", "w_gate", "w_up", "w_down"])
+@pytest.mark.parametrize("M,D,F", [(1, 1, 1), (5, 24, 13), (20, 100, 300), (70, 24, 9), (70, 800, 1), (70, 1024, 2), (1, 2040, 300), (20000, 16, 100), (4001, 33, 60)])
+def test_an_infinity_beside_two_planes(M, D, F, where, dtype):
+    """Few results: H, gg and gu in two planes, the lower of which is any small number, zero among them, where the definition has one finite factor."""
+    x, wg, wu, wd, gy = (t.abs().clamp(2.0 ** -6, 4) for t in gated_inputs(M, D, F, dtype))
+    x, gy = x * 2.0 ** -8, gy * 2.0 ** -8
+    if where == "x and gradient":
+        x[M // 2, D - 1] = float("inf")
+        gy[M - 1, 0] = float("inf")
+    else:
+        t = {"w_gate": wg, "w_up": wu, "w_down": wd}[where]
+        t[t.shape[0] // 2, t.shape[1] // 3] = float("inf")
+    leaves = [t.clone().requires_grad_() for t in (x, wg, wu, wd)]
+    y = ops().gated_mlp_rows(*leaves, activation="relu")
+    got = [y.detach(), *torch.autograd.grad(y, leaves, gy)]
+    ref = [t.double().clone().requires_grad_() for t in (x, wg, wu, wd)]
+    z = (torch.relu(ref[0] @ ref[1].t()) * (ref[0] @ ref[2].t())) @ ref[3].t()
+    want = [z.detach(), *torch.autograd.grad(z, ref, gy.double())]
+    for a, b, what in zip(got, want, ("y", "gx", "gw_gate", "gw_up", "gw_down")):
+        same = bool((torch.isinf(a) == torch.isinf(b)).all()) and bool((torch.isnan(a) == torch.isnan(b)).all())
+        assert same, what
+
+
 # ------------------------------------------------------------------------------------------------ results written in place
 @pytest.mark.parametrize("lead", [(6,), (2, 3), (1, 6, 1), ()])
 def test_results_can_be_written_in_place(lead):
