@@ -157,6 +157,7 @@ __device__ __forceinline__ F8 load8(const float *p) {
 }
 // four elements of an operand of a 16-bit type in two planes, v = p0 + p1 up to the square of the type's rounding; an infinity or NaN stays in plane 0 alone
 template <typename U> __device__ __forceinline__ void split2(float v, U (&p)[2]) {
+    asm("" : "+v"(v));          // (both planes from this float: the compiler would round a product to float16 from its exact value in one place and from the float in another)
     p[0] = from_f32<U>(v);
     p[1] = __builtin_isfinite(to_f32(p[0])) ? from_f32<U>(v - to_f32(p[0])) : (U)0.f;
 }

@@ -164,3 +164,30 @@ def test_lazily_negated_operands(lazy, D):
         want, = torch.autograd.grad(g(leaf), leaf, gy)
         got, = torch.autograd.grad(g(leaf), leaf, lazy(gy))
         assert torch.equal(got, want)
+
+
+# ------------------------------------------------------------------------------------------------ two planes
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M", [2, 20, 40, 100])
+@pytest.mark.parametrize("D", [8, 100, 1000])
+def test_the_lower_plane_is_what_the_upper_one_leaves(D, M, dtype):
+    """Few results, H, gg and gu in two planes.  Gate and up projection are 1 + 2^-12 in one row and 1 in another: H there is (1 + 2^-12)^2, which as a float lies
+    half way between two neighbours in float16 and unrounded does not, and both values must come from one rounding of it."""
+    F = 2
+    x, wg, wd, gy = (torch.zeros(s, dtype=dtype, device=DEV) for s in ((M, D), (F, D), (D, F), (M, D)))
+    x[:, 0] = 1
+    x[M - 1, 1] = wg[:, 1].fill_(2.0 ** -6)[0]
+    wg[:, 0] = 1
+    wd[0] = 1
+    gy[M - 1, 0], gy[0, 0] = 1, -1
+    leaves = [t.clone().requires_grad_() for t in (x, wg, wg, wd)]
+    for act in ("relu", "silu", "gelu"):
+        gx, gwg, gwu, gwd = torch.autograd.grad(ops().gated_mlp_rows(*leaves, activation=act), leaves, gy)
+        ref = [t.detach().double().requires_grad_() for t in leaves]
+        fn = dict(relu=torch.relu, silu=torch.nn.functional.silu, gelu=torch.nn.functional.gelu)[act]
+        want = torch.autograd.grad((fn(ref[0] @ ref[1].t()) * (ref[0] @ ref[2].t())) @ ref[3].t(), ref, gy.double())
+        e = torch.finfo(dtype).eps / 2
+        # each term, at most 1.3, is off by the square of the rounding and by the activation's fp32 arithmetic (8 2^-24 of 1 + |g|); their difference by a rounding too
+        for got, exact, what in ((gwg, want[1], "gw_gate"), (gwu, want[2], "gw_up"), (gwd.t(), want[3].t(), "gw_down")):
+            err = (got[:, 0].double() - exact[:, 0]).abs().max()
+            assert float(err) <= 2 * 1.3 * (e * e + 20 * 2.0 ** -24) + e * float(exact[:, 0].abs().max()), (act, what)
