@@ -163,12 +163,18 @@ template <typename T, typename U> struct Block {
 
     void check(int r) { if (rc == HS_OK) rc = r; }
 
-    // H, gg and gu of the 16-bit types in two planes where a result has few elements: rounded once they bring as much error into a result as its own rounding, 1.4 times
-    // in all over many elements, but over few of them anything up to twice; in two planes nothing that shows.  The steps of the products that read them
-    // double, which so small ones do not feel (a step of 1 x 32 x 2 976 bf16 is bound by the host); 1 x 4 096 x 12 288, where reading the weights is all there is,
-    // would: down projection 25.1 -> 28.4 us (eight waves a workgroup).
+    // H, gg and gu of the 16-bit types in one plane or two.  Rounded once they bring as much error into every result as its own rounding, 1.41 times in all; in two
+    // planes nothing that shows (distance from 64 bits over that of one rounding: 1.41 and 1.00 at 300 x 256 x 1 024 and 2 000 x 512 x 1 500).  The products that read
+    // them double.  bf16, one plane and two, forward and step in us: 8 192 x 4 096 x 12 288 1 912 / 3 830 and 6 182 / 12 514, 131 072 x 256 x 1 024 297 / 554 and
+    // 1 083 / 1 820, 1 021 x 1 000 x 2 730 44 / 59 and 133 / 185.  The caller chooses (HS_GATED_ONE_PLANE, HS_GATED_TWO_PLANES); without a choice it is two where a
+    // result has so few elements that their error is no average (32 of 1 x 32 x 2 976: anything from 1.2 to 1.8), and most such blocks are bound by the
+    // host: 2 x 1 024 x 2 816 10.9 / 11.8 and 82.8 / 84.1, 2 000 x 46 x 44 13.5 / 12.8 and 90.8 / 90.5; with weights to read 1 x 2 048 x 12 288 33.5 / 36.8 and
+    // 150 / 180; many narrow rows pay the most, 131 072 x 8 x 250 50 / 91 and 181 / 362.
     static constexpr int64_t kFineResults = 2048;
-    bool fine() const { return sizeof(U) == 2 && (M < F ? M : F) * D <= kFineResults; }
+    bool fine() const {
+        if (sizeof(U) == 4 || (a.activation & HS_GATED_ONE_PLANE)) return false;
+        return (a.activation & HS_GATED_TWO_PLANES) || (M < F ? M : F) * D <= kFineResults;
+    }
     int inner_planes() const { return fine() ? 2 : planes<U>(); }
     template <typename O> static const void *plane1(const O &o) { return (const char *)o.p + o.plane * 2; }        // (of an operand in two planes of 16 bits)
 
@@ -226,7 +232,7 @@ template <typename T, typename U> struct Block {
         }
         if (!run || rc != HS_OK) return;
         SmallArgs p = {};
-        p.x = a.x; p.w = a.w_gate; p.w1 = a.w_up; p.ldx = a.ldx; p.ldw = a.ld_gate; p.ldw1 = a.ld_up; p.M = (int)M; p.N = (int)F; p.K = (int)D; p.act = a.activation;
+        p.x = a.x; p.w = a.w_gate; p.w1 = a.w_up; p.ldx = a.ldx; p.ldw = a.ld_gate; p.ldw1 = a.ld_up; p.M = (int)M; p.N = (int)F; p.K = (int)D; p.act = a.activation & 0xff;
         p.g = sv.g; p.u = sv.u; p.h = (void *)sv.h.p; p.ldh = ldh; p.plane = sv.h.plane;
         if constexpr (sizeof(U) == 2) {
             if (fine()) check(launch_small<T, U, EPI_GATE, true>(p, s));
@@ -256,7 +262,7 @@ template <typename T, typename U> struct Block {
         pack();
         Args p = product(x, wg, M, F, D);
         p.seg[0][0].b1 = wu.p;
-        p.g = sv.g; p.u = sv.u; p.h = (void *)sv.h.p; p.ldh = ldh; p.plane = sv.h.plane; p.act = a.activation;
+        p.g = sv.g; p.u = sv.u; p.h = (void *)sv.h.p; p.ldh = ldh; p.plane = sv.h.plane; p.act = a.activation & 0xff;
         if (run && rc == HS_OK) {
             if (!fine()) check(launch_product<T, U, false, false, EPI_GATE>(p, plan_product<U>(M, 2 * ldh, steps(D), 1, false).tile, 1, s));
             else if constexpr (sizeof(U) == 2) check(launch_tile<T, U, 1, 2, 64, 64, 2, 2, false, false, EPI_GATE_FINE>(p, 1, s));
@@ -343,7 +349,7 @@ template <typename T, typename U> struct Block {
             const Operand gg{ws.take(n * 2 * inner_planes()), ldh, n}, gu{ws.take(n * 2 * inner_planes()), ldh, n};
             if (run && rc == HS_OK) {
                 Args p = again() ? product(x, wg, M, F, D) : product(gy, wd, M, F, D);
-                p.g = sv.g; p.u = sv.u; p.gg = (void *)gg.p; p.gu = (void *)gu.p; p.ldh = ldh; p.plane = n; p.act = a.activation;
+                p.g = sv.g; p.u = sv.u; p.gg = (void *)gg.p; p.gu = (void *)gu.p; p.ldh = ldh; p.plane = n; p.act = a.activation & 0xff;
                 if (again()) {
                     p.seg[0][0].b1 = wu.p;
                     p.seg[1][0] = Seg{gy.p, wd.p, nullptr};

@@ -3,9 +3,15 @@
 
 namespace {
 
+// an activation, and for the 16-bit types one of the flags at most
+bool activation_ok(const hsGatedMlp &a) {
+    const int32_t planes = a.activation & ~0xff;
+    return (a.activation & 0xff) <= HS_ACT_RELU && (planes == 0 || (a.dtype != HS_F32 && (planes == HS_GATED_ONE_PLANE || planes == HS_GATED_TWO_PLANES)));
+}
+
 bool sizes_ok(const hsGatedMlp &a) {
     return a.rows > 0 && a.dim > 0 && a.hidden > 0 && a.rows <= HS_GATED_MLP_MAX_ROWS && a.dim <= HS_GATED_MLP_MAX && a.hidden <= HS_GATED_MLP_MAX && a.ldx >= a.dim && a.ld_gate >= a.dim &&
-           a.ld_up >= a.dim && a.ld_down >= a.hidden && a.activation >= 0 && a.activation <= HS_ACT_RELU && hs_row::known_dtype(a.dtype);
+           a.ld_up >= a.dim && a.ld_down >= a.hidden && hs_row::known_dtype(a.dtype) && activation_ok(a);
 }
 
 int64_t call(const hsGatedMlp &a, int what, hipStream_t s) {

@@ -345,6 +345,7 @@ Tensor gated_mlp_rows(const Tensor &x, const Tensor &wg, const Tensor &wu, const
                 "x ", x.sizes(), ", w_gate ", wg.sizes(), ", w_up ", wu.sizes(), ", w_down ", wd.sizes(), ": expected [..., dim], [hidden, dim], [hidden, dim], [dim, hidden]");
     TORCH_CHECK(wg.size(0) <= HS_GATED_MLP_MAX && wg.size(1) <= HS_GATED_MLP_MAX, "dim ", wg.size(1), " and hidden ", wg.size(0), " must be at most ", HS_GATED_MLP_MAX);
     TORCH_CHECK(x.size(-1) == 0 || x.numel() / x.size(-1) <= HS_GATED_MLP_MAX_ROWS, "x ", x.sizes(), " has more than ", HS_GATED_MLP_MAX_ROWS, " rows");
+    TORCH_CHECK(activation < HS_GATED_ONE_PLANE || x.scalar_type() != at::kFloat, "planes is for the 16-bit types: a float32 operand is always three bf16 planes");
     if (recorded({&x, &wg, &wu, &wd})) return GatedMlpRows::apply(x, wg, wu, wd, activation);
     if (x.numel() == 0 || wg.size(0) == 0) return at::zeros_like(x);
     return gated(as_rows(x), as_rows(wg), as_rows(wu), as_rows(wd), activation, x.sizes(), nullptr);

@@ -151,6 +151,7 @@ _ROW_ENTRIES = ("hs_embed_fwd", "hs_embed_bwd_ws_bytes", "hs_embed_bwd", "hs_dro
                 "hs_gated_mlp_fwd", "hs_gated_mlp_bwd")
 _ROW_BYTES = ("hs_embed_bwd_ws_bytes", "hs_gated_mlp_saved_bytes", "hs_gated_mlp_fwd_ws_bytes", "hs_gated_mlp_bwd_ws_bytes")      # sizes, or a negative error
 ROW_ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "sigmoid": 3, "relu": 4}       # HS_ACT_*
+ROW_PLANES = {None: 0, 1: 0x100, 2: 0x200}      # HS_GATED_ONE_PLANE, HS_GATED_TWO_PLANES
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}  # HS_F32 / HS_BF16
 
 

@@ -37,19 +37,25 @@ def embedding_rows(indices, table, scale=1.0, padding_idx=None, out_dtype=None):
     return _be.row_autograd().embedding_rows(indices, table, scale, padding_idx, out_dtype)
 
 
-def gated_mlp_rows(x, w_gate, w_up, w_down, activation="silu"):
+def gated_mlp_rows(x, w_gate, w_up, w_down, activation="silu", planes=None):
     """(act(x Wg^T) * (x Wu^T)) Wd^T for x [..., dim], w_gate and w_up [hidden, dim], w_down [dim, hidden], all of one type.
 
     dim and hidden are at most 2^21.  activation: "silu", "gelu" (g Phi(g)), "gelu_tanh" (its tanh form), "sigmoid", "relu".  float32 operands are
     multiplied as three bf16 planes each (24 bits, as linear_rows under HOLOSCENE_FP32_GEMM=split3; an infinity among them gives NaN).  Rows may be
     strided; 16-bit operands whose rows are not 16-byte aligned are copied once per call.  The forward keeps the gated product for the backward pass, and both
     projections in fp32 where reading them back costs less than computing them again (dim > 768, in float32 > 128).  The gated product and its two
-    gradients are rounded to x's type between the products: in float16 they are infinite beyond 65 504."""
+    gradients are rounded to x's type between the products: in float16 they are infinite beyond 65 504, and less than 3e-8 is zero.
+
+    planes (bfloat16 and float16): in how many values of the type each element of these three is held -- 1: results are 1.4 times as far from exact as their own
+    rounding takes them; 2: no further than that, for up to twice the time; None: 2 where results are few (min(rows, hidden) dim <= 2 048), else 1.  float32
+    always holds them in its three planes."""
     for t, name in ((x, "x"), (w_gate, "w_gate"), (w_up, "w_up"), (w_down, "w_down")):
         _check_tensor(t, name)
     if activation not in _be.ROW_ACTIVATIONS:
         raise RuntimeError(f"activation must be one of {', '.join(ACTIVATIONS)}, got {activation!r}")
-    return _be.row_autograd().gated_mlp_rows(x, w_gate, w_up, w_down, _be.ROW_ACTIVATIONS[activation])
+    if planes not in _be.ROW_PLANES:
+        raise RuntimeError(f"planes must be None, 1 or 2, got {planes!r}")
+    return _be.row_autograd().gated_mlp_rows(x, w_gate, w_up, w_down, _be.ROW_ACTIVATIONS[activation] | _be.ROW_PLANES[planes])
 
 
 def dropout_rows(x, p, rng, residual=None):
@@ -84,17 +90,19 @@ class RowEmbedding(nn.Module):
 class GatedMLP(nn.Module):
     """The gated feed-forward block (gated_mlp_rows) with its three weights."""
 
-    def __init__(self, dim, hidden, activation="silu"):
+    def __init__(self, dim, hidden, activation="silu", planes=None):
         super().__init__()
+        if planes not in _be.ROW_PLANES:
+            raise ValueError(f"planes must be None, 1 or 2, got {planes!r}")
         if activation not in _be.ROW_ACTIVATIONS:
             raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}, got {activation!r}")
-        self.activation = activation
+        self.activation, self.planes = activation, planes
         self.w_gate = nn.Parameter(nn.Linear(dim, hidden, bias=False).weight.detach().clone())
         self.w_up = nn.Parameter(nn.Linear(dim, hidden, bias=False).weight.detach().clone())
         self.w_down = nn.Parameter(nn.Linear(hidden, dim, bias=False).weight.detach().clone())
 
     def forward(self, x):
-        return gated_mlp_rows(x, self.w_gate, self.w_up, self.w_down, self.activation)
+        return gated_mlp_rows(x, self.w_gate, self.w_up, self.w_down, self.activation, self.planes)
 
 
 class RowDropout(nn.Module):

@@ -917,6 +917,10 @@ int hs_dropout_rows(const void *x, const void *residual, void *y, int64_t n, int
 #define HS_ACT_GELU_TANH 2
 #define HS_ACT_SIGMOID 3
 #define HS_ACT_RELU 4
+/* Added to the activation (16-bit types): H, gg and gu are held in one or in two values of the type an element between the products, in the forward and in its
+ * backward alike.  Neither: two where min(rows, hidden) dim <= 2048, else one. */
+#define HS_GATED_ONE_PLANE 0x100
+#define HS_GATED_TWO_PLANES 0x200
 #define HS_GATED_MLP_MAX (1 << 21)      /* the largest dim and hidden */
 #define HS_GATED_MLP_MAX_ROWS 0x7fffff80        /* 2^31 - 128: the steps along the rows are counted in 32 bits */
 typedef struct hsGatedMlp {

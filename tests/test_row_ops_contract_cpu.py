@@ -63,3 +63,24 @@ def test_most_rows_of_a_block():
             assert all(f(gated(rows=rows, dtype=dtype, gw_down=256)) == -1 for rows in (most + 1, (1 << 31) - 63, (1 << 31) - 1, 1 << 31))
         for f in (lib().hs_gated_mlp_fwd, lib().hs_gated_mlp_bwd):
             assert all(f(gated(rows=rows, dtype=dtype, gw_down=256, ws_bytes=1 << 62), None) == -1 for rows in (most + 1, (1 << 31) - 63, (1 << 31) - 1, 1 << 31))
+
+
+# ------------------------------------------------------------------------------------------------ planes
+def test_planes_refusals_and_sizes():
+    one, two = 0x100, 0x200
+    f = lib().hs_gated_mlp_saved_bytes
+    for act in range(5):
+        assert f(gated(activation=act | one)) < f(gated(activation=act | two)) == f(gated(activation=act))        # (4 x 16: few results)
+        wide = dict(rows=500, dim=16, hidden=32)
+        big = dict(rows=5000, dim=256, ldx=256, ld_gate=256, ld_up=256)
+        assert f(gated(activation=act | one, **wide)) < f(gated(activation=act | two, **wide))
+        assert f(gated(activation=act | one, **big)) == f(gated(activation=act, **big)) < f(gated(activation=act | two, **big))
+    for bad in (5, 5 | one, one | two, 0x400, 0x10000 | one, -1):
+        assert f(gated(activation=bad)) == -1 and lib().hs_gated_mlp_fwd(gated(activation=bad), None) == -1 and lib().hs_gated_mlp_bwd(gated(activation=bad), None) == -1
+    assert f(gated(activation=one, dtype=0)) == -1 and f(gated(activation=two, dtype=0)) == -1        # (fp32: always three)
+    t = torch.zeros(4, 8)
+    for planes in (0, 3, "two"):
+        with pytest.raises(RuntimeError, match="planes must be"):
+            row_ops.gated_mlp_rows(t, t, t, t.t(), planes=planes)
+        with pytest.raises(ValueError, match="planes must be"):
+            row_ops.GatedMLP(8, 16, planes=planes)

@@ -191,3 +191,99 @@ def test_the_lower_plane_is_what_the_upper_one_leaves(D, M, dtype):
         for got, exact, what in ((gwg, want[1], "gw_gate"), (gwu, want[2], "gw_up"), (gwd.t(), want[3].t(), "gw_down")):
             err = (got[:, 0].double() - exact[:, 0]).abs().max()
             assert float(err) <= 2 * 1.3 * (e * e + 20 * 2.0 ** -24) + e * float(exact[:, 0].abs().max()), (act, what)
+
+
+# ------------------------------------------------------------------------------------------------ what is rounded, and how often
+H32 = 2.0 ** -24
+
+
+def block_bounds(x, wg, wu, wd, act, gy, planes):
+    """(value in 64 bits, bound) of y, gx, gWg, gWu, gWd, in 2-D operands: fp32 sums (k 2^-24 of the sum of magnitudes, counted twice for the matrix instruction's own
+    order and roundings), H, gg and gu rounded once in `planes` values of the type (3: fp32's planes, to 2^-24), G and U not at all, each result rounded once."""
+    t = x.dtype
+    e, under = torch.finfo(t).eps / 2, {torch.float32: 2.0 ** -150, torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25}[t]
+    e_in = H32 if planes == 3 else e ** planes         # (a second value holds what the first left, to half a step of that)
+    x, wg, wu, wd, gy = (v.detach().double() for v in (x, wg, wu, wd, gy))
+    M, D, F = x.shape[0], x.shape[1], wg.shape[0]
+
+    def mm(a, da, b, k):                # of a known to da, b exact
+        return a @ b, da @ b.abs() + (k + 16) * 2 * H32 * ((a.abs() + da) @ b.abs())
+
+    def times(*parts):                  # product of (value, error) pairs in fp32
+        val, err = parts[0]
+        for v, d in parts[1:]:
+            val, err = val * v, err * (v.abs() + d) + val.abs() * d
+        return val, err + 3 * H32 * (val.abs() + err)
+
+    def rounded(v, d, step):
+        return v, d + step * (v.abs() + d) + under
+    zero = torch.zeros((), dtype=torch.float64, device=x.device)
+    g, u = mm(x, zero.expand_as(x), wg.t(), D), mm(x, zero.expand_as(x), wu.t(), D)
+    leaf = g[0].clone().requires_grad_()
+    fn = dict(silu=torch.nn.functional.silu, relu=torch.relu)[act]
+    value = fn(leaf)
+    slope, = torch.autograd.grad(value.sum(), leaf)
+    own = 8 * H32 * (1 + g[0].abs())    # the activation's fp32 arithmetic
+    flips = (g[0].abs() <= g[1]).double() if act == "relu" else 0.0
+    a = value.detach(), dict(silu=1.1, relu=1.0)[act] * g[1] + own
+    s = slope, dict(silu=0.5, relu=0.0)[act] * g[1] + own + flips
+    h = rounded(*times(a, u), e_in)
+    gh = mm(gy, zero.expand_as(gy), wd, D)
+    gg, gu = rounded(*times(gh, u, s), e_in), rounded(*times(gh, a), e_in)
+    gx1, gx2 = mm(*gg, wg, 2 * F), mm(*gu, wu, 2 * F)
+    gwd, dgwd = mm(h[0].t(), h[1].t(), gy, M)
+    return [rounded(*p, e) for p in (mm(*h, wd.t(), F), (gx1[0] + gx2[0], gx1[1] + gx2[1]), mm(gg[0].t(), gg[1].t(), x, M), mm(gu[0].t(), gu[1].t(), x, M), (gwd.t(), dgwd.t()))]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("planes", [None, 1, 2])
+@pytest.mark.parametrize("M,D,F", [(1, 8, 8), (1, 2048, 24), (1, 2049, 24), (13, 250, 170), (31, 264, 40), (33, 130, 65), (70, 72, 130), (300, 264, 157), (70, 1000, 300), (2500, 96, 777), (1500, 1001, 65)])
+def test_planes_hold_what_they_say(M, D, F, planes, dtype):
+    if dtype == torch.float32 and planes is not None:
+        with pytest.raises(RuntimeError, match="16-bit types"):
+            ops().gated_mlp_rows(*gated_inputs(M, D, F, dtype)[:4], planes=planes)
+        return
+    act = "relu" if (M + D) % 2 else "silu"
+    x, wg, wu, wd, gy = gated_inputs(M, D, F, dtype, seed=3)
+    leaves = [t.clone().requires_grad_() for t in (x, wg, wu, wd)]
+    y = ops().gated_mlp_rows(*leaves, activation=act, planes=planes)
+    with torch.no_grad():
+        assert torch.equal(ops().gated_mlp_rows(x, wg, wu, wd, activation=act, planes=planes), y)
+    held = 3 if dtype == torch.float32 else planes or (2 if min(M, F) * D <= 2048 else 1)
+    for got, (want, bound), what in zip((y, *torch.autograd.grad(y, leaves, gy)), block_bounds(x, wg, wu, wd, act, gy, held), ("y", "gx", "gw_gate", "gw_up", "gw_down")):
+        bad = (got.double() - want).abs() > bound
+        assert not bool(bad.any()), f"{what}: {int(bad.sum())} of {bad.numel()}, by at most {float(((got.double() - want).abs() / bound).max()):.2f} bounds"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M", [2, 40, 300])
+@pytest.mark.parametrize("D", [8, 1000, 1024])
+def test_projections_are_not_rounded(D, M, dtype):
+    """G and U are 1 + 2^-12 in one row and 1 in another, both 1 in a 16-bit type: what a difference of the rows leaves shows whether they were kept."""
+    F = 16
+    x, wg, wd, gy = (torch.zeros(s, dtype=dtype, device=DEV) for s in ((M, D), (F, D), (D, F), (M, D)))
+    x[:, 0] = 1
+    x[M - 1, 1] = wg[:, 1].fill_(2.0 ** -6)[0]
+    wg[:, 0] = 1
+    wd[0] = 1
+    gy[M - 1, 0], gy[0, 0] = 1, -1
+    leaves = [t.clone().requires_grad_() for t in (x, wg, wg, wd)]
+    y = ops().gated_mlp_rows(*leaves, activation="relu", planes=2)
+    gx, gwg, gwu, gwd = torch.autograd.grad(y, leaves, gy)
+    assert bool((gwg[:, 0] == 2.0 ** -12).all()) and bool((gwu[:, 0] == 2.0 ** -12).all())
+    assert bool((gwd[0] == 2.0 ** -11).all())                      # (1 + 2^-12)^2 - 1, rounded to the type
+    # and in one plane, as the docstring says, they do not show
+    one = torch.autograd.grad(ops().gated_mlp_rows(*leaves, activation="relu", planes=1), leaves, gy)
+    assert not bool(one[1][:, 0].any()) and not bool(one[2][:, 0].any())
+
+
+def test_planes_of_the_module():
+    x, wg, wu, wd, _ = gated_inputs(200, 64, 96, torch.bfloat16)
+    mods = [ops().GatedMLP(64, 96, "silu", planes=p).to(DEV, torch.bfloat16) for p in (None, 1, 2)]
+    for m in mods:
+        with torch.no_grad():
+            for p, w in ((m.w_gate, wg), (m.w_up, wu), (m.w_down, wd)):
+                p.copy_(w)
+    y = [m(x) for m in mods]
+    assert torch.equal(y[0], y[1]) and not torch.equal(y[1], y[2])
+    assert all(torch.equal(y[k], ops().gated_mlp_rows(x, wg, wu, wd, "silu", planes=p)) for k, p in enumerate((None, 1, 2)))
