@@ -3,7 +3,7 @@
 
 extern "C" {
 
-int hs_abi_version(void) { return 10; }
+int hs_abi_version(void) { return HS_ABI_VERSION; }
 
 const char *hs_target_arch(void) { return "gfx950"; }
 

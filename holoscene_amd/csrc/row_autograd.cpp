@@ -37,7 +37,9 @@ struct Library {
     decltype(&hs_gated_mlp_bwd) gated_bwd;
 } lib = {};
 
-void bind(const py::dict &entries) {
+void bind(const py::dict &entries, int64_t abi_version) {
+    TORCH_CHECK(abi_version == HS_ABI_VERSION, "_row_autograd.so was built for ABI version ", HS_ABI_VERSION, " of libholoscene_hip.so, which has ", abi_version,
+                " -- rebuild (python -m holoscene_amd.csrc.build)");
     auto at = [&](const char *name) { return reinterpret_cast<void *>(entries[name].cast<uintptr_t>()); };
     lib.embed_fwd = reinterpret_cast<decltype(lib.embed_fwd)>(at("hs_embed_fwd"));
     lib.embed_bwd_ws_bytes = reinterpret_cast<decltype(lib.embed_bwd_ws_bytes)>(at("hs_embed_bwd_ws_bytes"));

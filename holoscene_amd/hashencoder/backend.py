@@ -224,7 +224,7 @@ def row_autograd():
         loader = importlib.machinery.ExtensionFileLoader("_row_autograd", path)
         module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_row_autograd", loader))
         loader.exec_module(module)
-        module.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _ROW_ENTRIES})
+        module.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _ROW_ENTRIES}, lib.hs_abi_version())
         _row_autograd = module
     return _row_autograd
 

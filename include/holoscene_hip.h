@@ -42,7 +42,8 @@ extern "C" {
 #define HS_F16 2        /* the row operators of section 10 only */
 
 /* ------------------------------------------------------------------ 0. library info */
-/* ABI version; bumped whenever a signature below changes. */
+/* ABI version; bumped whenever a signature or a structure below changes. */
+#define HS_ABI_VERSION 10
 int hs_abi_version(void);
 /* "gfx950" -- the only architecture this library is built for. */
 const char *hs_target_arch(void);

@@ -3,6 +3,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as fwd
 
+from holoscene_amd.hashencoder import backend
 from holoscene_amd.model import row_ops
 from test_row_ops_cpu import I64, gated, lib
 
@@ -84,3 +85,12 @@ def test_planes_refusals_and_sizes():
             row_ops.gated_mlp_rows(t, t, t, t.t(), planes=planes)
         with pytest.raises(ValueError, match="planes must be"):
             row_ops.GatedMLP(8, 16, planes=planes)
+
+
+# ------------------------------------------------------------------------------------------------ the two libraries
+def test_nodes_are_bound_to_their_own_abi_only():
+    nodes = backend.row_autograd()
+    assert lib().hs_abi_version() == backend.ABI_VERSION
+    for version in (backend.ABI_VERSION - 1, backend.ABI_VERSION + 1):
+        with pytest.raises(RuntimeError, match="ABI version"):
+            nodes.bind({}, version)
