@@ -194,7 +194,7 @@ __device__ __forceinline__ i32x4 descriptor(const void *p) {
     return i32x4{(int)__builtin_amdgcn_readfirstlane((int)(uint32_t)a), (int)__builtin_amdgcn_readfirstlane((int)((uint32_t)(a >> 32) & 0xffffu)), (int)kDescBytes, 0x00020000};
 }
 __device__ __forceinline__ void dma16(const i32x4 &desc, uint32_t voff, uint32_t to_lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to_lds), "v"(voff), "s"(desc) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to_lds), "v"(voff), "s"(desc) : "m0", "memory");
 }
 // everybody has this step's data (N of this wave's requests, for later steps, may still be under way) and is done with the previous step's
 template <int N> __device__ __forceinline__ void wait_and_meet() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
