@@ -6,6 +6,7 @@ import torch.autograd.forward_ad as fwd
 from holoscene_amd.hashencoder import backend
 from holoscene_amd.model import row_ops
 from test_row_ops_cpu import I64, gated, lib
+from test_row_ops_gpu import keep_reference
 
 
 def calls(t):
@@ -94,3 +95,14 @@ def test_nodes_are_bound_to_their_own_abi_only():
     for version in (backend.ABI_VERSION - 1, backend.ABI_VERSION + 1):
         with pytest.raises(RuntimeError, match="ABI version"):
             nodes.bind({}, version)
+
+
+# ------------------------------------------------------------------------------------------------ the oracles of the GPU tests
+def test_philox_known_answer_through_the_oracle():
+    """The published vector of Philox-4x32-10 (counter and key all ones -> 408f276d 41c83b0e a20bc7c6 6d5451fd) read out of keep_reference, which the kernel is
+    compared with: element e is kept at drop = u_e and not at u_e + 1."""
+    ones = (1 << 64) - 1
+    words = [0x408f276d, 0x41c83b0e, 0xa20bc7c6, 0x6d5451fd]
+    halves = [h for w in words for h in (w & 0xffff, w >> 16)]
+    for e, u in enumerate(halves):
+        assert bool(keep_reference(8, u, ones, ones, first=ones)[e]) and not bool(keep_reference(8, u + 1, ones, ones, first=ones)[e])
