@@ -287,3 +287,24 @@ def test_planes_of_the_module():
     y = [m(x) for m in mods]
     assert torch.equal(y[0], y[1]) and not torch.equal(y[1], y[2])
     assert all(torch.equal(y[k], ops().gated_mlp_rows(x, wg, wu, wd, "silu", planes=p)) for k, p in enumerate((None, 1, 2)))
+
+
+# ------------------------------------------------------------------------------------------------ what the backward pass reads
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,D,F", [(6, 8, 16), (70, 40, 100), (300, 1000, 130)])
+def test_a_kept_graph_gives_its_gradients_again(M, D, F, dtype):
+    """Nothing that the forward pass has kept is written by a backward pass; and it may be kept elsewhere in the meantime."""
+    x, wg, wu, wd, gy = gated_inputs(M, D, F, dtype)
+    wide = torch.cat([x, x], 1)[:, 1:D + 1]                                  # (rows of a wider tensor: another row distance when it comes back)
+    leaves = [t.detach().requires_grad_() for t in (wide, wg.t().contiguous().t(), wu, wd)]
+    rng, idx, table = torch.tensor([3, 4], device=DEV), torch.arange(M, device=DEV) % 5, x[:5].clone().requires_grad_()
+
+    def run():
+        rows = ops().dropout_rows(leaves[0], 0.2, rng, residual=ops().embedding_rows(idx, table))
+        return ops().gated_mlp_rows(rows, *leaves[1:])
+    y = run()
+    first = torch.autograd.grad(y, [*leaves, table], gy, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, torch.autograd.grad(y, [*leaves, table], gy)))
+    with torch.autograd.graph.save_on_cpu():
+        y = run()
+    assert all(torch.equal(a, b) for a, b in zip(first, torch.autograd.grad(y, [*leaves, table], gy)))
