@@ -5,7 +5,7 @@
 // call they, not the memory, would bound the 16-bit types; the probability is p to within 2^-17 and the scale is that of the t actually used, so
 // the expectation of y is exactly x.  The backward pass is the same launch on the gradient.  A dropped element is written as 0 (+ r_i) by
 // selection, not by a product: what it held -- an infinity, a NaN -- is not read into the result.
-// Bound by memory: 16 384 x 4 096 bf16 72 us with a residual (403 MB, 5.6 TB/s), 44 us without (268 MB, 6.1 TB/s; a large copy on the same card 5.0 TB/s).
+// Bound by memory: 16 384 x 4 096 bf16 74 us with a residual (403 MB, 5.4 TB/s), 45 us without (268 MB, 6.0 TB/s; a large copy on the same card 5.0 TB/s).
 #include "holoscene_hip.h"
 #include "philox.h"
 #include "row_types.h"

@@ -14,9 +14,9 @@
 //           of the zeros, most of the bytes, fill the memory's queues.
 // fp32 sums: 32 terms per chunk, then the partials; the last operation rounds to the table's type.
 //
-// Measured: 16 384 zipf-distributed rows of 2 048 bf16, table of 50 021: lookup 23.5 us (134 MB, 5.7 TB/s); gradient: sort 2 x (2.8 + 7.9), chunks and runs 12.6,
+// Measured: 16 384 zipf-distributed rows of 2 048 bf16, table of 50 021: lookup 22.6 us (134 MB, 5.9 TB/s); gradient: sort 2 x (2.9 + 7.8), chunks and runs 13.6,
 // rows 59 (205 MB of table written, 67 MB of gradient read: 54 us at the rate of a large copy).  131 072 rows of 32 fp32, 8 indices among 1 024: lookup 7.2, sort
-// 4.8 + 19.0 (one pass), chunks 9.9, rows 4.5.  The lookup and the rows are bound by memory, the sort by its chains of dependent LDS operations and launches.
+// 4.8 + 18.7 (one pass), chunks 9.8, rows 4.8.  The lookup and the rows are bound by memory, the sort by its chains of dependent LDS operations and launches.
 #include "holoscene_hip.h"
 #include "launch_util.h"
 #include "row_types.h"

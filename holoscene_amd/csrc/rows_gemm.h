@@ -9,18 +9,18 @@
 // Either operand may have K as its contiguous index ([rows, K], ld) or as its strided one ([K, rows], ld); all four products of the
 // block and its gradient are of that form, so nothing is ever transposed in memory.
 //
-// Workgroup = one BM x BN tile, K in steps of 64 through LDS, two buffers: step s + 1 is requested (LDS-DMA, 16 bytes a lane, no registers) before
-// step s is multiplied.  Chunks of 16 bytes are permuted on their way in (the DMA's LDS addresses are fixed, the lane's global address is free)
+// Workgroup = one BM x BN tile, K in steps of 64 through LDS, two to four buffers: one to three steps behind step s are requested (LDS-DMA, 16 bytes a lane, no
+// registers) before step s is multiplied.  Chunks of 16 bytes are permuted on their way in (the DMA's LDS addresses are fixed, the lane's global address is free)
 // so that every fragment read is free of bank conflicts without padding: K-contiguous tiles [rows][64] exchange chunk c of row r with c ^ (r & 7);
 // K-strided tiles [64][rows] exchange the 32-byte unit u of row k with u ^ (k & 3 | (k >> 3 & 1) << 2) and are read with the transposing
 // ds_read_b64_tr_b16.  What lies outside an operand is requested at an address beyond the buffer descriptor, which reads as zero.
 //
 // The tile's orientation in the matrix instruction is C^T (its rows = J): a lane then holds four consecutive columns of one row of C.
 //
-// Measured, 8 192 x 4 096 x 12 288 bf16 (256 x 256 tiles): gate and up 1.40 ms (1.18 PFLOP/s, with act(G) U and G, U written), down 0.67 (1.23), gx 1.30 (1.27), gWg and
-// gWu 1.35 (1.22), gWd 0.68 (1.21); the library's product of 8 192^3 reaches 1.40.  The matrix cores are busy 54 to 63 % of the cycles, the LDS 23 %, and the
+// Measured (medians of 30 passes), 8 192 x 4 096 x 12 288 bf16 (256 x 256 tiles): gate and up 1.41 ms (1.17 PFLOP/s, with act(G) U and G, U written), down 0.67 (1.23),
+// gx 1.30 (1.27), gWg and gWu 1.37 (1.20), gWd 0.69 (1.20); the library's product of 8 192^3 reaches 1.40.  The matrix cores are busy 54 to 63 % of the cycles, the LDS 23 %, and the
 // waves wait 30 % of theirs: what is left is the meeting of the waves at every step of 64.  At 131 072 x 256 x 1 024 a tile has four steps, and its beginning and end
-// are half of it: gate 217 us (0.63 PFLOP/s), down 82, gx 160, gWg and gWu 138, gWd 99.
+// are half of it: gate 224 us (0.61 PFLOP/s), down 86, gx 162, gWg and gWu 144, gWd 100.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -654,8 +654,8 @@ inline int launch_tile(Args p, int problems, hipStream_t s) {
 // ------------------------------------------------------------------------------------------------ gg and gu without G and U
 // gH = gy Wd, G = x Wg^T, U = x Wu^T over the same K = D in one workgroup: 4 D operations an element of H more than reading G and U back, 16 bytes less written
 // and read (fp32: 16-bit G and U would add two roundings to every gradient).  Tile 128 x 64 of each of the three, four waves, two workgroups a CU
-// (fp32: plane products as segments).  131 072 x 256 x 1 024: 370 us (0.56 PFLOP/s; matrix cores 25 % of the cycles, vector units 43 %, LDS 24 %; without the
-// stores 321).  Larger tiles read less and were slower: with K this short half the time is the beginnings and the ends of tiles, and a second workgroup
+// (fp32: plane products as segments).  131 072 x 256 x 1 024: 389 us (0.53 PFLOP/s, median; least 361; matrix cores 25 % of the cycles, vector units 43 %, LDS 24 %).
+// As least times: 370, without the stores 321.  Larger tiles read less and were slower: with K this short half the time is the beginnings and the ends of tiles, and a second workgroup
 // is what fills them (128 x 128 435, 256 x 64 435, 256 x 128 413, 64 x 64 423; eight waves 366, no gain for twice the LDS reads).
 constexpr int kAgainM = 128, kAgainJ = 64;
 
@@ -734,7 +734,7 @@ __global__ __launch_bounds__(256) void k_gate_bwd(const Args p) {
         buf ^= 1;
     }
     // A lane has G, U and gH of the same elements: gg and gu are computed where they are, rounded, and only then pass through LDS, so that full lines of global
-    // memory are written (131 072 x 256 x 1 024: 369 us; G, U and gH in fp32 through LDS: 381)
+    // memory are written (131 072 x 256 x 1 024, least times: 369 us; G, U and gH in fp32 through LDS: 381)
     using St = Staging<U, 2 * TJ, TJ, MT, WI, WAVES, MT, 2 * (int)kBuf>;
     const int li = lane & 15, lq = lane >> 4;
     if (j0 + TJ > p.J) {        // (uniform)

@@ -5,7 +5,7 @@
 // consecutive bytes).  The weights are the instruction's A: a lane ends with four consecutive results of one row of x.  The waves' partial sums meet in
 // LDS in the order of the waves.  Any row distance and alignment is read in place -- a copy of an unaligned weight would cost more than the product.
 // fp32: each operand is split into its three planes in registers.
-// Bound by reading the weights: 1 x 4 096 x 12 288 bf16 37.4 us (gate and up, 201 MB, 5.4 TB/s) and 20.5 us (down, 101 MB, 4.9 TB/s); 13 x 1 000 x 2 730 f16 6.0 and 5.8 us (16 MB: latency).
+// Bound by reading the weights: 1 x 4 096 x 12 288 bf16 37.3 us (gate and up, 201 MB, 5.4 TB/s) and 20.2 us (down, 101 MB, 5.0 TB/s); 13 x 1 000 x 2 730 f16 6.1 and 5.8 us (16 MB: latency).
 #pragma once
 #include "rows_gemm.h"
 
